@@ -323,6 +323,60 @@ int msl_attention_fp8_split(const void* q8, const void* k_cache, const void* v_c
                             int64_t ld_out, const void* gate, int64_t ld_gate, int kv_splits, void* workspace,
                             int* status, void* stream);
 
+/* ---- The K/V cache held in 4 bits.  Channels [16 i, 16 i + 16) of a (row, head) share one E4M3 scale s; an
+ * element is an E2M1 code c (0, .5, 1, 1.5, 2, 3, 4, 6 with a sign; element 2i in the low nibble of byte i: the
+ * grid and nibble order of the reference's expert weights, nvfp4.py:24-47) and stands for c * s * scale with one
+ * fp32 scale for the keys and one for the values.  Codes u8 [cache_rows, hkv, head_dim / 2], scales e4m3
+ * [cache_rows, hkv, head_dim / 16]: 4.5 bits an element, a little over half of the FP8 cache.  The reference caches
+ * FP8 only (submission.py:740-785) and has no counterpart to these five calls.
+ *
+ * msl_page_plan: one step's pages, positions and cache slots from the request lengths, on the device.  Request b
+ * holds ceil(seq_lens[b] / page_size) pages in its row of page_table [batch, max_pages] and adds new_lens[b]
+ * tokens; the pages it lacks are taken in request order from free_pages [n_free], starting at *free_head, and
+ * entered into its row; no other entry is written.  cu_seqlens_q [batch + 1] is the exclusive prefix sum of
+ * new_lens, positions [tokens] and cache_loc [tokens] (page * page_size + position % page_size) list the new tokens
+ * request by request; entries behind the last request get position 0 and cache_loc -1 (a padded buffer).
+ * *free_head_out = *free_head + pages taken (another word than free_head; a page list that is a ring is the caller's
+ * affair).  MSL_ERR_CAPACITY goes to *status when the free list or a table row runs out (the tokens concerned get
+ * cache_loc -1, the table entries -1), when the new tokens outnumber `tokens` (the rest is left out) or when a length
+ * is negative (it counts as 0).  batch <= 16384. */
+int msl_page_plan(const int* new_lens, const int* seq_lens, int* page_table, int max_pages, const int* free_pages,
+                  int n_free, const int* free_head, int* free_head_out, int batch, int page_size, int tokens,
+                  int* cu_seqlens_q, int64_t* positions, int64_t* cache_loc, int* status, void* stream);
+
+/* msl_qk_rope_store for the 4-bit cache: the same norm and rotation of q and k; q -> bf16 [tokens, hq, head_dim];
+ * k and v -> codes and scales of row cache_loc[t].  For each block of 16
+ *   s = e4m3(min(448, max|z| / (6 * scale))),  c = e2m1(z / (s * scale)),
+ * to nearest, ties to even, decided on values held in 64 bits; a block whose s is 0 gets zero codes.  Infinities and
+ * NaN of k and v have no code: they count as +-2^128 or a little above and saturate.  A negative cache_loc marks a
+ * padding token (nothing is stored, nothing reported); one at or beyond cache_rows is skipped and reported in
+ * *status.  No two tokens may share a row.  head_dim 64 or 128. */
+int msl_qk_rope_store_kv4(const void* qkv, int64_t ld, const int64_t* positions, const int64_t* cache_loc,
+                          const float* inv_freq, const float* k_scale, const float* v_scale, void* q, void* k_cache,
+                          void* k_sf, void* v_cache, void* v_sf, int tokens, int hq, int hkv, int head_dim,
+                          int64_t cache_rows, int* status, void* stream);
+
+/* Read-back: out[i, :] = the values of cache row rows[i], i < n, for rows of `width` = hkv * head_dim elements
+ * (out_mode MSL_OUT_BF16 or MSL_OUT_F32; rounded once from fp32).  A negative row gives zeros; one at or beyond
+ * cache_rows gives zeros and MSL_ERR_CAPACITY in *status. */
+int msl_kv4_rows(const void* codes, const void* scales, const float* scale, const int64_t* rows, int64_t n, int width,
+                 int64_t cache_rows, int out_mode, void* out, int* status, void* stream);
+
+/* msl_attention_fp8 over the 4-bit cache: the same masks, paging and epilogue, queries in bf16 [tokens, hq,
+ * head_dim] with row pitch ld_q, any number of query heads per KV head up to 128.  max_q_len is the longest
+ * request's number of new tokens (rows beyond it, and rows behind the last request, are left as they are).  A page
+ * table entry that is negative, beyond the cache or missing (past max_pages) hides its keys and is reported in
+ * *status; a row that sees no key is zero.  Scale bytes 0x7f and 0xff (NaN, never stored) read as 448.  The cache
+ * must hold fewer than 2^31 rows.  `workspace`: msl_attention_kv4_workspace bytes of caller-owned device memory,
+ * 16-byte aligned, no initialisation; calls that overlap on the GPU need one each. */
+int64_t msl_attention_kv4_workspace(int batch, int max_q_len, int hq, int hkv, int head_dim);
+int msl_attention_kv4(const void* q, int64_t ld_q, const void* k_cache, const void* k_sf, const void* v_cache,
+                      const void* v_sf, const int* page_table, int max_pages, const int* seq_lens,
+                      const int* cu_seqlens_q, const float* k_scale, const float* v_scale, float softmax_scale,
+                      int batch, int max_q_len, int tokens, int hq, int hkv, int head_dim, int page_size, int window,
+                      int64_t cache_rows, void* out, int64_t ld_out, const void* gate, int64_t ld_gate,
+                      void* workspace, int64_t workspace_bytes, int* status, void* stream);
+
 /* Measured ceiling of one tensor-core instruction shape: every SM issues `iters` tcgen05.mma of
  * M = 128 x N = n back to back on operands resident in shared memory (kind 0: bf16, K = 16; 1: e4m3,
  * K = 32; 2: NVFP4 block scaled, K = 64), no loads and no epilogue.  The caller times the launch

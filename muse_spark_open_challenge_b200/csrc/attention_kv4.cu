@@ -1,0 +1,671 @@
+// Causal varlen attention over the paged 4-bit K/V cache (format: csrc/kv4.cu), few query rows per KV head:
+// decode steps, verify blocks.
+//
+// A worker (one CTA of four warps) owns an equal share of all key tiles of the batch: the tiles of every
+// (request, block of R query rows, KV head) are laid end to end and cut into `workers` equal ranges, so ragged
+// lengths cost nothing.  A range that covers all tiles of a work item writes its rows; the others leave
+// (O, maximum, sum) in the workspace and kv4_merge_kernel joins them.  The ranges follow from the lengths, which
+// live on the device: both kernels form the same sums, no host knows them.
+//
+// Each warp takes 32 of a tile's 128 keys straight from global memory into registers, in the layout of the
+// MMA operands.  The contraction index of Q K^T and the row index of O^T may be permuted freely, and the
+// permutation is chosen so that a lane's share is contiguous in memory:
+//   S^T[key][q] = K Q^T   lane (g, t) holds channels [D/4 t, D/4 (t+1)) of keys g and g + 8: one 16-byte load
+//                         (8 at head_dim 64), whose elements lie in at most two scale blocks
+//   O^T[d][q]  += V^T P^T lane (g, t) holds channels [D/8 g, D/8 (g+1)) of keys 2t, 2t+1, 2t+8, 2t+9: one
+//                         8-byte load a key (4), which lies in one scale block; the low nibbles are MMA row g,
+//                         the high ones row g + 8
+// Codes become f16 by the e2m1 conversion, times their block scale: exact (2 + 4 significant bits).  P^T moves
+// from the accumulator's layout to the operand's by one 8 x 8 transpose in registers.  Queries (bf16) are scaled by
+// a power of two per row so that the largest magnitude lies in [2^14, 2^15) and held in f16: exact for every
+// element within 2^28 of the row's largest.  P is f16 (2^-12 relative), statistics and O are fp32.
+#include <cuda_fp16.h>
+
+#include "msl_common.cuh"
+#include "msl_host.h"
+
+namespace msl {
+
+constexpr int kKvWarps = 4;
+constexpr int kKvTile = 32 * kKvWarps;     // keys of a tile
+constexpr float kKvTau = 8.0f;             // the running maximum may lag by 2^8: P stays within f16
+
+struct Kv4Args {
+  const __nv_bfloat16* q;       // [tokens][hq][D], row pitch ld_q
+  int64_t ld_q;
+  const uint8_t *k, *ks, *v, *vs;
+  const int* page_table;        // [batch][max_pages]
+  int max_pages;
+  const int* seq_lens;
+  const int* cu_seqlens_q;
+  const float* k_scale;
+  const float* v_scale;
+  float softmax_scale;
+  int batch, max_q_len, tokens, hq, hkv, page_size, window;
+  int64_t cache_rows;
+  __nv_bfloat16* out;
+  int64_t ld_out;
+  const __nv_bfloat16* gate;
+  int64_t ld_gate;
+  float* part;                  // [workers][2][R][D + 2]
+  int workers;
+  int* status;
+};
+
+// A request as the schedule sees it: q rows [begin, begin + len), `seq` cached tokens.
+struct Kv4Req {
+  int begin, len, seq;
+};
+__device__ __forceinline__ Kv4Req kv4_request(const Kv4Args& p, int b) {
+  Kv4Req r;
+  r.begin = max(0, min(p.cu_seqlens_q[b], p.tokens));
+  const int end = max(r.begin, min(p.cu_seqlens_q[b + 1], p.tokens));
+  r.len = min(end - r.begin, p.max_q_len);
+  r.seq = p.seq_lens[b];
+  return r;
+}
+// Key tiles [first, last) that rows [R i, R (i + 1)) of a request's len * G rows can see.
+struct Kv4Span {
+  int first, last;
+};
+template <int R>
+__device__ __forceinline__ Kv4Span kv4_span(const Kv4Args& p, const Kv4Req& r, int G, int i) {
+  const int last_tok = min(r.len - 1, (R * i + R - 1) / G);
+  const int low_tok = R * i / G;
+  // keys past the table's row have no page: they are not walked (the kernel reports them)
+  const int hi = static_cast<int>(min(static_cast<int64_t>(r.seq) + last_tok + 1,
+                                      static_cast<int64_t>(p.max_pages) * p.page_size));
+  const int lo = p.window ? max(0, r.seq + low_tok - p.window + 1) : 0;
+  Kv4Span s;
+  s.first = lo / kKvTile;
+  s.last = max(s.first + 1, (hi + kKvTile - 1) / kKvTile);   // a row block with nothing to see still writes its zeros
+  return s;
+}
+template <int R>
+__device__ __forceinline__ int64_t kv4_tiles(const Kv4Args& p, const Kv4Req& r, int G) {
+  const int blocks = (r.len * G + R - 1) / R;
+  int64_t sum = 0;
+  for (int i = 0; i < blocks; ++i) {
+    const Kv4Span s = kv4_span<R>(p, r, G, i);
+    sum += s.last - s.first;
+  }
+  return sum * p.hkv;
+}
+
+__device__ __forceinline__ int64_t block_sum_i64(int64_t v, int64_t* scratch) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = v;
+  __syncthreads();
+  int64_t s = 0;
+  for (int w = 0; w < kKvWarps; ++w) s += scratch[w];
+  __syncthreads();
+  return s;
+}
+
+__device__ __forceinline__ uint32_t h2_bits(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
+__device__ __forceinline__ __half2 bits_h2(uint32_t u) { return *reinterpret_cast<__half2*>(&u); }
+__device__ __forceinline__ float kv_ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// The four bytes of a word, each a pair of e2m1 codes -> f16x2 (low nibble in the low half).
+__device__ __forceinline__ void e2m1x8(uint32_t w, __half2 (&h)[4]) {
+  uint32_t a, b, c, d;
+  asm("{.reg .b8 x, y, z, u;\n\tmov.b32 {x, y, z, u}, %4;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %0, x;\n\tcvt.rn.f16x2.e2m1x2 %1, y;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %2, z;\n\tcvt.rn.f16x2.e2m1x2 %3, u;}"
+      : "=r"(a), "=r"(b), "=r"(c), "=r"(d) : "r"(w));
+  h[0] = bits_h2(a); h[1] = bits_h2(b); h[2] = bits_h2(c); h[3] = bits_h2(d);
+}
+// Two e4m3 scales -> f16x2.  The NaN codes (never written by the store) read as 448: a NaN would reach rows that
+// do not see the key, as 0 * NaN in P V.
+__device__ __forceinline__ __half2 scales_h2(uint32_t two) {
+  uint32_t h;
+  asm("{.reg .b16 x;\n\tcvt.u16.u32 x, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, x;}" : "=r"(h) : "r"(two));
+  return __hmin2(bits_h2(h), __half2half2(__ushort_as_half(0x5F00)));   // 448
+}
+__device__ __forceinline__ void mma_16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                          uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+      "{%0, %1, %2, %3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
+  uint32_t o;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(o) : "r"(v));
+  return o;
+}
+
+// One lane's share of 16 keys, as loaded.
+template <int D>
+struct Kv4Frag {
+  static constexpr int KW = D / 32;        // words of K codes per key (D / 4 channels)
+  static constexpr int VW = D / 64;        // words of V codes per key (D / 8 channels)
+  uint32_t k[2][KW], v[4][VW];
+  uint32_t ks[2], vs[4];
+};
+
+template <int D>
+__device__ __forceinline__ void kv4_load(Kv4Frag<D>& f, const Kv4Args& p, int kvh, int rows, int half, int lane) {
+  const int g = lane >> 2, t = lane & 3;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int row = __shfl_sync(0xffffffffu, rows, 16 * half + g + 8 * i);
+    const int64_t at = static_cast<int64_t>(row) * p.hkv + kvh;
+    f.ks[i] = 0;
+#pragma unroll
+    for (int w = 0; w < Kv4Frag<D>::KW; ++w) f.k[i][w] = 0;
+    if (row >= 0) {
+      if constexpr (D == 128) {
+        const uint4 c = *reinterpret_cast<const uint4*>(p.k + at * 64 + t * 16);
+        f.k[i][0] = c.x; f.k[i][1] = c.y; f.k[i][2] = c.z; f.k[i][3] = c.w;
+        f.ks[i] = *reinterpret_cast<const uint16_t*>(p.ks + at * 8 + t * 2);
+      } else {
+        const uint2 c = *reinterpret_cast<const uint2*>(p.k + at * 32 + t * 8);
+        f.k[i][0] = c.x; f.k[i][1] = c.y;
+        f.ks[i] = p.ks[at * 4 + t];
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int row = __shfl_sync(0xffffffffu, rows, 16 * half + 2 * t + (i & 1) + 8 * (i >> 1));
+    const int64_t at = static_cast<int64_t>(row) * p.hkv + kvh;
+    f.vs[i] = 0;
+#pragma unroll
+    for (int w = 0; w < Kv4Frag<D>::VW; ++w) f.v[i][w] = 0;
+    if (row >= 0) {
+      if constexpr (D == 128) {
+        const uint2 c = *reinterpret_cast<const uint2*>(p.v + at * 64 + g * 8);
+        f.v[i][0] = c.x; f.v[i][1] = c.y;
+        f.vs[i] = p.vs[at * 8 + g];
+      } else {
+        f.v[i][0] = *reinterpret_cast<const uint32_t*>(p.v + at * 32 + g * 4);
+        f.vs[i] = p.vs[at * 4 + g / 2];
+      }
+    }
+  }
+}
+
+// The cache row of key `key` (-1: hidden from every row of the block, or no valid page).
+__device__ __forceinline__ int kv4_row(const Kv4Args& p, const int* table, int key, int lo, int hi) {
+  if (key < lo || key >= hi) return -1;
+  const int idx = key / p.page_size;
+  const int page = idx < p.max_pages ? table[idx] : -1;
+  const int64_t row = static_cast<int64_t>(page) * p.page_size + (key - idx * p.page_size);
+  if (page < 0 || row >= p.cache_rows) {
+    report_error(p.status, MSL_ERR_CAPACITY);
+    return -1;
+  }
+  return static_cast<int>(row);
+}
+
+// Shared-memory layout of a warp's O [R][D]: channel d of the lane group D/8 at pitch D/8 + 2, so that the float2
+// stores of a warp (8 groups x 4 row pairs) fall into different banks.
+template <int D>
+struct Kv4Merge {
+  static constexpr int kGroup = D / 8 + 2;
+  static constexpr int kRow = 8 * kGroup + 8;
+};
+
+// Rows of a finished block: O / l, v_scale, optional per-head RMS norm * sigmoid(gate), bf16.  One warp per row,
+// lane holds channels [D/32 lane, ...).
+template <int D>
+__device__ __forceinline__ void kv4_write_row(const Kv4Args& p, float (&o)[D / 32], float l, int64_t token, int head,
+                                              int lane) {
+  constexpr int PER = D / 32;
+  const float c = l > 0.f ? *p.v_scale / l : 0.f;          // a row that sees nothing is zero
+  // a NaN sum (a NaN query) must stay visible
+  const float scale = l != l ? l : c;
+  float ss = 0.f;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) { o[i] *= scale; ss += o[i] * o[i]; }
+  if (p.gate != nullptr) {
+    const float r = 1.0f / sqrtf(warp_sum(ss) / D + 1e-5f);
+    const __nv_bfloat16* grow = p.gate + token * p.ld_gate + head * D + lane * PER;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) o[i] *= r / (1.0f + __expf(-__bfloat162float(grow[i])));
+  }
+  __nv_bfloat16* orow = p.out + token * p.ld_out + head * D + lane * PER;
+#pragma unroll
+  for (int i = 0; i < PER; i += 2) *reinterpret_cast<uint32_t*>(orow + i) = pack_bf16x2(o[i], o[i + 1]);
+}
+
+template <int D, int NB>
+__global__ void __launch_bounds__(32 * kKvWarps)
+attention_kv4_kernel(Kv4Args p) {
+  constexpr int R = 8 * NB;
+  constexpr int KS = D / 16;               // MMA steps of Q K^T, and 16-row tiles of O^T
+  using M = Kv4Merge<D>;
+  __shared__ float sm_o[kKvWarps][R][M::kRow];
+  __shared__ float sm_m[kKvWarps][R], sm_l[kKvWarps][R];
+  __shared__ int64_t scratch[kKvWarps];
+  __shared__ int sm_b;
+  __shared__ int64_t sm_at;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+  const int G = p.hq / p.hkv;
+
+  // ---- this worker's range of tiles
+  const int per = (p.batch + blockDim.x - 1) / blockDim.x;
+  const int b0 = min(tid * per, p.batch), b1 = min(b0 + per, p.batch);
+  int64_t mine = 0;
+  for (int b = b0; b < b1; ++b) mine += kv4_tiles<R>(p, kv4_request(p, b), G);
+  int64_t inc = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t a = __shfl_up_sync(0xffffffffu, inc, o);
+    if (lane >= o) inc += a;
+  }
+  if (lane == 31) scratch[warp] = inc;
+  __syncthreads();
+  int64_t total = 0;
+  for (int w = 0; w < kKvWarps; ++w) {
+    if (w < warp) inc += scratch[w];
+    total += scratch[w];
+  }
+  const int64_t workers = min(static_cast<int64_t>(p.workers), total);   // no empty range in between
+  if (blockIdx.x >= workers) return;                        // uniform
+  int64_t at = total * blockIdx.x / workers;
+  const int64_t end = total * (blockIdx.x + 1) / workers;
+  if (inc - mine <= at && at < inc) {                       // one thread: walk its few requests
+    int64_t base = inc - mine;
+    int b = b0;
+    for (; b < b1 - 1; ++b) {
+      const int64_t n = kv4_tiles<R>(p, kv4_request(p, b), G);
+      if (at < base + n) break;
+      base += n;
+    }
+    sm_b = b;
+    sm_at = base;
+  }
+  __syncthreads();
+  int b = sm_b;
+  int64_t skip = at - sm_at;                                // tiles of request b before this range
+  const float scale_log2 = p.softmax_scale * (*p.k_scale) * 1.4426950408889634f;
+
+  for (; at < end && b < p.batch; ++b) {
+    const Kv4Req r = kv4_request(p, b);
+    const int blocks = (r.len * G + R - 1) / R;
+    const int* table = p.page_table + static_cast<int64_t>(b) * p.max_pages;
+    for (int i = 0; i < blocks && at < end; ++i) {
+      const Kv4Span span = kv4_span<R>(p, r, G, i);
+      const int n_span = span.last - span.first;
+      if (skip >= static_cast<int64_t>(n_span) * p.hkv) { skip -= static_cast<int64_t>(n_span) * p.hkv; continue; }
+      for (int kvh = static_cast<int>(skip / n_span); kvh < p.hkv && at < end; ++kvh) {
+        const int off = static_cast<int>(skip % n_span);
+        skip = 0;
+        const int n = static_cast<int>(min(end - at, static_cast<int64_t>(n_span - off)));
+        // ---- rows of the block: row = token * G + head in group
+        const int rows = min(R, r.len * G - i * R);
+        const int last_tok = (i * R + rows - 1) / G;
+        const int hi = r.seq + last_tok + 1;                // keys [lo, hi) are visible to some row
+        const int lo = p.window ? max(0, r.seq + i * R / G - p.window + 1) : 0;
+        if (tid == 0 && hi > static_cast<int64_t>(p.max_pages) * p.page_size) report_error(p.status, MSL_ERR_CAPACITY);
+        const int all_lo = p.window ? max(0, r.seq + last_tok - p.window + 1) : 0;   // keys [all_lo, all_hi) to all
+        const int all_hi = r.seq + i * R / G + 1;
+        uint32_t qf[NB][KS][2];
+        float qs[NB][2];                                    // log2 scale of columns 2t, 2t + 1
+        int qpos[NB][2];
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) {
+          const int row = nb * 8 + g;
+          uint32_t raw[KS * 2];
+#pragma unroll
+          for (int w = 0; w < KS * 2; ++w) raw[w] = 0;
+          if (row < rows) {
+            const int tok = (i * R + row) / G, head = kvh * G + (i * R + row) % G;
+            const uint4* src = reinterpret_cast<const uint4*>(p.q + (static_cast<int64_t>(r.begin) + tok) * p.ld_q +
+                                                              head * D + t * (D / 4));
+#pragma unroll
+            for (int w = 0; w < KS / 2; ++w) {
+              const uint4 x = src[w];
+              raw[4 * w] = x.x; raw[4 * w + 1] = x.y; raw[4 * w + 2] = x.z; raw[4 * w + 3] = x.w;
+            }
+          }
+          uint32_t mx = 0;                                  // largest magnitude as bits (NaN and infinity on top)
+#pragma unroll
+          for (int w = 0; w < KS * 2; ++w) mx = max(mx, max(raw[w] & 0x7fffu, (raw[w] >> 16) & 0x7fffu));
+          mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+          mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+          // 2^(141 - e) takes the exponent e to 141 = 127 + 14; its inverse goes into the row's score scale
+          const int e = min(max(static_cast<int>(mx >> 7), 16), 254);
+          const float up = __uint_as_float(static_cast<uint32_t>(127 + 141 - e) << 23);
+          const float down = scale_log2 / up;
+#pragma unroll
+          for (int w = 0; w < KS * 2; ++w)
+            qf[nb][w / 2][w & 1] = h2_bits(__floats2half2_rn(bf16_bits_to_f32(raw[w] & 0xffffu) * up,
+                                                             bf16_bits_to_f32(raw[w] >> 16) * up));
+          qs[nb][0] = __shfl_sync(0xffffffffu, down, 8 * t);         // lane (g = 2t, 0) holds row 2t
+          qs[nb][1] = __shfl_sync(0xffffffffu, down, 8 * t + 4);
+#pragma unroll
+          for (int c = 0; c < 2; ++c) qpos[nb][c] = r.seq + (i * R + nb * 8 + 2 * t + c) / G;
+        }
+        float o[NB][KS][4], m[NB][2], l[NB][2];
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) {
+#pragma unroll
+          for (int c = 0; c < 2; ++c) { m[nb][c] = -INFINITY; l[nb][c] = 0.f; }
+#pragma unroll
+          for (int k = 0; k < KS; ++k)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) o[nb][k][c] = 0.f;
+        }
+        // ---- the keys, 32 a step
+        const int key_first = (span.first + off) * kKvTile + warp * 32;
+        int row_cur = kv4_row(p, table, key_first + lane, lo, hi);
+        Kv4Frag<D> f[2];
+        kv4_load<D>(f[0], p, kvh, row_cur, 0, lane);
+        kv4_load<D>(f[1], p, kvh, row_cur, 1, lane);
+        int row_next = n > 1 ? kv4_row(p, table, key_first + kKvTile + lane, lo, hi) : -1;
+        for (int j = 0; j < n; ++j) {
+          const int key0 = key_first + j * kKvTile;
+          const bool partial = __any_sync(0xffffffffu, row_cur < 0) || key0 < all_lo || key0 + 32 > all_hi;
+          uint32_t vmem[2][4][Kv4Frag<D>::VW];
+          uint32_t vsc[2][4];
+          float s[2][NB][4];
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+              for (int c = 0; c < 4; ++c) s[h][nb][c] = 0.f;
+            __half2 sc[2];
+#pragma unroll
+            for (int x = 0; x < 2; ++x) sc[x] = scales_h2(f[h].ks[x]);
+#pragma unroll
+            for (int w = 0; w < Kv4Frag<D>::KW; ++w) {      // one word = two MMA steps
+              __half2 a[4], c[4];
+              e2m1x8(f[h].k[0][w], a);
+              e2m1x8(f[h].k[1][w], c);
+              const bool second = D == 128 && w >= 2;       // which of the lane's two scale blocks
+              const __half2 s0 = second ? __high2half2(sc[0]) : __low2half2(sc[0]);
+              const __half2 s1 = second ? __high2half2(sc[1]) : __low2half2(sc[1]);
+#pragma unroll
+              for (int x = 0; x < 4; ++x) { a[x] = __hmul2(a[x], s0); c[x] = __hmul2(c[x], s1); }
+#pragma unroll
+              for (int nb = 0; nb < NB; ++nb) {
+                mma_16816(s[h][nb], h2_bits(a[0]), h2_bits(c[0]), h2_bits(a[1]), h2_bits(c[1]), qf[nb][2 * w][0],
+                          qf[nb][2 * w][1]);
+                mma_16816(s[h][nb], h2_bits(a[2]), h2_bits(c[2]), h2_bits(a[3]), h2_bits(c[3]), qf[nb][2 * w + 1][0],
+                          qf[nb][2 * w + 1][1]);
+              }
+            }
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+              vsc[h][x] = f[h].vs[x];
+#pragma unroll
+              for (int w = 0; w < Kv4Frag<D>::VW; ++w) vmem[h][x][w] = f[h].v[x][w];
+            }
+          }
+          const int row_was = row_cur;
+          if (j + 1 < n) {                                  // the next 32 keys are on their way during the rest
+            row_cur = row_next;
+            kv4_load<D>(f[0], p, kvh, row_cur, 0, lane);
+            kv4_load<D>(f[1], p, kvh, row_cur, 1, lane);
+            row_next = j + 2 < n ? kv4_row(p, table, key0 + 2 * kKvTile + lane, lo, hi) : -1;
+          }
+          // ---- scores in log2 units, masked where some row does not see a key
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+              for (int c = 0; c < 4; ++c) s[h][nb][c] *= qs[nb][c & 1];
+          if (partial) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+              for (int x = 0; x < 2; ++x) {
+                const int kk = 16 * h + g + 8 * x;
+                const bool held = __shfl_sync(0xffffffffu, row_was, kk) >= 0;
+#pragma unroll
+                for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                  for (int c = 0; c < 2; ++c) {
+                    const int key = key0 + kk;
+                    const bool seen = held && key <= qpos[nb][c] && (!p.window || key > qpos[nb][c] - p.window);
+                    if (!seen) s[h][nb][2 * x + c] = -INFINITY;
+                  }
+              }
+          }
+          // ---- running maximum: it moves when a row of the warp exceeds it by more than 2^tau
+          float top[NB][2];
+          bool move = false;
+#pragma unroll
+          for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              float x = fmaxf(fmaxf(s[0][nb][c], s[0][nb][2 + c]), fmaxf(s[1][nb][c], s[1][nb][2 + c]));
+              top[nb][c] = x;
+              move |= x > m[nb][c] + kKvTau || (m[nb][c] == -INFINITY && x > -INFINITY);
+            }
+          if (__any_sync(0xffffffffu, move)) {
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+              for (int c = 0; c < 2; ++c) {
+                float x = top[nb][c];
+#pragma unroll
+                for (int d = 4; d < 32; d <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, d));
+                const float new_m = fmaxf(m[nb][c], x);
+                const float corr = kv_ex2(m[nb][c] - (new_m == -INFINITY ? 0.f : new_m));
+                m[nb][c] = new_m;
+                l[nb][c] *= corr;
+#pragma unroll
+                for (int k = 0; k < KS; ++k) { o[nb][k][c] *= corr; o[nb][k][2 + c] *= corr; }
+              }
+          }
+          uint32_t pf[2][NB][2];
+#pragma unroll
+          for (int nb = 0; nb < NB; ++nb) {
+            const float n0 = m[nb][0] == -INFINITY ? 0.f : m[nb][0], n1 = m[nb][1] == -INFINITY ? 0.f : m[nb][1];
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+              for (int x = 0; x < 2; ++x) {
+                const float e0 = kv_ex2(s[h][nb][2 * x] - n0), e1 = kv_ex2(s[h][nb][2 * x + 1] - n1);
+                l[nb][0] += e0;
+                l[nb][1] += e1;
+                pf[h][nb][x] = transpose8x8(h2_bits(__floats2half2_rn(e0, e1)));
+              }
+          }
+          // ---- O^T += V^T P^T
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const __half2 s01 = scales_h2(vsc[h][0] | (vsc[h][1] << 8));
+            const __half2 s23 = scales_h2(vsc[h][2] | (vsc[h][3] << 8));
+#pragma unroll
+            for (int w = 0; w < Kv4Frag<D>::VW; ++w) {      // one word a key = four 16-row tiles
+              // pairs along the keys: low nibbles (even channels, MMA rows g) and high ones (odd, g + 8)
+              const uint32_t lo01 = (vmem[h][0][w] & 0x0f0f0f0fu) | ((vmem[h][1][w] << 4) & 0xf0f0f0f0u);
+              const uint32_t hi01 = ((vmem[h][0][w] >> 4) & 0x0f0f0f0fu) | (vmem[h][1][w] & 0xf0f0f0f0u);
+              const uint32_t lo23 = (vmem[h][2][w] & 0x0f0f0f0fu) | ((vmem[h][3][w] << 4) & 0xf0f0f0f0u);
+              const uint32_t hi23 = ((vmem[h][2][w] >> 4) & 0x0f0f0f0fu) | (vmem[h][3][w] & 0xf0f0f0f0u);
+              __half2 a0[4], a1[4], a2[4], a3[4];
+              e2m1x8(lo01, a0);
+              e2m1x8(hi01, a1);
+              e2m1x8(lo23, a2);
+              e2m1x8(hi23, a3);
+#pragma unroll
+              for (int x = 0; x < 4; ++x) {
+                const uint32_t u0 = h2_bits(__hmul2(a0[x], s01)), u1 = h2_bits(__hmul2(a1[x], s01));
+                const uint32_t u2 = h2_bits(__hmul2(a2[x], s23)), u3 = h2_bits(__hmul2(a3[x], s23));
+#pragma unroll
+                for (int nb = 0; nb < NB; ++nb)
+                  mma_16816(o[nb][4 * w + x], u0, u1, u2, u3, pf[h][nb][0], pf[h][nb][1]);
+              }
+            }
+          }
+        }
+        // ---- join the four warps
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) {
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            float x = l[nb][c];
+#pragma unroll
+            for (int d = 4; d < 32; d <<= 1) x += __shfl_xor_sync(0xffffffffu, x, d);
+            const int row = nb * 8 + 2 * t + c;
+            if (g == 0) { sm_m[warp][row] = m[nb][c]; sm_l[warp][row] = x; }
+#pragma unroll
+            for (int k = 0; k < KS; ++k)
+              *reinterpret_cast<float2*>(&sm_o[warp][row][g * M::kGroup + 2 * k]) =
+                  make_float2(o[nb][k][c], o[nb][k][2 + c]);
+          }
+        }
+        __syncthreads();
+        const bool whole = n == n_span;
+        // a worker has at most two partial results: the rest of an item that an earlier worker began (slot 0) and
+        // the beginning of one that a later worker ends (slot 1)
+        float* part = p.part + (static_cast<int64_t>(blockIdx.x) * 2 + (off == 0 ? 1 : 0)) * R * (D + 2);
+        for (int row = warp; row < rows; row += kKvWarps) {
+          float mx = -INFINITY;
+#pragma unroll
+          for (int w = 0; w < kKvWarps; ++w) mx = fmaxf(mx, sm_m[w][row]);
+          float acc[D / 32], sum = 0.f;
+#pragma unroll
+          for (int x = 0; x < D / 32; ++x) acc[x] = 0.f;
+#pragma unroll
+          for (int w = 0; w < kKvWarps; ++w) {
+            const float c = kv_ex2(sm_m[w][row] - (mx == -INFINITY ? 0.f : mx));
+            sum += sm_l[w][row] * c;
+#pragma unroll
+            for (int x = 0; x < D / 32; ++x) {
+              const int d = lane * (D / 32) + x;
+              acc[x] += sm_o[w][row][(d / (D / 8)) * M::kGroup + d % (D / 8)] * c;
+            }
+          }
+          if (whole) {
+            const int tok = (i * R + row) / G, head = kvh * G + (i * R + row) % G;
+            kv4_write_row<D>(p, acc, sum, static_cast<int64_t>(r.begin) + tok, head, lane);
+          } else {
+            float* dst = part + row * (D + 2);
+            if (lane == 0) { dst[0] = mx; dst[1] = sum; }
+#pragma unroll
+            for (int x = 0; x < D / 32; x += 2)
+              *reinterpret_cast<float2*>(dst + 2 + lane * (D / 32) + x) = make_float2(acc[x], acc[x + 1]);
+          }
+        }
+        __syncthreads();
+        at += n;
+      }
+    }
+    // `skip` is below request b's tiles when the range starts in it, and zero from then on
+  }
+}
+
+// Joins the partial results of work items that several workers share.  One CTA per (row block and KV head,
+// request), one warp per row; items that one worker covered are final already.
+template <int D, int NB>
+__global__ void __launch_bounds__(32 * kKvWarps)
+kv4_merge_kernel(Kv4Args p) {
+  constexpr int R = 8 * NB, PER = D / 32;
+  __shared__ int64_t scratch[kKvWarps];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int G = p.hq / p.hkv;
+  const int b = blockIdx.y, i = blockIdx.x / p.hkv, kvh = blockIdx.x % p.hkv;
+  int64_t before = 0, all = 0;
+  for (int x = tid; x < p.batch; x += blockDim.x) {
+    const int64_t n = kv4_tiles<R>(p, kv4_request(p, x), G);
+    all += n;
+    if (x < b) before += n;
+  }
+  before = block_sum_i64(before, scratch);
+  all = block_sum_i64(all, scratch);
+  const Kv4Req r = kv4_request(p, b);
+  if (i * R >= r.len * G) return;
+  for (int x = 0; x < i; ++x) {
+    const Kv4Span s = kv4_span<R>(p, r, G, x);
+    before += static_cast<int64_t>(s.last - s.first) * p.hkv;
+  }
+  const Kv4Span span = kv4_span<R>(p, r, G, i);
+  const int n_span = span.last - span.first;
+  const int64_t t0 = before + static_cast<int64_t>(kvh) * n_span, t1 = t0 + n_span;   // this item's tiles
+  // tile t belongs to the largest w with floor(all * w / workers) <= t
+  const int64_t workers = min(static_cast<int64_t>(p.workers), all);
+  const int64_t w0 = ((t0 + 1) * workers - 1) / all, w1 = (t1 * workers - 1) / all;
+  if (w0 == w1) return;
+  const int rows = min(R, r.len * G - i * R);
+  for (int row = warp; row < rows; row += kKvWarps) {
+    float mx = -INFINITY;
+    for (int64_t w = w0; w <= w1; ++w) mx = fmaxf(mx, p.part[((w * 2 + (w == w0 ? 1 : 0)) * R + row) * (D + 2)]);
+    float acc[PER], sum = 0.f;
+#pragma unroll
+    for (int x = 0; x < PER; ++x) acc[x] = 0.f;
+    for (int64_t w = w0; w <= w1; ++w) {
+      const float* src = p.part + ((w * 2 + (w == w0 ? 1 : 0)) * R + row) * (D + 2);
+      const float c = kv_ex2(src[0] - (mx == -INFINITY ? 0.f : mx));
+      sum += src[1] * c;
+#pragma unroll
+      for (int x = 0; x < PER; ++x) acc[x] += src[2 + lane * PER + x] * c;
+    }
+    const int tok = (i * R + row) / G, head = kvh * G + (i * R + row) % G;
+    kv4_write_row<D>(p, acc, sum, static_cast<int64_t>(r.begin) + tok, head, lane);
+  }
+}
+
+constexpr int kKvCtasPerSm = 3;
+
+template <int D, int NB>
+static int launch_kv4(const Kv4Args& a, cudaStream_t st) {
+  constexpr int R = 8 * NB;
+  attention_kv4_kernel<D, NB><<<a.workers, 32 * kKvWarps, 0, st>>>(a);
+  const int G = a.hq / a.hkv;
+  const int64_t blocks = (static_cast<int64_t>(a.max_q_len) * G + R - 1) / R;
+  const dim3 grid(static_cast<unsigned>(blocks * a.hkv), a.batch);
+  kv4_merge_kernel<D, NB><<<grid, 32 * kKvWarps, 0, st>>>(a);
+  return cudaGetLastError() == cudaSuccess ? MSL_OK : MSL_ERR_CUDA;
+}
+
+// Query rows a CTA holds: one MMA column block of 8 where the group's rows fit, else two.
+static int kv4_row_blocks(int max_q_len, int G) { return static_cast<int64_t>(max_q_len) * G <= 8 ? 1 : 2; }
+
+static bool misaligned(const void* p, int bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) != 0; }
+
+}  // namespace msl
+
+using namespace msl;
+
+extern "C" int64_t msl_attention_kv4_workspace(int batch, int max_q_len, int hq, int hkv, int head_dim) {
+  if (batch <= 0 || max_q_len <= 0 || hq <= 0 || hkv <= 0 || hq % hkv || (head_dim != 64 && head_dim != 128)) return 0;
+  const int64_t workers = static_cast<int64_t>(sm_count()) * kKvCtasPerSm;
+  return workers * 2 * 8 * kv4_row_blocks(max_q_len, hq / hkv) * (head_dim + 2) * 4;
+}
+
+extern "C" int msl_attention_kv4(const void* q, int64_t ld_q, const void* k_cache, const void* k_sf,
+                                 const void* v_cache, const void* v_sf, const int* page_table, int max_pages,
+                                 const int* seq_lens, const int* cu_seqlens_q, const float* k_scale,
+                                 const float* v_scale, float softmax_scale, int batch, int max_q_len, int tokens,
+                                 int hq, int hkv, int head_dim, int page_size, int window, int64_t cache_rows,
+                                 void* out, int64_t ld_out, const void* gate, int64_t ld_gate, void* workspace,
+                                 int64_t workspace_bytes, int* status, void* stream) {
+  if (batch <= 0 || max_q_len <= 0 || tokens < 0 || hq <= 0 || hkv <= 0 || hq % hkv || page_size <= 0 || window < 0 ||
+      max_pages <= 0 || cache_rows <= 0 || cache_rows > 0x7fffffff)
+    return MSL_ERR_ARG;
+  if (head_dim != 64 && head_dim != 128) return MSL_ERR_UNSUPPORTED;
+  const int G = hq / hkv;
+  if (G > 128 || batch > 65535) return MSL_ERR_UNSUPPORTED;
+  if (tokens == 0) return MSL_OK;
+  if (!q || !k_cache || !k_sf || !v_cache || !v_sf || !page_table || !seq_lens || !cu_seqlens_q || !k_scale ||
+      !v_scale || !out || !workspace)
+    return MSL_ERR_ARG;
+  const int64_t cols = static_cast<int64_t>(hq) * head_dim;
+  if (ld_q < cols || ld_out < cols || (gate && ld_gate < cols)) return MSL_ERR_ARG;
+  if (misaligned(q, 16) || (ld_q & 7) || misaligned(k_cache, 16) || misaligned(v_cache, 16) || misaligned(k_sf, 8) ||
+      misaligned(v_sf, 8) || misaligned(out, 16) || (ld_out & 7) || (gate && (misaligned(gate, 16) || (ld_gate & 7))) ||
+      misaligned(workspace, 16))
+    return MSL_ERR_ALIGN;
+  if (workspace_bytes < msl_attention_kv4_workspace(batch, max_q_len, hq, hkv, head_dim)) return MSL_ERR_CAPACITY;
+  const auto u8 = [](const void* x) { return static_cast<const uint8_t*>(x); };
+  const Kv4Args a{static_cast<const __nv_bfloat16*>(q), ld_q, u8(k_cache), u8(k_sf), u8(v_cache), u8(v_sf),
+                  page_table, max_pages, seq_lens, cu_seqlens_q, k_scale, v_scale, softmax_scale, batch, max_q_len,
+                  tokens, hq, hkv, page_size, window, cache_rows, static_cast<__nv_bfloat16*>(out), ld_out,
+                  static_cast<const __nv_bfloat16*>(gate), ld_gate, static_cast<float*>(workspace),
+                  sm_count() * kKvCtasPerSm, status};
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (kv4_row_blocks(max_q_len, G) == 1) return head_dim == 128 ? launch_kv4<128, 1>(a, st) : launch_kv4<64, 1>(a, st);
+  return head_dim == 128 ? launch_kv4<128, 2>(a, st) : launch_kv4<64, 2>(a, st);
+}

@@ -11,7 +11,8 @@ be captured in a CUDA graph and replayed on fresh inputs of the same shape.
 All sizes come from the weight shapes and `data["config"]`, so the same code serves the
 reference's native shard and the benchmark configurations.  Beyond the reference's contract:
 `cu_seqlens_q` may be ragged; without "pooler"/"unpooler" weights the experts read the FFN input
-directly; "shared_w13"/"shared_w2" add a dense BF16 shared expert.
+directly; "shared_w13"/"shared_w2" add a dense BF16 shared expert; with "k_cache_sf" / "v_cache_sf" in
+`data` the K/V cache is held in 4 bits ("k_cache" / "v_cache" are then its codes, include/msl.h).
 """
 from __future__ import annotations
 
@@ -143,6 +144,8 @@ def attention_stage(data, st, after_store=None):
     qkv = ops.gemm(data["attn_input"], st["qkv_gate"], status=status)
     _mark(st, "gemm_qkv")
     inv_freq = _inv_freq(st, cfg["rope_theta"], d) if cfg["rope_theta"] else None
+    if "k_cache_sf" in data:
+        return _attention_kv4(data, st, qkv, inv_freq, after_store)
     q8 = ops.qk_rope_store(qkv, data["positions"], data["cache_loc"], inv_freq, data["k_scale"], data["v_scale"],
                            data["k_cache"], data["v_cache"], hq, hkv, d, status=status)
     _mark(st, "qk_rope_store")
@@ -154,6 +157,25 @@ def attention_stage(data, st, after_store=None):
                          data["cu_seqlens_q"], data["k_scale"], data["v_scale"],
                          cfg["sm_scale"] * cfg["qk_scale_factor"], cfg["batch"], cfg["q_len"], hq, hkv, d,
                          cfg["page_size"], cfg["window"], gate=gate, status=status)
+    _mark(st, "attention")
+    return out
+
+
+def _attention_kv4(data, st, qkv, inv_freq, after_store):
+    """The rest of `attention_stage` over a K/V cache held in 4 bits: data["k_cache"] / data["v_cache"] are the codes
+    and data["k_cache_sf"] / data["v_cache_sf"] the block scales."""
+    cfg = data["config"]
+    hq, hkv, d = cfg["num_q_heads"], cfg["num_kv_heads"], cfg["head_dim"]
+    if after_store is not None:
+        raise MslError("a sequence prefilled in chunks on several ranks needs the FP8 cache")
+    cache = (data["k_cache"], data["k_cache_sf"], data["v_cache"], data["v_cache_sf"])
+    q = ops.qk_rope_store_kv4(qkv, data["positions"], data["cache_loc"], inv_freq, data["k_scale"], data["v_scale"],
+                              *cache, hq, hkv, d, status=st["status"])
+    _mark(st, "qk_rope_store")
+    out = ops.attention_kv4(q, *cache, data["page_table"], data["seq_lens"], data["cu_seqlens_q"], data["k_scale"],
+                            data["v_scale"], cfg["sm_scale"] * cfg["qk_scale_factor"], cfg["batch"], cfg["q_len"], hq,
+                            hkv, d, cfg["page_size"], cfg["window"], gate=qkv[:, (hq + 2 * hkv) * d:],
+                            status=st["status"])
     _mark(st, "attention")
     return out
 

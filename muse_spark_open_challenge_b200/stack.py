@@ -49,6 +49,8 @@ def layer_inputs(step: dict, index: int, hidden, stream) -> dict:
     activations handed on by the layer before (or the step's own for layer 0)."""
     d = {k: step[k] for k in _SHARED_KEYS if k in step}
     d["k_cache"], d["v_cache"] = step["k_caches"][index], step["v_caches"][index]
+    if "k_cache_sfs" in step:                          # caches held in 4 bits: the codes' block scales
+        d["k_cache_sf"], d["v_cache_sf"] = step["k_cache_sfs"][index], step["v_cache_sfs"][index]
     d["attn_input"] = step["attn_input"] if hidden is None else hidden
     d["stream"] = step["stream"] if stream is None else stream
     return d
@@ -56,7 +58,8 @@ def layer_inputs(step: dict, index: int, hidden, stream) -> dict:
 
 def forward(step: dict, states: list, run_layer=None):
     """One step through all layers on the current stream.  `step`: a layer `data` dict whose "k_cache" /
-    "v_cache" are replaced by the lists "k_caches" / "v_caches" (one per layer).  Returns (hidden bf16,
+    "v_cache" are replaced by the lists "k_caches" / "v_caches" (one per layer; for caches held in 4 bits the lists
+    "k_cache_sfs" / "v_cache_sfs" stand beside them).  Returns (hidden bf16,
     stream fp32, [expert ids per layer]).  `run_layer(data, state, index)` defaults to
     `layer.kernel_fn`."""
     hidden = stream = None

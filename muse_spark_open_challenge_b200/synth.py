@@ -167,6 +167,19 @@ def make_input(shape: LayerShape, new_lens, ctx_lens, seed: int = 0, page: int =
     }
 
 
+def kv4_cache(shape: LayerShape, pages: int, page: int, seed: int = 0, device: str = "cpu") -> dict:
+    """A filled K/V cache held in 4 bits: uniform codes, E4M3 block scales around 1/4 (values of deviation near 1
+    with a cache scale of 1).  Keys "k_cache", "k_cache_sf", "v_cache", "v_cache_sf" of a layer's `data`."""
+    gen = torch.Generator(device=device).manual_seed(seed)
+    out = {}
+    for name in ("k_cache", "v_cache"):
+        rows = (pages, page, shape.hkv)
+        out[name] = torch.randint(0, 256, (*rows, shape.head_dim // 2), dtype=torch.uint8, generator=gen, device=device)
+        z = torch.randn((*rows, shape.head_dim // 16), generator=gen, device=device)
+        out[name + "_sf"] = torch.exp2(-1.75 + 0.3 * z).to(FP8)
+    return out
+
+
 def uniform_lengths(batch: int, lo: int, hi: int, seed: int = 0) -> list[int]:
     """Lengths lo + floor(u * (hi - lo + 1)) from a seeded CPU generator."""
     u = torch.rand((batch,), generator=torch.Generator().manual_seed(seed))
