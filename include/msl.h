@@ -367,9 +367,10 @@ int msl_kv4_rows(const void* codes, const void* scales, const float* scale, cons
  * request's number of new tokens (rows beyond it, and rows behind the last request, are left as they are).  A page
  * table entry that is negative, beyond the cache or missing (past max_pages) hides its keys and is reported in
  * *status; a row that sees no key is zero.  Scale bytes 0x7f and 0xff (NaN, never stored) read as 448.  The cache
- * must hold fewer than 2^31 rows.  `workspace`: msl_attention_kv4_workspace bytes of caller-owned device memory,
- * 16-byte aligned, no initialisation; calls that overlap on the GPU need one each. */
-int64_t msl_attention_kv4_workspace(int batch, int max_q_len, int hq, int hkv, int head_dim);
+ * must hold fewer than 2^31 rows.  `workspace`: msl_attention_kv4_workspace bytes (may be 0) of caller-owned device
+ * memory, 16-byte aligned, no initialisation; calls that overlap on the GPU need one each. */
+int64_t msl_attention_kv4_workspace(int batch, int max_q_len, int tokens, int hq, int hkv, int head_dim, int max_pages,
+                                    int page_size, int window);
 int msl_attention_kv4(const void* q, int64_t ld_q, const void* k_cache, const void* k_sf, const void* v_cache,
                       const void* v_sf, const int* page_table, int max_pages, const int* seq_lens,
                       const int* cu_seqlens_q, const float* k_scale, const float* v_scale, float softmax_scale,

@@ -66,7 +66,7 @@ SIGNATURES = {
     "msl_page_plan": (_i, [_p, _p, _p, _i, _p, _i, _p, _p, _i, _i, _i, _p, _p, _p, _p, _p]),
     "msl_qk_rope_store_kv4": (_i, [_p, _i64, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _i, _i, _i, _i, _i64, _p, _p]),
     "msl_kv4_rows": (_i, [_p, _p, _p, _p, _i64, _i, _i64, _i, _p, _p, _p]),
-    "msl_attention_kv4_workspace": (_i64, [_i, _i, _i, _i, _i]),
+    "msl_attention_kv4_workspace": (_i64, [_i, _i, _i, _i, _i, _i, _i, _i, _i]),
     "msl_attention_kv4": (_i, [_p, _i64, _p, _p, _p, _p, _p, _i, _p, _p, _p, _p, _f, _i, _i, _i, _i, _i, _i, _i, _i,
                                _i64, _p, _i64, _p, _i64, _p, _i64, _p, _p]),
 }

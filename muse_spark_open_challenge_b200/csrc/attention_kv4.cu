@@ -19,38 +19,13 @@
 // from the accumulator's layout to the operand's by one 8 x 8 transpose in registers.  Queries (bf16) are scaled by
 // a power of two per row so that the largest magnitude lies in [2^14, 2^15) and held in f16: exact for every
 // element within 2^28 of the row's largest.  P is f16 (2^-12 relative), statistics and O are fp32.
-#include <cuda_fp16.h>
-
-#include "msl_common.cuh"
-#include "msl_host.h"
+#include "kv4_common.cuh"
 
 namespace msl {
 
 constexpr int kKvWarps = 4;
 constexpr int kKvTile = 32 * kKvWarps;     // keys of a tile
 constexpr float kKvTau = 8.0f;             // the running maximum may lag by 2^8: P stays within f16
-
-struct Kv4Args {
-  const __nv_bfloat16* q;       // [tokens][hq][D], row pitch ld_q
-  int64_t ld_q;
-  const uint8_t *k, *ks, *v, *vs;
-  const int* page_table;        // [batch][max_pages]
-  int max_pages;
-  const int* seq_lens;
-  const int* cu_seqlens_q;
-  const float* k_scale;
-  const float* v_scale;
-  float softmax_scale;
-  int batch, max_q_len, tokens, hq, hkv, page_size, window;
-  int64_t cache_rows;
-  __nv_bfloat16* out;
-  int64_t ld_out;
-  const __nv_bfloat16* gate;
-  int64_t ld_gate;
-  float* part;                  // [workers][2][R][D + 2]
-  int workers;
-  int* status;
-};
 
 // A request as the schedule sees it: q rows [begin, begin + len), `seq` cached tokens.
 struct Kv4Req {
@@ -103,29 +78,6 @@ __device__ __forceinline__ int64_t block_sum_i64(int64_t v, int64_t* scratch) {
   return s;
 }
 
-__device__ __forceinline__ uint32_t h2_bits(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
-__device__ __forceinline__ __half2 bits_h2(uint32_t u) { return *reinterpret_cast<__half2*>(&u); }
-__device__ __forceinline__ float kv_ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-// The four bytes of a word, each a pair of e2m1 codes -> f16x2 (low nibble in the low half).
-__device__ __forceinline__ void e2m1x8(uint32_t w, __half2 (&h)[4]) {
-  uint32_t a, b, c, d;
-  asm("{.reg .b8 x, y, z, u;\n\tmov.b32 {x, y, z, u}, %4;\n\t"
-      "cvt.rn.f16x2.e2m1x2 %0, x;\n\tcvt.rn.f16x2.e2m1x2 %1, y;\n\t"
-      "cvt.rn.f16x2.e2m1x2 %2, z;\n\tcvt.rn.f16x2.e2m1x2 %3, u;}"
-      : "=r"(a), "=r"(b), "=r"(c), "=r"(d) : "r"(w));
-  h[0] = bits_h2(a); h[1] = bits_h2(b); h[2] = bits_h2(c); h[3] = bits_h2(d);
-}
-// Two e4m3 scales -> f16x2.  The NaN codes (never written by the store) read as 448: a NaN would reach rows that
-// do not see the key, as 0 * NaN in P V.
-__device__ __forceinline__ __half2 scales_h2(uint32_t two) {
-  uint32_t h;
-  asm("{.reg .b16 x;\n\tcvt.u16.u32 x, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, x;}" : "=r"(h) : "r"(two));
-  return __hmin2(bits_h2(h), __half2half2(__ushort_as_half(0x5F00)));   // 448
-}
 __device__ __forceinline__ void mma_16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
                                           uint32_t b0, uint32_t b1) {
   asm volatile(
@@ -190,19 +142,6 @@ __device__ __forceinline__ void kv4_load(Kv4Frag<D>& f, const Kv4Args& p, int kv
   }
 }
 
-// The cache row of key `key` (-1: hidden from every row of the block, or no valid page).
-__device__ __forceinline__ int kv4_row(const Kv4Args& p, const int* table, int key, int lo, int hi) {
-  if (key < lo || key >= hi) return -1;
-  const int idx = key / p.page_size;
-  const int page = idx < p.max_pages ? table[idx] : -1;
-  const int64_t row = static_cast<int64_t>(page) * p.page_size + (key - idx * p.page_size);
-  if (page < 0 || row >= p.cache_rows) {
-    report_error(p.status, MSL_ERR_CAPACITY);
-    return -1;
-  }
-  return static_cast<int>(row);
-}
-
 // Shared-memory layout of a warp's O [R][D]: channel d of the lane group D/8 at pitch D/8 + 2, so that the float2
 // stores of a warp (8 groups x 4 row pairs) fall into different banks.
 template <int D>
@@ -210,29 +149,6 @@ struct Kv4Merge {
   static constexpr int kGroup = D / 8 + 2;
   static constexpr int kRow = 8 * kGroup + 8;
 };
-
-// Rows of a finished block: O / l, v_scale, optional per-head RMS norm * sigmoid(gate), bf16.  One warp per row,
-// lane holds channels [D/32 lane, ...).
-template <int D>
-__device__ __forceinline__ void kv4_write_row(const Kv4Args& p, float (&o)[D / 32], float l, int64_t token, int head,
-                                              int lane) {
-  constexpr int PER = D / 32;
-  const float c = l > 0.f ? *p.v_scale / l : 0.f;          // a row that sees nothing is zero
-  // a NaN sum (a NaN query) must stay visible
-  const float scale = l != l ? l : c;
-  float ss = 0.f;
-#pragma unroll
-  for (int i = 0; i < PER; ++i) { o[i] *= scale; ss += o[i] * o[i]; }
-  if (p.gate != nullptr) {
-    const float r = 1.0f / sqrtf(warp_sum(ss) / D + 1e-5f);
-    const __nv_bfloat16* grow = p.gate + token * p.ld_gate + head * D + lane * PER;
-#pragma unroll
-    for (int i = 0; i < PER; ++i) o[i] *= r / (1.0f + __expf(-__bfloat162float(grow[i])));
-  }
-  __nv_bfloat16* orow = p.out + token * p.ld_out + head * D + lane * PER;
-#pragma unroll
-  for (int i = 0; i < PER; i += 2) *reinterpret_cast<uint32_t*>(orow + i) = pack_bf16x2(o[i], o[i + 1]);
-}
 
 template <int D, int NB>
 __global__ void __launch_bounds__(32 * kKvWarps)
@@ -450,7 +366,8 @@ attention_kv4_kernel(Kv4Args p) {
                 float x = top[nb][c];
 #pragma unroll
                 for (int d = 4; d < 32; d <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, d));
-                const float new_m = fmaxf(m[nb][c], x);
+                // each column (query row) decides for itself: its bits do not depend on its neighbours
+                const float new_m = (x > m[nb][c] + kKvTau || m[nb][c] == -INFINITY) ? x : m[nb][c];
                 const float corr = kv_ex2(m[nb][c] - (new_m == -INFINITY ? 0.f : new_m));
                 m[nb][c] = new_m;
                 l[nb][c] *= corr;
@@ -621,7 +538,31 @@ static int launch_kv4(const Kv4Args& a, cudaStream_t st) {
 }
 
 // Query rows a CTA holds: one MMA column block of 8 where the group's rows fit, else two.
-static int kv4_row_blocks(int max_q_len, int G) { return static_cast<int64_t>(max_q_len) * G <= 8 ? 1 : 2; }
+static int kv4_row_blocks(int64_t rows) { return rows <= 8 ? 1 : 2; }
+
+// Up to this many query rows per KV head the mma.sync kernel above streams the keys once per 16 rows; beyond it the
+// tcgen05 kernel takes them 256 at a time.
+constexpr int kKvFewRows = 64;
+
+struct Kv4Plan {
+  bool few;
+  int splits;
+  int64_t bytes;
+};
+static Kv4Plan kv4_plan(int batch, int max_q_len, int tokens, int hq, int hkv, int head_dim, int max_pages, int page_size,
+                        int window) {
+  Kv4Plan plan{true, 1, 0};
+  const int64_t rows = static_cast<int64_t>(max_q_len) * (hq / hkv);
+  plan.few = rows <= kKvFewRows;
+  if (plan.few) {
+    const int64_t workers = static_cast<int64_t>(sm_count()) * kKvCtasPerSm;
+    plan.bytes = workers * 2 * 8 * kv4_row_blocks(rows) * (head_dim + 2) * 4;
+  } else {
+    plan.splits = msl_attention_split_plan(batch, max_q_len, hq, hkv, max_pages, page_size, window);
+    plan.bytes = kv4_tc_workspace(plan.splits, tokens, hq, head_dim);
+  }
+  return plan;
+}
 
 static bool misaligned(const void* p, int bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) != 0; }
 
@@ -629,10 +570,12 @@ static bool misaligned(const void* p, int bytes) { return (reinterpret_cast<uint
 
 using namespace msl;
 
-extern "C" int64_t msl_attention_kv4_workspace(int batch, int max_q_len, int hq, int hkv, int head_dim) {
-  if (batch <= 0 || max_q_len <= 0 || hq <= 0 || hkv <= 0 || hq % hkv || (head_dim != 64 && head_dim != 128)) return 0;
-  const int64_t workers = static_cast<int64_t>(sm_count()) * kKvCtasPerSm;
-  return workers * 2 * 8 * kv4_row_blocks(max_q_len, hq / hkv) * (head_dim + 2) * 4;
+extern "C" int64_t msl_attention_kv4_workspace(int batch, int max_q_len, int tokens, int hq, int hkv, int head_dim,
+                                               int max_pages, int page_size, int window) {
+  if (batch <= 0 || max_q_len <= 0 || tokens <= 0 || hq <= 0 || hkv <= 0 || hq % hkv || hq / hkv > 128 ||
+      max_pages <= 0 || page_size <= 0 || window < 0)
+    return 0;
+  return kv4_plan(batch, max_q_len, tokens, hq, hkv, head_dim, max_pages, page_size, window).bytes;
 }
 
 extern "C" int msl_attention_kv4(const void* q, int64_t ld_q, const void* k_cache, const void* k_sf,
@@ -650,22 +593,26 @@ extern "C" int msl_attention_kv4(const void* q, int64_t ld_q, const void* k_cach
   if (G > 128 || batch > 65535) return MSL_ERR_UNSUPPORTED;
   if (tokens == 0) return MSL_OK;
   if (!q || !k_cache || !k_sf || !v_cache || !v_sf || !page_table || !seq_lens || !cu_seqlens_q || !k_scale ||
-      !v_scale || !out || !workspace)
+      !v_scale || !out)
     return MSL_ERR_ARG;
+  const Kv4Plan plan = kv4_plan(batch, max_q_len, tokens, hq, hkv, head_dim, max_pages, page_size, window);
+  if (plan.bytes > 0 && !workspace) return MSL_ERR_ARG;
   const int64_t cols = static_cast<int64_t>(hq) * head_dim;
   if (ld_q < cols || ld_out < cols || (gate && ld_gate < cols)) return MSL_ERR_ARG;
   if (misaligned(q, 16) || (ld_q & 7) || misaligned(k_cache, 16) || misaligned(v_cache, 16) || misaligned(k_sf, 8) ||
       misaligned(v_sf, 8) || misaligned(out, 16) || (ld_out & 7) || (gate && (misaligned(gate, 16) || (ld_gate & 7))) ||
       misaligned(workspace, 16))
     return MSL_ERR_ALIGN;
-  if (workspace_bytes < msl_attention_kv4_workspace(batch, max_q_len, hq, hkv, head_dim)) return MSL_ERR_CAPACITY;
+  if (workspace_bytes < plan.bytes) return MSL_ERR_CAPACITY;
   const auto u8 = [](const void* x) { return static_cast<const uint8_t*>(x); };
   const Kv4Args a{static_cast<const __nv_bfloat16*>(q), ld_q, u8(k_cache), u8(k_sf), u8(v_cache), u8(v_sf),
                   page_table, max_pages, seq_lens, cu_seqlens_q, k_scale, v_scale, softmax_scale, batch, max_q_len,
                   tokens, hq, hkv, page_size, window, cache_rows, static_cast<__nv_bfloat16*>(out), ld_out,
                   static_cast<const __nv_bfloat16*>(gate), ld_gate, static_cast<float*>(workspace),
-                  sm_count() * kKvCtasPerSm, status};
+                  sm_count() * kKvCtasPerSm, plan.splits, status};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (kv4_row_blocks(max_q_len, G) == 1) return head_dim == 128 ? launch_kv4<128, 1>(a, st) : launch_kv4<64, 1>(a, st);
+  if (!plan.few) return launch_kv4_tc(a, head_dim, st);
+  if (kv4_row_blocks(static_cast<int64_t>(max_q_len) * G) == 1)
+    return head_dim == 128 ? launch_kv4<128, 1>(a, st) : launch_kv4<64, 1>(a, st);
   return head_dim == 128 ? launch_kv4<128, 2>(a, st) : launch_kv4<64, 2>(a, st);
 }

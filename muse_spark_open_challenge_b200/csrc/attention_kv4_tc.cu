@@ -1,0 +1,614 @@
+// Causal varlen attention over the paged 4-bit K/V cache, many query rows per KV head (prefill, chunks), on tcgen05.
+//
+// One CTA per (request, KV head, block of 2 * floor(128 / G) query tokens[, key slice]); two 128-row query sub-tiles
+// (rows are (token, head in group) pairs) share every K/V tile.  512 threads:
+//   warps 0-3, 4-7  softmax groups of sub-tile 0 / 1, one thread per row, as in the FP8 kernel (csrc/attention_fp8.cu):
+//                   the row of S in registers, maximum, exponentials taken in turns by the two warps of a scheduler,
+//                   P written back to tensor memory over the first 64 columns of the sub-tile's own S, in two halves.
+//                   Before that each thread brings its query row into shared memory: scaled by a power of two to f16
+//                   (largest magnitude in [2^14, 2^15)), so that one operand type serves both products
+//   warp  8         tensor memory and tcgen05.mma issue: S_s = Q_s K^T, O_s += P_s V (kind::f16, fp32 accumulators)
+//   warps 12-15     producers: thread = key of the tile.  Codes and scales go from global memory to registers a tile
+//                   ahead, become f16 (e2m1 conversion times the block scale: exact) and are stored as K-major (K) and
+//                   N-major (V) swizzled operand tiles of a ring
+//   warps 9-11      idle: they round the warpgroup up whose registers the others use
+// Registers are split 176 (softmax) / 56 / 104 (producers): 128 x (176 + 176 + 56 + 104) = 65536, the launch's total.
+// P is f16 (2^-12 relative) times 2^6, which with a lag of the running maximum of at most 2^8 stays below 2^15.
+// A key whose page is missing is hidden: producers leave one bit per key, and the mask pass takes it with the causal
+// limits.  Every wait is bounded.
+#include "kv4_common.cuh"
+
+namespace msl {
+
+constexpr int kTM = 128;        // rows of a query sub-tile
+constexpr int kTN = 128;        // keys of a tile
+constexpr int kTcThreads = 512;
+constexpr float kTcTau = 8.0f;
+constexpr float kTcShift = 6.0f;
+
+template <int D>
+struct TcSmem {
+  static constexpr int kTile = kTN * D * 2;                // bytes of one K, V or Q tile
+  static constexpr int kStages = D == 128 ? 5 : 8;         // ring of K and V tiles in turn
+  static constexpr int kQ = 0;                             // 2 sub-tiles
+  static constexpr int kRing = 2 * kTile;
+  static constexpr int kHeld = kRing + kStages * kTile;    // 8 x 4 words: the keys of a tile that have a page
+  static constexpr int kBar = kHeld + 8 * 16;
+  // q_full, full[stages], empty[stages], s_full[2], p_lo[2], p_hi[2], pv_done[2], turn[8]
+  static constexpr int kNumBars = 1 + 2 * kStages + 16;
+  static constexpr int kTotal = kBar + kNumBars * 8 + 16;
+};
+
+template <int N>
+__device__ __forceinline__ void reg_alloc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N>
+__device__ __forceinline__ void reg_dealloc() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+
+__device__ __forceinline__ void tc_st32(uint32_t taddr, const uint32_t (&o)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+      "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};"
+      ::"r"(taddr), "r"(o[0]), "r"(o[1]), "r"(o[2]), "r"(o[3]), "r"(o[4]), "r"(o[5]), "r"(o[6]), "r"(o[7]),
+      "r"(o[8]), "r"(o[9]), "r"(o[10]), "r"(o[11]), "r"(o[12]), "r"(o[13]), "r"(o[14]), "r"(o[15]), "r"(o[16]),
+      "r"(o[17]), "r"(o[18]), "r"(o[19]), "r"(o[20]), "r"(o[21]), "r"(o[22]), "r"(o[23]), "r"(o[24]), "r"(o[25]),
+      "r"(o[26]), "r"(o[27]), "r"(o[28]), "r"(o[29]), "r"(o[30]), "r"(o[31])
+      : "memory");
+}
+
+__device__ __forceinline__ float tc_max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+__device__ __forceinline__ float tc_row_max(const uint32_t (&s0)[32], const uint32_t (&s1)[32], float m) {
+  float acc[4] = {m, -INFINITY, -INFINITY, -INFINITY};     // independent chains
+#pragma unroll
+  for (int i = 0; i < 32; ++i) acc[i & 3] = tc_max3(acc[i & 3], __uint_as_float(s0[i]), __uint_as_float(s1[i]));
+  return fmaxf(fmaxf(acc[0], acc[1]), fmaxf(acc[2], acc[3]));
+}
+// Scores of keys that this row does not see become -inf: lim_lo < column <= lim_hi and a page are needed.
+__device__ __forceinline__ void tc_mask(uint32_t (&s)[32], int col0, int lim_hi, int lim_lo, uint32_t held) {
+#pragma unroll
+  for (int i = 0; i < 32; ++i) {
+    const int col = col0 + i;
+    if (!(col <= lim_hi && col > lim_lo && ((held >> i) & 1u))) s[i] = 0xff800000u;
+  }
+}
+// 64 columns of a row of S: exponentials summed into l and packed as f16 pairs in key order.
+__device__ __forceinline__ void tc_softmax_half(const uint32_t (&s0)[32], const uint32_t (&s1)[32], float scale_log2,
+                                                float neg_m, float& l, uint32_t (&packed)[32]) {
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const uint32_t(&s)[32] = h ? s1 : s0;
+    float part[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < 32; i += 2) {
+      const float a = kv_ex2(fmaf(__uint_as_float(s[i]), scale_log2, neg_m));
+      const float b = kv_ex2(fmaf(__uint_as_float(s[i + 1]), scale_log2, neg_m));
+      part[(i / 2) & 3] += a;
+      part[(i / 2 + 2) & 3] += b;
+      packed[16 * h + i / 2] = h2_bits(__floats2half2_rn(a, b));
+    }
+    l += (part[0] + part[1]) + (part[2] + part[3]);
+  }
+}
+
+// A key row's codes and scales as loaded.
+template <int D>
+struct TcRow {
+  uint32_t c[D / 8];
+  uint32_t s[D / 64];
+};
+template <int D>
+__device__ __forceinline__ void tc_load_row(TcRow<D>& x, const uint8_t* codes, const uint8_t* scales, int row, int hkv,
+                                            int kvh) {
+#pragma unroll
+  for (int i = 0; i < D / 8; ++i) x.c[i] = 0;
+#pragma unroll
+  for (int i = 0; i < D / 64; ++i) x.s[i] = 0;
+  if (row >= 0) {
+    const int64_t at = static_cast<int64_t>(row) * hkv + kvh;
+    const uint4* src = reinterpret_cast<const uint4*>(codes + at * (D / 2));
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i) {
+      const uint4 v = src[i];
+      x.c[4 * i] = v.x; x.c[4 * i + 1] = v.y; x.c[4 * i + 2] = v.z; x.c[4 * i + 3] = v.w;
+    }
+    if constexpr (D == 128) {
+      const uint2 v = *reinterpret_cast<const uint2*>(scales + at * 8);
+      x.s[0] = v.x; x.s[1] = v.y;
+    } else {
+      x.s[0] = *reinterpret_cast<const uint32_t*>(scales + at * 4);
+    }
+  }
+}
+// ... as f16 into row r of a tile of 64-channel slabs [128 rows][128 bytes], 128-byte swizzle.
+template <int D>
+__device__ __forceinline__ void tc_store_row(const TcRow<D>& x, uint8_t* tile, int r) {
+#pragma unroll
+  for (int b = 0; b < D / 16; b += 2) {                     // two scale blocks of 16 channels
+    const __half2 s2 = scales_h2((x.s[b / 4] >> (8 * (b & 3))) & 0xffffu);
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const __half2 s = e ? __high2half2(s2) : __low2half2(s2);
+#pragma unroll
+      for (int w = 0; w < 2; ++w) {
+        const int chunk = 2 * (b + e) + w;                  // 8 channels = 16 bytes
+        __half2 h[4];
+        e2m1x8(x.c[chunk], h);
+        *reinterpret_cast<uint4*>(tile + (chunk / 8) * (kTN * 128) + swz128(r, chunk % 8)) =
+            make_uint4(h2_bits(__hmul2(h[0], s)), h2_bits(__hmul2(h[1], s)), h2_bits(__hmul2(h[2], s)),
+                       h2_bits(__hmul2(h[3], s)));
+      }
+    }
+  }
+}
+
+template <int D>
+__global__ void __launch_bounds__(kTcThreads, 1)
+attention_kv4_tc_kernel(Kv4Args p) {
+  using S = TcSmem<D>;
+  constexpr int kSt = S::kStages;
+  constexpr int kSlab = kTN * 128;                         // 128 rows x 64 f16 channels
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + S::kBar);
+  uint64_t* q_full = bars;
+  uint64_t* full = bars + 1;
+  uint64_t* empty = full + kSt;
+  uint64_t* s_full = empty + kSt;
+  uint64_t* p_lo = s_full + 2;
+  uint64_t* p_hi = p_lo + 2;
+  uint64_t* pv_done = p_hi + 2;
+  uint64_t* turn = pv_done + 2;                            // [group][warp in group]: the exponential unit's turn
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + S::kNumBars);
+  volatile uint32_t* abort_flag = tmem_slot + 1;
+  uint32_t* held = reinterpret_cast<uint32_t*>(smem + S::kHeld);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int G = p.hq / p.hkv;
+  const int TQ = kTM / G;                                  // query tokens per sub-tile
+  const int b = blockIdx.z, kvh = blockIdx.y;
+  const int q_begin = max(0, min(p.cu_seqlens_q[b], p.tokens));
+  const int q_len = min(max(0, min(p.cu_seqlens_q[b + 1], p.tokens) - q_begin), p.max_q_len);
+  // Longest key ranges first: later query blocks attend to more keys.
+  const int n_qblk = (q_len + 2 * TQ - 1) / (2 * TQ);
+  const int split = static_cast<int>(blockIdx.x) % p.kv_splits;
+  const int qblk = n_qblk - 1 - static_cast<int>(blockIdx.x) / p.kv_splits;
+  if (qblk < 0) return;                                    // uniform for the CTA, before any barrier
+  const int q0 = qblk * 2 * TQ;
+  const int seq = p.seq_lens[b];
+  const int64_t table_keys = static_cast<int64_t>(p.max_pages) * p.page_size;
+  int kt_begin = p.window ? max(0, seq + q0 - p.window + 1) / kTN : 0;
+  const int key_lo = p.window ? max(0, seq + q0 - p.window + 1) : 0;
+  // per sub-tile: valid rows, last query position, number of key tiles (one at least: a row that sees nothing is
+  // still written)
+  int rows_valid[2], max_qpos[2], n_sub[2];
+#pragma unroll
+  for (int s = 0; s < 2; ++s) {
+    const int first = q0 + s * TQ;
+    const int cnt = max(0, min(TQ, q_len - first));
+    rows_valid[s] = cnt * G;
+    max_qpos[s] = seq + first + cnt - 1;
+    const int last_key = static_cast<int>(min(static_cast<int64_t>(max_qpos[s]), table_keys - 1));
+    n_sub[s] = cnt > 0 ? max(1, last_key / kTN + 1 - kt_begin) : 0;
+  }
+  const int last_qpos = max(rows_valid[0] ? max_qpos[0] : -1, rows_valid[1] ? max_qpos[1] : -1);
+  if (threadIdx.x == 0 && last_qpos >= table_keys) report_error(p.status, MSL_ERR_CAPACITY);
+  if (p.kv_splits > 1) {
+    // this CTA's slice of the key tiles; a slice may be empty for one or both sub-tiles
+    const int n_full = max(n_sub[0], n_sub[1]);
+    const int chunk = (n_full + p.kv_splits - 1) / p.kv_splits;
+    const int lo = split * chunk, hi = min(n_full, lo + chunk);
+#pragma unroll
+    for (int s = 0; s < 2; ++s) n_sub[s] = max(0, min(n_sub[s], hi) - lo);
+    kt_begin += lo;
+  }
+  float* part_ml = p.part + static_cast<int64_t>(p.kv_splits) * p.tokens * p.hq * D;
+  const int n_tiles = max(n_sub[0], n_sub[1]);
+  if (n_tiles == 0) {                                      // an empty slice; uniform for the CTA, before any barrier
+    for (int i = threadIdx.x; i < 2 * kTM; i += blockDim.x) {
+      const int s = i / kTM, r = i % kTM;
+      if (r < rows_valid[s]) {
+        const int64_t idx = (static_cast<int64_t>(split) * p.tokens + q_begin + q0 + s * TQ + r / G) * p.hq +
+                            kvh * G + r % G;
+        part_ml[2 * idx] = -INFINITY;
+        part_ml[2 * idx + 1] = 0.f;
+      }
+    }
+    return;
+  }
+
+  if (threadIdx.x == 0) {
+    mbar_init(q_full, 8);
+    for (int i = 0; i < kSt; ++i) { mbar_init(&full[i], 4); mbar_init(&empty[i], 1); }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&s_full[i], 1);
+      mbar_init(&p_lo[i], 4);
+      mbar_init(&p_hi[i], 4);
+      mbar_init(&pv_done[i], 1);
+    }
+    for (int i = 0; i < 8; ++i) mbar_init(&turn[i], 1);
+    *abort_flag = 0;
+    mbar_fence_init();
+  }
+  if (warp == 8) tmem_alloc(tmem_slot, 512);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+
+  if (warp >= 12) {
+    // ------------------------------------------------------------------ producers: thread = key of the tile
+    reg_dealloc<104>();
+    const int r = (warp - 12) * 32 + lane;
+    const int* table = p.page_table + static_cast<int64_t>(b) * p.max_pages;
+    const int first_key = kt_begin * kTN + r;
+    int row = kv4_row(p, table, first_key, key_lo, last_qpos + 1);
+    int row_next = n_tiles > 1 ? kv4_row(p, table, first_key + kTN, key_lo, last_qpos + 1) : -1;
+    TcRow<D> k, v;
+    tc_load_row<D>(k, p.k, p.ks, row, p.hkv, kvh);
+    tc_load_row<D>(v, p.v, p.vs, row, p.hkv, kvh);
+    bool ok = true;
+    for (int j = 0; j < n_tiles; ++j) {
+      const uint32_t mask = __ballot_sync(0xffffffffu, row >= 0);
+      int row_after = -1;
+      if (j + 2 < n_tiles) row_after = kv4_row(p, table, first_key + (j + 2) * kTN, key_lo, last_qpos + 1);
+      const int i0 = 2 * j, st0 = i0 % kSt;
+      if (*abort_flag || !mbar_wait(&empty[st0], ((i0 / kSt) & 1) ^ 1, true)) { ok = false; break; }
+      tc_store_row<D>(k, smem + S::kRing + st0 * S::kTile, r);
+      if (lane == 0) held[(j & 7) * 4 + warp - 12] = mask;
+      fence_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&full[st0]);
+      if (j + 1 < n_tiles) tc_load_row<D>(k, p.k, p.ks, row_next, p.hkv, kvh);
+      const int i1 = i0 + 1, st1 = i1 % kSt;
+      if (*abort_flag || !mbar_wait(&empty[st1], ((i1 / kSt) & 1) ^ 1, true)) { ok = false; break; }
+      tc_store_row<D>(v, smem + S::kRing + st1 * S::kTile, r);
+      fence_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&full[st1]);
+      if (j + 1 < n_tiles) tc_load_row<D>(v, p.v, p.vs, row_next, p.hkv, kvh);
+      row = row_next;
+      row_next = row_after;
+    }
+    if (!ok && lane == 0) { *abort_flag = 1; report_error(p.status, MSL_ERR_DEVICE_TIMEOUT); }
+  } else if (warp >= 8) {
+    reg_dealloc<56>();
+    if (warp == 8) {
+      // ---------------------------------------------------------------- MMA issuer (warp-uniform, one elected lane)
+      const uint32_t on = elect_one();
+      constexpr uint32_t idesc_qk = make_idesc(0, 0, kTM, kTN);
+      constexpr uint32_t idesc_pv = make_idesc(0, 0, kTM, D, 0, 1);     // A = P from TMEM (K-major), B = V, N-major
+      const uint32_t sq = smem_u32(smem + S::kQ), ring = smem_u32(smem + S::kRing);
+      auto issue_qk = [&](int s, uint32_t sk) {
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k) {                 // 32 bytes of a slab's 128-byte rows each
+          const uint32_t off = (k / 4) * kSlab + (k % 4) * 32;
+          tc_mma_f16_if(on, tmem_base + s * kTN, make_sdesc(sq + s * S::kTile + off, 16, 1024, 2),
+                        make_sdesc(sk + off, 16, 1024, 2), idesc_qk, k != 0);
+        }
+        tc_commit_if(on, &s_full[s]);
+      };
+      // keys [64 half, 64 half + 64) of the tile: P columns [32 half, +32) of the sub-tile's S, 8 per MMA
+      auto issue_pv_half = [&](int s, uint32_t sv, int half, bool first) {
+#pragma unroll
+        for (int k = 4 * half; k < 4 * half + 4; ++k)
+          tc_mma_f16_ts_if(on, tmem_base + 2 * kTN + s * kTN, tmem_base + s * kTN + k * 8,
+                           make_sdesc(sv + k * 16 * 128, kSlab, 1024, 2), idesc_pv, !(first && k == 0));
+      };
+      bool ok = mbar_wait(q_full, 0) && mbar_wait(&full[0], 0);
+      if (ok) {
+        tc_fence_after();
+        if (n_sub[0] > 0) issue_qk(0, ring);
+        if (n_sub[1] > 0) issue_qk(1, ring);
+        tc_commit_if(on, &empty[0]);
+      }
+      for (int j = 0; j < n_tiles && ok; ++j) {
+        const uint32_t ph = j & 1;
+        const int iv = 2 * j + 1, sv_st = iv % kSt, ik = 2 * j + 2, sk_st = ik % kSt;
+        const uint32_t sv = ring + sv_st * S::kTile, sk = ring + sk_st * S::kTile;
+        bool v_ready = false, k_ready = false;
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+          if (j < n_sub[s]) {
+            if (!v_ready) {
+              if (*abort_flag || !mbar_wait(&full[sv_st], (iv / kSt) & 1)) { ok = false; break; }
+              v_ready = true;
+            }
+            if (*abort_flag || !mbar_wait(&p_lo[s], ph)) { ok = false; break; }
+            tc_fence_after();
+            issue_pv_half(s, sv, 0, j == 0);
+            if (*abort_flag || !mbar_wait(&p_hi[s], ph)) { ok = false; break; }
+            tc_fence_after();
+            issue_pv_half(s, sv, 1, false);
+            if (j == n_sub[s] - 1) tc_commit_if(on, &pv_done[s]);
+            if (j + 1 < n_sub[s]) {
+              if (!k_ready) {
+                if (*abort_flag || !mbar_wait(&full[sk_st], (ik / kSt) & 1)) { ok = false; break; }
+                tc_fence_after();
+                k_ready = true;
+              }
+              issue_qk(s, sk);
+            }
+          }
+        }
+        if (!ok) break;
+        tc_commit_if(on, &empty[sv_st]);
+        if (k_ready) tc_commit_if(on, &empty[sk_st]);
+      }
+      if (!ok && lane == 0) { *abort_flag = 1; report_error(p.status, MSL_ERR_DEVICE_TIMEOUT); }
+    }
+  } else {
+    // ------------------------------------------------------------------ softmax / correction / epilogue
+    reg_alloc<176>();
+    const int sub = warp >> 2;                             // query sub-tile of this group
+    const int r = (warp & 3) * 32 + lane;                  // row = TMEM lane
+    const int n_mine = n_sub[sub], n_other = n_sub[sub ^ 1];
+    const int tq = r / G, g = r - tq * G;
+    const bool row_valid = r < rows_valid[sub];
+    const int first_tok = q0 + sub * TQ;
+    const int qpos = seq + min(first_tok + tq, max(q_len - 1, 0));
+    const int sub_min_qpos = seq + first_tok;
+    float scale_log2 = p.softmax_scale * (*p.k_scale) * 1.4426950408889634f;
+    {
+      // this thread's query row, f16 with the largest magnitude in [2^14, 2^15)
+      const uint4* src = reinterpret_cast<const uint4*>(
+          p.q + (static_cast<int64_t>(q_begin) + first_tok + tq) * p.ld_q + (kvh * G + g) * D);
+      uint8_t* dst = smem + S::kQ + sub * S::kTile;
+      uint32_t w[D / 2];
+#pragma unroll
+      for (int i = 0; i < D / 8; ++i) {
+        uint4 x = make_uint4(0, 0, 0, 0);
+        if (row_valid) x = src[i];
+        w[4 * i] = x.x; w[4 * i + 1] = x.y; w[4 * i + 2] = x.z; w[4 * i + 3] = x.w;
+      }
+      uint32_t mx = 0;
+#pragma unroll
+      for (int i = 0; i < D / 2; ++i) mx = max(mx, max(w[i] & 0x7fffu, (w[i] >> 16) & 0x7fffu));
+      const int e = min(max(static_cast<int>(mx >> 7), 16), 254);
+      const float up = __uint_as_float(static_cast<uint32_t>(127 + 141 - e) << 23);
+      scale_log2 = scale_log2 / up;
+#pragma unroll
+      for (int i = 0; i < D / 8; ++i) {
+        uint32_t h[4];
+#pragma unroll
+        for (int x = 0; x < 4; ++x)
+          h[x] = h2_bits(__floats2half2_rn(bf16_bits_to_f32(w[4 * i + x] & 0xffffu) * up,
+                                           bf16_bits_to_f32(w[4 * i + x] >> 16) * up));
+        *reinterpret_cast<uint4*>(dst + (i / 8) * kSlab + swz128(r, i % 8)) = make_uint4(h[0], h[1], h[2], h[3]);
+      }
+      fence_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(q_full);
+    }
+    const uint32_t lane_sel = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    const uint32_t tmem_s = tmem_base + sub * kTN + lane_sel;
+    const uint32_t tmem_o = tmem_base + 2 * kTN + sub * kTN + lane_sel;
+    float m_run = -INFINITY, l_run = 0.f;                  // l accumulates 2^kTcShift * sum of exponentials
+    bool ok = true;
+    for (int j = 0; j < n_mine && ok; ++j) {
+      const uint32_t ph = j & 1;
+      const int key0 = (kt_begin + j) * kTN;
+      if (*abort_flag || !mbar_wait(&s_full[sub], ph)) { ok = false; break; }
+      tc_fence_after();
+      const uint4 hm = *reinterpret_cast<const uint4*>(held + (j & 7) * 4);
+      const bool full_tile = (key0 + kTN - 1 <= sub_min_qpos) && (!p.window || key0 > max_qpos[sub] - p.window) &&
+                             (hm.x & hm.y & hm.z & hm.w) == 0xffffffffu;
+      const int lim_hi = qpos - key0;                       // visible columns: lim_lo < col <= lim_hi
+      const int lim_lo = p.window ? qpos - p.window - key0 : -1;
+      uint32_t sa[32], sb[32], sc[32], sd[32];
+      tmem_ld32(tmem_s, sa);
+      tmem_ld32(tmem_s + 32, sb);
+      tmem_ld32(tmem_s + 64, sc);
+      tmem_ld32(tmem_s + 96, sd);
+      tmem_ld_wait();
+      if (!full_tile) {
+        tc_mask(sa, 0, lim_hi, lim_lo, hm.x);
+        tc_mask(sb, 32, lim_hi, lim_lo, hm.y);
+        tc_mask(sc, 64, lim_hi, lim_lo, hm.z);
+        tc_mask(sd, 96, lim_hi, lim_lo, hm.w);
+      }
+      const float m_cand = tc_row_max(sc, sd, tc_row_max(sa, sb, -INFINITY)) * scale_log2;
+      // A row's reference maximum moves when the row exceeds it by more than tau, or finds its first visible key.  Each
+      // row decides for itself, so that its bits do not depend on its neighbours; the warp rescales together.
+      const bool move = m_cand > m_run + kTcTau || (m_run == -INFINITY && m_cand > -INFINITY);
+      const bool event = __any_sync(0xffffffffu, move);
+      float corr = 1.0f;
+      if (move) {
+        corr = kv_ex2(m_run - m_cand);                      // 0 when m_run = -inf
+        m_run = m_cand;
+      }
+      const float m_use = (m_run == -INFINITY) ? 0.f : m_run;
+      const bool resc = j > 0 && event;                     // warp-uniform
+      // The two warps that share a scheduler (one of each group) take turns at the exponential pass.  Order: group 0
+      // tile 0, group 1 tile 0, group 0 tile 1, ...; a turn is skipped where the partner has no such tile.
+      if (sub == 0 ? (j >= 1 && j - 1 < n_other) : (j < n_other)) {
+        if (*abort_flag || !mbar_wait(&turn[sub * 4 + (warp & 3)], (sub == 0 ? j - 1 : j) & 1)) { ok = false; break; }
+      }
+      const float neg_m = kTcShift - m_use;
+      float l_tile = 0.f;
+      uint32_t pk[32], pk2[32];
+      tc_softmax_half(sa, sb, scale_log2, neg_m, l_tile, pk);
+      if (!resc) {
+        tc_st32(tmem_s, pk);
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_lo[sub]);
+      }
+      __syncwarp();
+      if (lane == 0 && (sub == 0 ? (j < n_other) : (j + 1 < n_other))) mbar_arrive(&turn[(sub ^ 1) * 4 + (warp & 3)]);
+      tc_softmax_half(sc, sd, scale_log2, neg_m, l_tile, pk2);
+      if (resc) {
+        // O moves to the new maximum before any of this tile's P is used.  S(j) was ready only after P V(j-1) had
+        // finished (the tensor pipe ran it first), so O is quiet.
+#pragma unroll
+        for (int c = 0; c < D; c += 32) {
+          uint32_t oa[32];
+          tmem_ld32(tmem_o + c, oa);
+          tmem_ld_wait();
+#pragma unroll
+          for (int i = 0; i < 32; ++i) oa[i] = __float_as_uint(__uint_as_float(oa[i]) * corr);
+          tc_st32(tmem_o + c, oa);
+        }
+        tc_st32(tmem_s, pk);
+      }
+      tc_st32(tmem_s + 32, pk2);
+      tmem_st_wait();                                       // P and a rescaled O
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        if (resc) mbar_arrive(&p_lo[sub]);
+        mbar_arrive(&p_hi[sub]);
+      }
+      l_run = l_run * corr + l_tile;
+    }
+    // ---------------------------------------------------------------- epilogue
+    if (ok && n_mine > 0) {
+      if (*abort_flag || !mbar_wait(&pv_done[sub], 0)) ok = false;     // committed once, behind the last P V
+    }
+    if (p.kv_splits > 1) {
+      // partial result of this key slice: O as it stands in TMEM, with the maximum and sum it refers to
+      const bool have = ok && n_mine > 0;
+      if (have) tc_fence_after();
+      const int64_t idx = (static_cast<int64_t>(split) * p.tokens + q_begin + first_tok + tq) * p.hq + kvh * G + g;
+      if (row_valid) {
+        part_ml[2 * idx] = have ? m_run : -INFINITY;
+        part_ml[2 * idx + 1] = have ? l_run : 0.f;
+      }
+      if (have) {
+#pragma unroll 1
+        for (int c = 0; c < D; c += 32) {
+          uint32_t o[32];
+          tmem_ld32(tmem_o + c, o);
+          tmem_ld_wait();
+          if (row_valid) {
+            float4* dst = reinterpret_cast<float4*>(p.part + idx * D + c);
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              dst[i] = make_float4(__uint_as_float(o[4 * i]), __uint_as_float(o[4 * i + 1]),
+                                   __uint_as_float(o[4 * i + 2]), __uint_as_float(o[4 * i + 3]));
+          }
+        }
+      }
+    } else if (ok && n_mine > 0) {
+      tc_fence_after();
+      // l carries the same power of two as P; a row that sees nothing is zero, a NaN sum (a NaN query) stays visible
+      const float c_out = l_run > 0.f ? (*p.v_scale) / l_run : (l_run != l_run ? l_run : 0.f);
+      float r_norm = 1.0f;
+      if (p.gate != nullptr) {
+        float ss = 0.f;
+#pragma unroll 1
+        for (int c = 0; c < D; c += 32) {
+          uint32_t o[32];
+          tmem_ld32(tmem_o + c, o);
+          tmem_ld_wait();
+#pragma unroll
+          for (int i = 0; i < 32; ++i) { const float x = __uint_as_float(o[i]) * c_out; ss += x * x; }
+        }
+        r_norm = 1.0f / sqrtf(ss / D + 1e-5f);
+      }
+      const int64_t token = static_cast<int64_t>(q_begin) + first_tok + tq;
+      const int head = kvh * G + g;
+      __nv_bfloat16* orow = p.out + token * p.ld_out + head * D;
+      const __nv_bfloat16* grow = p.gate ? p.gate + token * p.ld_gate + head * D : nullptr;
+#pragma unroll 1
+      for (int c = 0; c < D; c += 32) {
+        uint32_t o[32];
+        tmem_ld32(tmem_o + c, o);
+        tmem_ld_wait();
+        if (row_valid) {
+          float v[32];
+#pragma unroll
+          for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(o[i]) * c_out * r_norm;
+          if (grow != nullptr) {
+#pragma unroll
+            for (int i = 0; i < 32; i += 8) {
+              const uint4 gq = *reinterpret_cast<const uint4*>(grow + c + i);
+              const uint32_t gw[4] = {gq.x, gq.y, gq.z, gq.w};
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                v[i + 2 * e] *= 1.0f / (1.0f + __expf(-bf16_bits_to_f32(gw[e] & 0xffffu)));
+                v[i + 2 * e + 1] *= 1.0f / (1.0f + __expf(-bf16_bits_to_f32(gw[e] >> 16)));
+              }
+            }
+          }
+#pragma unroll
+          for (int i = 0; i < 32; i += 8)
+            *reinterpret_cast<uint4*>(orow + c + i) =
+                make_uint4(pack_bf16x2(v[i], v[i + 1]), pack_bf16x2(v[i + 2], v[i + 3]),
+                           pack_bf16x2(v[i + 4], v[i + 5]), pack_bf16x2(v[i + 6], v[i + 7]));
+        }
+      }
+    }
+    if (!ok && lane == 0) { *abort_flag = 1; report_error(p.status, MSL_ERR_DEVICE_TIMEOUT); }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 8) {
+    __syncwarp();
+    tmem_dealloc(tmem_base, 512);
+  }
+}
+
+// Joins the key slices: one warp per (token, head); slice s holds O and l relative to its own maximum.  Rows that no
+// request owns are left as they are, so the request of a row is looked up first.
+template <int D>
+__global__ void __launch_bounds__(256)
+kv4_tc_merge_kernel(Kv4Args p) {
+  constexpr int PER = D / 32;
+  const int lane = threadIdx.x & 31;
+  const int b = blockIdx.y;
+  const int q_begin = max(0, min(p.cu_seqlens_q[b], p.tokens));
+  const int q_len = min(max(0, min(p.cu_seqlens_q[b + 1], p.tokens) - q_begin), p.max_q_len);
+  const int64_t item = static_cast<int64_t>(blockIdx.x) * (blockDim.x >> 5) + (threadIdx.x >> 5);
+  if (item >= static_cast<int64_t>(q_len) * p.hq) return;
+  const int64_t token = q_begin + item / p.hq;
+  const int head = static_cast<int>(item % p.hq);
+  const float* part_ml = p.part + static_cast<int64_t>(p.kv_splits) * p.tokens * p.hq * D;
+  const int64_t stride = static_cast<int64_t>(p.tokens) * p.hq, base = token * p.hq + head;
+  float mx = -INFINITY;
+  for (int s = 0; s < p.kv_splits; ++s) mx = fmaxf(mx, part_ml[2 * (s * stride + base)]);
+  float acc[PER], sum = 0.f;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) acc[i] = 0.f;
+  for (int s = 0; s < p.kv_splits; ++s) {
+    const int64_t at = s * stride + base;
+    const float l = part_ml[2 * at + 1];
+    if (l == 0.f) continue;                                 // an empty slice wrote no O
+    const float w = kv_ex2(part_ml[2 * at] - (mx == -INFINITY ? 0.f : mx));
+    sum += l * w;
+    const float* o = p.part + at * D + lane * PER;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) acc[i] += o[i] * w;
+  }
+  kv4_write_row<D>(p, acc, sum, token, head, lane);
+}
+
+template <int D>
+static int launch_tc(const Kv4Args& a, cudaStream_t st) {
+  const int smem = TcSmem<D>::kTotal + 1024;
+  static SmemConfig config;
+  if (int rc = config.ensure(attention_kv4_tc_kernel<D>, smem)) return rc;
+  const int tq2 = 2 * (kTM / (a.hq / a.hkv));
+  const dim3 grid(((a.max_q_len + tq2 - 1) / tq2) * a.kv_splits, a.hkv, a.batch);
+  attention_kv4_tc_kernel<D><<<grid, kTcThreads, smem, st>>>(a);
+  if (a.kv_splits > 1) {
+    const int64_t items = static_cast<int64_t>(a.max_q_len) * a.hq;
+    kv4_tc_merge_kernel<D><<<dim3(static_cast<unsigned>((items + 7) / 8), a.batch), 256, 0, st>>>(a);
+  }
+  return cudaGetLastError() == cudaSuccess ? MSL_OK : MSL_ERR_CUDA;
+}
+
+int launch_kv4_tc(const Kv4Args& a, int head_dim, cudaStream_t st) {
+  return head_dim == 128 ? launch_tc<128>(a, st) : launch_tc<64>(a, st);
+}
+
+int64_t kv4_tc_workspace(int kv_splits, int tokens, int hq, int head_dim) {
+  return kv_splits <= 1 ? 0 : static_cast<int64_t>(kv_splits) * tokens * hq * (head_dim + 2) * 4;
+}
+
+}  // namespace msl

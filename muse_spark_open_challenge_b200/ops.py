@@ -488,7 +488,7 @@ def attention_kv4(q, k_cache, k_sf, v_cache, v_sf, page_table, seq_lens, cu_seql
                     raise MslError(f"{name}: expected shape {(t, cols)}, got {tuple(x.shape)}")
         pitch = lambda x: max(x.stride(0), cols) if t < 2 else x.stride(0)     # noqa: E731  (one row has no pitch)
         lib = _lib.lib()
-        size = int(lib.msl_attention_kv4_workspace(batch, max_q_len, hq, hkv, head_dim))
+        size = lib.msl_attention_kv4_workspace(batch, max_q_len, t, hq, hkv, head_dim, page_table.shape[1], page_size, window)
         work = torch.empty(max(size, 16), dtype=torch.uint8, device=q.device)
         check(lib.msl_attention_kv4(q.data_ptr(), pitch(q), k_cache.data_ptr(), k_sf.data_ptr(), v_cache.data_ptr(),
                                     v_sf.data_ptr(), page_table.data_ptr(), page_table.shape[1], seq_lens.data_ptr(),

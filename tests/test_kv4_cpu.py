@@ -85,7 +85,8 @@ def attention_call(lib, **kw):
              gate=NULL, ld_gate=0, work=FAKE, bytes=None)
     a.update(kw)
     if a["bytes"] is None:
-        a["bytes"] = lib.msl_attention_kv4_workspace(a["batch"], a["longest"], a["hq"], a["hkv"], a["dim"])
+        a["bytes"] = lib.msl_attention_kv4_workspace(a["batch"], a["longest"], a["tokens"], a["hq"], a["hkv"], a["dim"],
+                                                     a["max_pages"], a["page"], a["window"])
     return lib.msl_attention_kv4(a["q"], a["ld_q"], a["k"], a["kf"], a["v"], a["vf"], a["table"], a["max_pages"], a["seq"],
                                  a["cu"], a["ks"], a["vs"], 0.125, a["batch"], a["longest"], a["tokens"], a["hq"],
                                  a["hkv"], a["dim"], a["page"], a["window"], a["rows"], a["out"], a["ld_out"], a["gate"],
