@@ -6,7 +6,7 @@ Every wrapper validates dtypes/contiguity, launches on `torch.cuda.current_strea
 """
 from __future__ import annotations
 
-import contextlib
+import functools
 
 import torch
 
@@ -337,56 +337,62 @@ def grouped_gemm_nvfp4_bs(xq, w_codes, w_scales_tiled, global_scales, offsets, o
 
 
 # ---- the K/V cache held in 4 bits
-def _one_device(**tensors):
-    """Check that the given tensors (None: absent) share one CUDA device and return a context in which it is the
-    current one, so that `_stream()` is that device's current stream."""
-    dev = None
-    for name, t in tensors.items():
-        if t is None:
-            continue
-        if not t.is_cuda:
-            raise MslError(f"{name}: expected a CUDA tensor, got one on {t.device}")
-        if dev is None:
-            dev = t.device
-        elif t.device != dev:
-            raise MslError(f"{name}: on {t.device}, the other tensors are on {dev}")
-    return contextlib.nullcontext() if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
+# A decode step is a few microseconds of GPU time, so these wrappers check with few Python operations; the sizes,
+# pitches and alignments are checked again behind the C ABI.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
+    (lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
+def _device(index, tensors, names):
+    """All of `tensors` (None: absent) must be on CUDA device `index`."""
+    for i, t in enumerate(tensors):
+        if t is not None and t.get_device() != index:
+            raise MslError(f"{names.split()[i]}: on {t.device}, expected cuda:{index}")
+    if index < 0:
+        raise MslError(f"{names.split()[0]}: expected a CUDA tensor")
 
 
 def _is(t, dtype, shape, name):
-    """A contiguous tensor of this type and shape (-1: any size)."""
-    if t.dtype != dtype or not t.is_contiguous():
-        raise MslError(f"{name}: expected a contiguous tensor of {dtype}, got {t.dtype} with strides {t.stride()}")
-    if t.dim() != len(shape) or any(w >= 0 and w != s for w, s in zip(shape, t.shape)):
-        raise MslError(f"{name}: expected shape {tuple(shape)}, got {tuple(t.shape)}")
+    """A contiguous tensor of this type and shape."""
+    if t.dtype is not dtype or t.shape != shape or not t.is_contiguous():
+        raise MslError(f"{name}: expected a contiguous tensor of {dtype} and shape {tuple(shape)}, got {t.dtype}, "
+                       f"{tuple(t.shape)}, strides {t.stride()}")
 
 
-def _scalar(t, name):
-    if t.dtype != torch.float32 or t.numel() != 1:
-        raise MslError(f"{name}: expected one fp32 value on the device")
+def _scalars(*scales):
+    for t in scales:
+        if t.dtype is not torch.float32 or t.numel() != 1:
+            raise MslError("a cache scale is one fp32 value on the device")
 
 
 def _status(t):
-    if t is not None and (t.dtype != torch.int32 or t.numel() < 1):
+    if t is not None and t.dtype is not torch.int32:
         raise MslError("status: expected an int32 tensor")
 
 
 def _kv4_cache(codes, scales, hkv, head_dim, name):
     """Rows of a 4-bit cache: codes u8 [..., hkv, head_dim / 2], scales e4m3 (or its bytes) [..., hkv, head_dim / 16]."""
-    if codes.dtype != torch.uint8 or scales.dtype not in (FP8, torch.uint8):
+    if codes.dtype is not torch.uint8 or (scales.dtype is not FP8 and scales.dtype is not torch.uint8):
         raise MslError(f"{name}: expected uint8 codes and e4m3 scales, got {codes.dtype} and {scales.dtype}")
-    if not codes.is_contiguous() or not scales.is_contiguous():
-        raise MslError(f"{name}: codes and scales must be contiguous")
-    if codes.dim() < 3 or codes.shape[-2:] != (hkv, head_dim // 2) or \
-            tuple(scales.shape) != (*codes.shape[:-1], head_dim // 16):
-        raise MslError(f"{name}: codes {tuple(codes.shape)} and scales {tuple(scales.shape)} are not rows of {hkv} heads "
+    shape, of_scales = codes.shape, scales.shape
+    if len(shape) < 3 or shape[-1] * 2 != head_dim or shape[-2] != hkv or of_scales[-1:] != (head_dim // 16,) or \
+            of_scales[:-1] != shape[:-1] or not codes.is_contiguous() or not scales.is_contiguous():
+        raise MslError(f"{name}: codes {tuple(shape)} and scales {tuple(of_scales)} are not contiguous rows of {hkv} heads "
                        f"x {head_dim} channels")
     return codes.numel() // (hkv * head_dim // 2)
 
 
 def _heads(hq, hkv, head_dim):
-    if hq <= 0 or hkv <= 0 or hq % hkv or head_dim not in (64, 128):
+    if hq <= 0 or hkv <= 0 or hq % hkv or (head_dim != 64 and head_dim != 128):
         raise MslError(f"{hq} query heads over {hkv} KV heads of {head_dim} channels are not supported")
+
+
+def _pitch(t, rows, cols, name):
+    """Row pitch of a bf16 [rows, cols] view with contiguous rows (a single row has none: its width will do)."""
+    if t.dtype is not torch.bfloat16 or t.shape != (rows, cols) or (cols > 1 and t.stride(1) != 1):
+        raise MslError(f"{name}: expected bf16 {(rows, cols)} with contiguous rows, got {t.dtype} {tuple(t.shape)}, strides "
+                       f"{t.stride()}")
+    return t.stride(0) if rows > 1 else cols
 
 
 def page_plan(new_lens, seq_lens, page_table, free_pages, free_head, page_size, tokens, status=None):
@@ -396,22 +402,29 @@ def page_plan(new_lens, seq_lens, page_table, free_pages, free_head, page_size, 
     into its row.  Returns (cu_seqlens_q i32 [B + 1], positions i64 [tokens], cache_loc i64 [tokens], the new free head
     i32 [1]); entries behind the last new token get position 0 and cache_loc -1.  Too few free pages, too short a
     table row or more new tokens than `tokens` are reported in `status`; slots without a page are -1."""
-    batch = new_lens.numel()
-    with _one_device(new_lens=new_lens, seq_lens=seq_lens, page_table=page_table, free_pages=free_pages,
-                     free_head=free_head, status=status):
-        _is(new_lens, torch.int32, (-1,), "new_lens"), _is(seq_lens, torch.int32, (batch,), "seq_lens")
-        _is(page_table, torch.int32, (batch, -1), "page_table"), _is(free_pages, torch.int32, (-1,), "free_pages")
-        _is(free_head, torch.int32, (1,), "free_head"), _status(status)
-        dev = new_lens.device
-        cu = torch.empty(batch + 1, dtype=torch.int32, device=dev)
-        head = torch.empty(1, dtype=torch.int32, device=dev)
-        slots = torch.empty((2, tokens), dtype=torch.int64, device=dev)
-        check(_lib.lib().msl_page_plan(new_lens.data_ptr(), seq_lens.data_ptr(), page_table.data_ptr(),
-                                       page_table.shape[1], free_pages.data_ptr(), free_pages.numel(),
-                                       free_head.data_ptr(), head.data_ptr(), batch, page_size, tokens, cu.data_ptr(),
-                                       slots[0].data_ptr(), slots[1].data_ptr(), _ptr(status), _stream()),
-              "msl_page_plan")
-    return cu, slots[0], slots[1], head
+    index = new_lens.get_device()
+    _device(index, (new_lens, seq_lens, page_table, free_pages, free_head, status),
+            "new_lens seq_lens page_table free_pages free_head status")
+    if index != torch.cuda.current_device():
+        with torch.cuda.device(index):
+            return page_plan(new_lens, seq_lens, page_table, free_pages, free_head, page_size, tokens, status)
+    batch, i32 = new_lens.numel(), torch.int32
+    if page_table.dim() != 2 or tokens < 0:
+        raise MslError("page_plan: expected a page table [requests, max_pages] and a number of tokens")
+    max_pages, n_free = page_table.shape[1], free_pages.numel()
+    _is(new_lens, i32, (batch,), "new_lens"), _is(seq_lens, i32, (batch,), "seq_lens")
+    _is(page_table, i32, (batch, max_pages), "page_table"), _is(free_pages, i32, (n_free,), "free_pages")
+    _is(free_head, i32, (1,), "free_head"), _status(status)
+    dev = new_lens.device
+    cu = torch.empty(batch + 1, dtype=i32, device=dev)
+    head = torch.empty(1, dtype=i32, device=dev)
+    positions = torch.empty(tokens, dtype=torch.int64, device=dev)
+    cache_loc = torch.empty(tokens, dtype=torch.int64, device=dev)
+    check(_lib.lib().msl_page_plan(new_lens.data_ptr(), seq_lens.data_ptr(), page_table.data_ptr(), max_pages,
+                                   free_pages.data_ptr(), n_free, free_head.data_ptr(), head.data_ptr(), batch,
+                                   page_size, tokens, cu.data_ptr(), positions.data_ptr(), cache_loc.data_ptr(),
+                                   _ptr(status), _raw_stream(index)), "msl_page_plan")
+    return cu, positions, cache_loc, head
 
 
 def qk_rope_store_kv4(qkv, positions, cache_loc, inv_freq, k_scale, v_scale, k_cache, k_sf, v_cache, v_sf, hq, hkv,
@@ -419,45 +432,57 @@ def qk_rope_store_kv4(qkv, positions, cache_loc, inv_freq, k_scale, v_scale, k_c
     """`qk_rope_store` for the 4-bit cache: returns q bf16 [T, hq, head_dim] and writes the new K/V rows as codes
     (u8 [..., hkv, head_dim / 2]) and block scales (e4m3 [..., hkv, head_dim / 16]).  A negative cache_loc marks a padding
     token, which is not stored."""
-    with _one_device(qkv=qkv, positions=positions, cache_loc=cache_loc, inv_freq=inv_freq, k_scale=k_scale,
-                     v_scale=v_scale, k_cache=k_cache, k_sf=k_sf, v_cache=v_cache, v_sf=v_sf, status=status):
-        _heads(hq, hkv, head_dim), _need(qkv, torch.bfloat16, "qkv"), _status(status)
-        ld = _rows(qkv, "qkv")
-        t = qkv.shape[0]
-        if qkv.shape[1] < (hq + 2 * hkv) * head_dim:
-            raise MslError(f"qkv: {qkv.shape[1]} columns are fewer than the q, k and v heads have")
-        _is(positions, torch.int64, (t,), "positions"), _is(cache_loc, torch.int64, (t,), "cache_loc")
-        if inv_freq is not None:
-            _is(inv_freq, torch.float32, (head_dim // 2,), "inv_freq")
-        _scalar(k_scale, "k_scale"), _scalar(v_scale, "v_scale")
-        rows = _kv4_cache(k_cache, k_sf, hkv, head_dim, "k_cache")
-        if _kv4_cache(v_cache, v_sf, hkv, head_dim, "v_cache") != rows:
-            raise MslError("the key and value caches have different numbers of rows")
-        q = torch.empty((t, hq, head_dim), dtype=torch.bfloat16, device=qkv.device)
-        check(_lib.lib().msl_qk_rope_store_kv4(qkv.data_ptr(), max(ld, qkv.shape[1]) if t < 2 else ld,
-                                               positions.data_ptr(), cache_loc.data_ptr(), _ptr(inv_freq),
-                                               k_scale.data_ptr(), v_scale.data_ptr(), q.data_ptr(),
-                                               k_cache.data_ptr(), k_sf.data_ptr(), v_cache.data_ptr(),
-                                               v_sf.data_ptr(), t, hq, hkv, head_dim, rows, _ptr(status), _stream()),
-              "msl_qk_rope_store_kv4")
+    index = qkv.get_device()
+    _device(index, (qkv, positions, cache_loc, inv_freq, k_scale, v_scale, k_cache, k_sf, v_cache, v_sf, status),
+            "qkv positions cache_loc inv_freq k_scale v_scale k_cache k_sf v_cache v_sf status")
+    if index != torch.cuda.current_device():
+        with torch.cuda.device(index):
+            return qk_rope_store_kv4(qkv, positions, cache_loc, inv_freq, k_scale, v_scale, k_cache, k_sf, v_cache, v_sf,
+                                     hq, hkv, head_dim, status)
+    _heads(hq, hkv, head_dim), _status(status), _scalars(k_scale, v_scale)
+    if qkv.dim() != 2 or qkv.shape[1] < (hq + 2 * hkv) * head_dim:
+        raise MslError(f"qkv: {tuple(qkv.shape)} has fewer columns than the q, k and v heads")
+    t, cols = qkv.shape
+    ld = _pitch(qkv, t, cols, "qkv")
+    _is(positions, torch.int64, (t,), "positions"), _is(cache_loc, torch.int64, (t,), "cache_loc")
+    if inv_freq is not None:
+        _is(inv_freq, torch.float32, (head_dim // 2,), "inv_freq")
+    rows = _kv4_cache(k_cache, k_sf, hkv, head_dim, "k_cache")
+    if _kv4_cache(v_cache, v_sf, hkv, head_dim, "v_cache") != rows:
+        raise MslError("the key and value caches have different numbers of rows")
+    q = torch.empty((t, hq, head_dim), dtype=torch.bfloat16, device=qkv.device)
+    check(_lib.lib().msl_qk_rope_store_kv4(qkv.data_ptr(), ld, positions.data_ptr(), cache_loc.data_ptr(),
+                                           _ptr(inv_freq), k_scale.data_ptr(), v_scale.data_ptr(), q.data_ptr(),
+                                           k_cache.data_ptr(), k_sf.data_ptr(), v_cache.data_ptr(), v_sf.data_ptr(), t,
+                                           hq, hkv, head_dim, rows, _ptr(status), _raw_stream(index)),
+          "msl_qk_rope_store_kv4")
     return q
 
 
 def kv4_rows(codes, scales, scale, rows, dtype=torch.bfloat16, status=None):
     """The values that cache rows `rows` (i64 [n]) of a 4-bit cache stand for: bf16 or fp32 [n, hkv, head_dim].
     A negative row gives zeros."""
-    with _one_device(codes=codes, scales=scales, scale=scale, rows=rows, status=status):
-        if codes.dim() < 3 or dtype not in (torch.bfloat16, torch.float32):
-            raise MslError("kv4_rows: expected codes [..., hkv, head_dim / 2] and a bf16 or fp32 result")
-        hkv, head_dim = codes.shape[-2], 2 * codes.shape[-1]
-        have = _kv4_cache(codes, scales, hkv, head_dim, "kv4_rows")
-        _is(rows, torch.int64, (-1,), "rows"), _scalar(scale, "scale"), _status(status)
-        out = torch.empty((rows.numel(), hkv, head_dim), dtype=dtype, device=codes.device)
-        check(_lib.lib().msl_kv4_rows(codes.data_ptr(), scales.data_ptr(), scale.data_ptr(), rows.data_ptr(),
-                                      rows.numel(), hkv * head_dim, have,
-                                      OUT_F32 if dtype == torch.float32 else OUT_BF16, out.data_ptr(), _ptr(status),
-                                      _stream()), "msl_kv4_rows")
+    index = codes.get_device()
+    _device(index, (codes, scales, scale, rows, status), "codes scales scale rows status")
+    if index != torch.cuda.current_device():
+        with torch.cuda.device(index):
+            return kv4_rows(codes, scales, scale, rows, dtype, status)
+    if codes.dim() < 3 or (dtype is not torch.bfloat16 and dtype is not torch.float32):
+        raise MslError("kv4_rows: expected codes [..., hkv, head_dim / 2] and a bf16 or fp32 result")
+    hkv, head_dim, n = codes.shape[-2], 2 * codes.shape[-1], rows.numel()
+    have = _kv4_cache(codes, scales, hkv, head_dim, "kv4_rows")
+    _is(rows, torch.int64, (n,), "rows"), _scalars(scale), _status(status)
+    out = torch.empty((n, hkv, head_dim), dtype=dtype, device=codes.device)
+    check(_lib.lib().msl_kv4_rows(codes.data_ptr(), scales.data_ptr(), scale.data_ptr(), rows.data_ptr(), n,
+                                  hkv * head_dim, have, OUT_F32 if dtype is torch.float32 else OUT_BF16, out.data_ptr(),
+                                  _ptr(status), _raw_stream(index)), "msl_kv4_rows")
     return out
+
+
+@functools.lru_cache(maxsize=4096)
+def _attention_kv4_workspace(index, *sizes):
+    """msl_attention_kv4_workspace on device `index` (its SM count enters the plan)."""
+    return _lib.lib().msl_attention_kv4_workspace(*sizes)
 
 
 def attention_kv4(q, k_cache, k_sf, v_cache, v_sf, page_table, seq_lens, cu_seqlens_q, k_scale, v_scale, softmax_scale,
@@ -465,37 +490,40 @@ def attention_kv4(q, k_cache, k_sf, v_cache, v_sf, page_table, seq_lens, cu_seql
     """`attention` over the 4-bit cache: q bf16 [T, hq, head_dim] (`qk_rope_store_kv4`'s; the heads of a token must be
     contiguous), result bf16 [T, hq * head_dim].  Rows behind the last request are left as they are (undefined when
     `out` is not given); a row that sees no key is zero."""
-    with _one_device(q=q, k_cache=k_cache, k_sf=k_sf, v_cache=v_cache, v_sf=v_sf, page_table=page_table,
-                     seq_lens=seq_lens, cu_seqlens_q=cu_seqlens_q, k_scale=k_scale, v_scale=v_scale, gate=gate, out=out,
-                     status=status):
-        _heads(hq, hkv, head_dim), _need(q, torch.bfloat16, "q"), _status(status)
-        t, cols = q.shape[0], hq * head_dim
-        if q.dim() != 3 or tuple(q.shape[1:]) != (hq, head_dim) or q.stride(2) != 1 or (hq > 1 and q.stride(1) != head_dim):
-            raise MslError(f"q: expected [tokens, {hq}, {head_dim}] with contiguous heads, got {tuple(q.shape)} "
-                           f"with strides {q.stride()}")
-        _is(page_table, torch.int32, (batch, -1), "page_table"), _is(seq_lens, torch.int32, (batch,), "seq_lens")
-        _is(cu_seqlens_q, torch.int32, (batch + 1,), "cu_seqlens_q")
-        _scalar(k_scale, "k_scale"), _scalar(v_scale, "v_scale")
-        rows = _kv4_cache(k_cache, k_sf, hkv, head_dim, "k_cache")
-        if _kv4_cache(v_cache, v_sf, hkv, head_dim, "v_cache") != rows:
-            raise MslError("the key and value caches have different numbers of rows")
-        if out is None:
-            out = torch.empty((t, cols), dtype=torch.bfloat16, device=q.device)
-        for name, x in (("out", out), ("gate", gate)):
-            if x is not None:
-                _need(x, torch.bfloat16, name)
-                if _rows(x, name) < 0 or tuple(x.shape) != (t, cols):
-                    raise MslError(f"{name}: expected shape {(t, cols)}, got {tuple(x.shape)}")
-        pitch = lambda x: max(x.stride(0), cols) if t < 2 else x.stride(0)     # noqa: E731  (one row has no pitch)
-        lib = _lib.lib()
-        size = lib.msl_attention_kv4_workspace(batch, max_q_len, t, hq, hkv, head_dim, page_table.shape[1], page_size, window)
-        work = torch.empty(max(size, 16), dtype=torch.uint8, device=q.device)
-        check(lib.msl_attention_kv4(q.data_ptr(), pitch(q), k_cache.data_ptr(), k_sf.data_ptr(), v_cache.data_ptr(),
-                                    v_sf.data_ptr(), page_table.data_ptr(), page_table.shape[1], seq_lens.data_ptr(),
-                                    cu_seqlens_q.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
-                                    float(softmax_scale), batch, max_q_len, t, hq, hkv, head_dim, page_size, window,
-                                    rows, out.data_ptr(), pitch(out), _ptr(gate), 0 if gate is None else pitch(gate),
-                                    work.data_ptr(), size, _ptr(status), _stream()), "msl_attention_kv4")
+    index = q.get_device()
+    _device(index, (q, k_cache, k_sf, v_cache, v_sf, page_table, seq_lens, cu_seqlens_q, k_scale, v_scale, gate, out,
+                    status),
+            "q k_cache k_sf v_cache v_sf page_table seq_lens cu_seqlens_q k_scale v_scale gate out status")
+    if index != torch.cuda.current_device():
+        with torch.cuda.device(index):
+            return attention_kv4(q, k_cache, k_sf, v_cache, v_sf, page_table, seq_lens, cu_seqlens_q, k_scale, v_scale,
+                                 softmax_scale, batch, max_q_len, hq, hkv, head_dim, page_size, window, gate, out, status)
+    _heads(hq, hkv, head_dim), _status(status), _scalars(k_scale, v_scale)
+    t, cols = q.shape[0], hq * head_dim
+    if q.dtype is not torch.bfloat16 or q.shape != (t, hq, head_dim) or q.stride(2) != 1 or \
+            (hq > 1 and q.stride(1) != head_dim):
+        raise MslError(f"q: expected bf16 [tokens, {hq}, {head_dim}] with contiguous heads, got {q.dtype} {tuple(q.shape)}, "
+                       f"strides {q.stride()}")
+    if page_table.dim() != 2:
+        raise MslError("page_table: expected [requests, max_pages]")
+    max_pages = page_table.shape[1]
+    _is(page_table, torch.int32, (batch, max_pages), "page_table"), _is(seq_lens, torch.int32, (batch,), "seq_lens")
+    _is(cu_seqlens_q, torch.int32, (batch + 1,), "cu_seqlens_q")
+    rows = _kv4_cache(k_cache, k_sf, hkv, head_dim, "k_cache")
+    if _kv4_cache(v_cache, v_sf, hkv, head_dim, "v_cache") != rows:
+        raise MslError("the key and value caches have different numbers of rows")
+    if out is None:
+        out = torch.empty((t, cols), dtype=torch.bfloat16, device=q.device)
+    ld_out = _pitch(out, t, cols, "out")
+    ld_gate = 0 if gate is None else _pitch(gate, t, cols, "gate")
+    size = _attention_kv4_workspace(index, batch, max_q_len, t, hq, hkv, head_dim, max_pages, page_size, window)
+    work = torch.empty(size, dtype=torch.uint8, device=q.device) if size else None
+    check(_lib.lib().msl_attention_kv4(q.data_ptr(), q.stride(0) if t > 1 else cols, k_cache.data_ptr(), k_sf.data_ptr(),
+                                       v_cache.data_ptr(), v_sf.data_ptr(), page_table.data_ptr(), max_pages,
+                                       seq_lens.data_ptr(), cu_seqlens_q.data_ptr(), k_scale.data_ptr(),
+                                       v_scale.data_ptr(), softmax_scale, batch, max_q_len, t, hq, hkv, head_dim,
+                                       page_size, window, rows, out.data_ptr(), ld_out, _ptr(gate), ld_gate, _ptr(work),
+                                       size, _ptr(status), _raw_stream(index)), "msl_attention_kv4")
     return out
 
 
