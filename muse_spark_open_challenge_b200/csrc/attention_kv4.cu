@@ -19,12 +19,15 @@
 // from the accumulator's layout to the operand's by one 8 x 8 transpose in registers.  Queries (bf16) are scaled by
 // a power of two per row so that the largest magnitude lies in [2^14, 2^15) and held in f16: exact for every
 // element within 2^28 of the row's largest.  P is f16 (2^-12 relative), statistics and O are fp32.
+#include <climits>
+
 #include "kv4_common.cuh"
 
 namespace msl {
 
 constexpr int kKvWarps = 4;
 constexpr int kKvTile = 32 * kKvWarps;     // keys of a tile
+constexpr int kKvCtasPerSm = 3;
 constexpr float kKvTau = 8.0f;             // the running maximum may lag by 2^8: P stays within f16
 
 // A request as the schedule sees it: q rows [begin, begin + len), `seq` cached tokens.
@@ -91,55 +94,76 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
   return o;
 }
 
-// One lane's share of 16 keys, as loaded.
+// A warp's ring of 32-key stages in shared memory: K codes, V codes, their scales, one word with a bit per key that has
+// a cache row.  Filled by cp.async straight from the pages; kStages - 1 of them are in flight while one is computed.
+// A lane's V words (one per key, keys 2 apart) would fall into the same banks: within each 128 bytes the 16-byte units
+// are permuted by the row.
 template <int D>
-struct Kv4Frag {
-  static constexpr int KW = D / 32;        // words of K codes per key (D / 4 channels)
-  static constexpr int VW = D / 64;        // words of V codes per key (D / 8 channels)
-  uint32_t k[2][KW], v[4][VW];
-  uint32_t ks[2], vs[4];
+struct Kv4Ring {
+  static constexpr int kRowBytes = D / 2, kChunks = D / 32, kSfBytes = D / 16;
+  static constexpr int kV = 32 * kRowBytes, kKs = 2 * kV, kVs = kKs + 32 * kSfBytes, kHeld = kVs + 32 * kSfBytes;
+  static constexpr int kStage = kHeld + 16;
+  static constexpr int kStages = 4;
+  static constexpr int kWarp = kStages * kStage;
 };
-
 template <int D>
-__device__ __forceinline__ void kv4_load(Kv4Frag<D>& f, const Kv4Args& p, int kvh, int rows, int half, int lane) {
-  const int g = lane >> 2, t = lane & 3;
+__device__ __forceinline__ uint32_t kv4_v_offset(int row, int byte) {   // byte < D / 2 of a V row
+  constexpr int kPer = D == 128 ? 2 : 4;                    // rows per 128 bytes
+  constexpr int kShift = D == 128 ? 1 : 2;
+  const int unit = (row & (kPer - 1)) * Kv4Ring<D>::kChunks + (byte >> 4);
+  return (row >> kShift) * 128 + ((unit ^ (2 * ((row >> kShift) & (D == 128 ? 3 : 1)))) << 4) + (byte & 15);
+}
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, int bytes) {   // fewer bytes: zeros behind them
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+template <int N>
+__device__ __forceinline__ void cp_async_small(uint32_t dst, const void* src, int bytes) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(N), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+// Start copying the 32 keys whose cache rows the lanes hold (-1: zeros).
+template <int D>
+__device__ __forceinline__ void kv4_issue(const Kv4Args& p, uint8_t* stage, int kvh, int row, int lane) {
+  using S = Kv4Ring<D>;
+  const uint32_t base = smem_u32(stage);
+  const uint32_t mask = __ballot_sync(0xffffffffu, row >= 0);
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int row = __shfl_sync(0xffffffffu, rows, 16 * half + g + 8 * i);
-    const int64_t at = static_cast<int64_t>(row) * p.hkv + kvh;
-    f.ks[i] = 0;
-#pragma unroll
-    for (int w = 0; w < Kv4Frag<D>::KW; ++w) f.k[i][w] = 0;
-    if (row >= 0) {
-      if constexpr (D == 128) {
-        const uint4 c = *reinterpret_cast<const uint4*>(p.k + at * 64 + t * 16);
-        f.k[i][0] = c.x; f.k[i][1] = c.y; f.k[i][2] = c.z; f.k[i][3] = c.w;
-        f.ks[i] = *reinterpret_cast<const uint16_t*>(p.ks + at * 8 + t * 2);
-      } else {
-        const uint2 c = *reinterpret_cast<const uint2*>(p.k + at * 32 + t * 8);
-        f.k[i][0] = c.x; f.k[i][1] = c.y;
-        f.ks[i] = p.ks[at * 4 + t];
-      }
-    }
+  for (int i = 0; i < S::kChunks; ++i) {
+    const int r = (32 / S::kChunks) * i + lane / S::kChunks, c = lane % S::kChunks;
+    const int from = __shfl_sync(0xffffffffu, row, r);
+    const int64_t off = (static_cast<int64_t>(max(from, 0)) * p.hkv + kvh) * S::kRowBytes + c * 16;
+    const int bytes = from >= 0 ? 16 : 0;
+    cp_async16(base + r * S::kRowBytes + c * 16, p.k + off, bytes);
+    cp_async16(base + S::kV + kv4_v_offset<D>(r, c * 16), p.v + off, bytes);
   }
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int row = __shfl_sync(0xffffffffu, rows, 16 * half + 2 * t + (i & 1) + 8 * (i >> 1));
-    const int64_t at = static_cast<int64_t>(row) * p.hkv + kvh;
-    f.vs[i] = 0;
-#pragma unroll
-    for (int w = 0; w < Kv4Frag<D>::VW; ++w) f.v[i][w] = 0;
-    if (row >= 0) {
-      if constexpr (D == 128) {
-        const uint2 c = *reinterpret_cast<const uint2*>(p.v + at * 64 + g * 8);
-        f.v[i][0] = c.x; f.v[i][1] = c.y;
-        f.vs[i] = p.vs[at * 8 + g];
-      } else {
-        f.v[i][0] = *reinterpret_cast<const uint32_t*>(p.v + at * 32 + g * 4);
-        f.vs[i] = p.vs[at * 4 + g / 2];
-      }
-    }
+  const int64_t off = (static_cast<int64_t>(max(row, 0)) * p.hkv + kvh) * S::kSfBytes;
+  const int bytes = row >= 0 ? S::kSfBytes : 0;
+  cp_async_small<S::kSfBytes>(base + S::kKs + lane * S::kSfBytes, p.ks + off, bytes);
+  cp_async_small<S::kSfBytes>(base + S::kVs + lane * S::kSfBytes, p.vs + off, bytes);
+  if (lane == 0) *reinterpret_cast<uint32_t*>(stage + S::kHeld) = mask;
+}
+
+// A key's page table entry, loaded a step before its row is needed.
+struct Kv4Page {
+  int page, off;                            // page INT_MIN: the key is hidden from every row
+};
+__device__ __forceinline__ Kv4Page kv4_page(const Kv4Args& p, const int* table, int key, int lo, int hi) {
+  Kv4Page x{INT_MIN, 0};
+  if (key >= lo && key < hi) {
+    const int idx = p.page_shift >= 0 ? key >> p.page_shift : key / p.page_size;
+    x.off = key - idx * p.page_size;
+    x.page = idx < p.max_pages ? table[idx] : -1;
   }
+  return x;
+}
+__device__ __forceinline__ int kv4_row_of(const Kv4Args& p, const Kv4Page& x) {
+  const int64_t row = static_cast<int64_t>(x.page) * p.page_size + x.off;
+  if (x.page >= 0 && row < p.cache_rows) return static_cast<int>(row);
+  if (x.page != INT_MIN) report_error(p.status, MSL_ERR_CAPACITY);
+  return -1;
 }
 
 // Shared-memory layout of a warp's O [R][D]: channel d of the lane group D/8 at pitch D/8 + 2, so that the float2
@@ -151,18 +175,23 @@ struct Kv4Merge {
 };
 
 template <int D, int NB>
-__global__ void __launch_bounds__(32 * kKvWarps)
+__global__ void __launch_bounds__(32 * kKvWarps, kKvCtasPerSm)
 attention_kv4_kernel(Kv4Args p) {
   constexpr int R = 8 * NB;
   constexpr int KS = D / 16;               // MMA steps of Q K^T, and 16-row tiles of O^T
   using M = Kv4Merge<D>;
-  __shared__ float sm_o[kKvWarps][R][M::kRow];
+  using S = Kv4Ring<D>;
+  static_assert(R * M::kRow * 4 <= S::kWarp, "a warp's O takes the place of its ring");
+  extern __shared__ __align__(128) uint8_t kv4_smem[];
+  const auto sm_o = [&](int w, int row) { return reinterpret_cast<float*>(kv4_smem + w * S::kWarp) + row * M::kRow; };
   __shared__ float sm_m[kKvWarps][R], sm_l[kKvWarps][R];
   __shared__ int64_t scratch[kKvWarps];
   __shared__ int sm_b;
   __shared__ int64_t sm_at;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   const int G = p.hq / p.hkv;
+  uint8_t* ring = kv4_smem + warp * S::kWarp;
+  pdl_launch_dependents();
 
   // ---- this worker's range of tiles
   const int per = (p.batch + blockDim.x - 1) / blockDim.x;
@@ -271,16 +300,31 @@ attention_kv4_kernel(Kv4Args p) {
         }
         // ---- the keys, 32 a step
         const int key_first = (span.first + off) * kKvTile + warp * 32;
-        int row_cur = kv4_row(p, table, key_first + lane, lo, hi);
-        Kv4Frag<D> f[2];
-        kv4_load<D>(f[0], p, kvh, row_cur, 0, lane);
-        kv4_load<D>(f[1], p, kvh, row_cur, 1, lane);
-        int row_next = n > 1 ? kv4_row(p, table, key_first + kKvTile + lane, lo, hi) : -1;
+        const auto page_of = [&](int j) {
+          return j < n ? kv4_page(p, table, key_first + j * kKvTile + lane, lo, hi) : Kv4Page{INT_MIN, 0};
+        };
+        Kv4Page ahead[S::kStages];
+#pragma unroll
+        for (int j = 0; j < S::kStages; ++j) ahead[j] = page_of(j);
+#pragma unroll
+        for (int j = 0; j < S::kStages - 1; ++j) {
+          if (j < n) kv4_issue<D>(p, ring + j * S::kStage, kvh, kv4_row_of(p, ahead[j]), lane);
+          cp_async_commit();
+        }
+        Kv4Page page_next = ahead[S::kStages - 1];          // of step j + kStages - 1
+        int slot = 0;
         for (int j = 0; j < n; ++j) {
           const int key0 = key_first + j * kKvTile;
-          const bool partial = __any_sync(0xffffffffu, row_cur < 0) || key0 < all_lo || key0 + 32 > all_hi;
-          uint32_t vmem[2][4][Kv4Frag<D>::VW];
-          uint32_t vsc[2][4];
+          uint8_t* stage = ring + slot * S::kStage;
+          cp_async_wait<S::kStages - 2>();
+          __syncwarp();                                     // every lane's copies are in, and the last slot is free
+          if (j + S::kStages - 1 < n)
+            kv4_issue<D>(p, ring + (slot == 0 ? S::kStages - 1 : slot - 1) * S::kStage, kvh, kv4_row_of(p, page_next), lane);
+          cp_async_commit();
+          page_next = page_of(j + S::kStages);
+          slot = slot + 1 == S::kStages ? 0 : slot + 1;
+          const uint32_t held = *reinterpret_cast<const uint32_t*>(stage + S::kHeld);
+          const bool partial = held != 0xffffffffu || key0 < all_lo || key0 + 32 > all_hi;
           float s[2][NB][4];
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
@@ -288,14 +332,26 @@ attention_kv4_kernel(Kv4Args p) {
             for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
               for (int c = 0; c < 4; ++c) s[h][nb][c] = 0.f;
+            uint32_t k[2][D / 32];
             __half2 sc[2];
 #pragma unroll
-            for (int x = 0; x < 2; ++x) sc[x] = scales_h2(f[h].ks[x]);
+            for (int x = 0; x < 2; ++x) {
+              const int row = 16 * h + 8 * x + g;
+              if constexpr (D == 128) {
+                const uint4 v = *reinterpret_cast<const uint4*>(stage + row * 64 + t * 16);
+                k[x][0] = v.x; k[x][1] = v.y; k[x][2] = v.z; k[x][3] = v.w;
+                sc[x] = scales_h2(*reinterpret_cast<const uint16_t*>(stage + S::kKs + row * 8 + t * 2));
+              } else {
+                const uint2 v = *reinterpret_cast<const uint2*>(stage + row * 32 + t * 8);
+                k[x][0] = v.x; k[x][1] = v.y;
+                sc[x] = scales_h2(stage[S::kKs + row * 4 + t]);
+              }
+            }
 #pragma unroll
-            for (int w = 0; w < Kv4Frag<D>::KW; ++w) {      // one word = two MMA steps
+            for (int w = 0; w < D / 32; ++w) {              // one word = two MMA steps
               __half2 a[4], c[4];
-              e2m1x8(f[h].k[0][w], a);
-              e2m1x8(f[h].k[1][w], c);
+              e2m1x8(k[0][w], a);
+              e2m1x8(k[1][w], c);
               const bool second = D == 128 && w >= 2;       // which of the lane's two scale blocks
               const __half2 s0 = second ? __high2half2(sc[0]) : __low2half2(sc[0]);
               const __half2 s1 = second ? __high2half2(sc[1]) : __low2half2(sc[1]);
@@ -309,19 +365,6 @@ attention_kv4_kernel(Kv4Args p) {
                           qf[nb][2 * w + 1][1]);
               }
             }
-#pragma unroll
-            for (int x = 0; x < 4; ++x) {
-              vsc[h][x] = f[h].vs[x];
-#pragma unroll
-              for (int w = 0; w < Kv4Frag<D>::VW; ++w) vmem[h][x][w] = f[h].v[x][w];
-            }
-          }
-          const int row_was = row_cur;
-          if (j + 1 < n) {                                  // the next 32 keys are on their way during the rest
-            row_cur = row_next;
-            kv4_load<D>(f[0], p, kvh, row_cur, 0, lane);
-            kv4_load<D>(f[1], p, kvh, row_cur, 1, lane);
-            row_next = j + 2 < n ? kv4_row(p, table, key0 + 2 * kKvTile + lane, lo, hi) : -1;
           }
           // ---- scores in log2 units, masked where some row does not see a key
 #pragma unroll
@@ -336,13 +379,12 @@ attention_kv4_kernel(Kv4Args p) {
 #pragma unroll
               for (int x = 0; x < 2; ++x) {
                 const int kk = 16 * h + g + 8 * x;
-                const bool held = __shfl_sync(0xffffffffu, row_was, kk) >= 0;
 #pragma unroll
                 for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
                   for (int c = 0; c < 2; ++c) {
                     const int key = key0 + kk;
-                    const bool seen = held && key <= qpos[nb][c] && (!p.window || key > qpos[nb][c] - p.window);
+                    const bool seen = ((held >> kk) & 1u) && key <= qpos[nb][c] && (!p.window || key > qpos[nb][c] - p.window);
                     if (!seen) s[h][nb][2 * x + c] = -INFINITY;
                   }
               }
@@ -392,15 +434,30 @@ attention_kv4_kernel(Kv4Args p) {
           // ---- O^T += V^T P^T
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            const __half2 s01 = scales_h2(vsc[h][0] | (vsc[h][1] << 8));
-            const __half2 s23 = scales_h2(vsc[h][2] | (vsc[h][3] << 8));
+            uint32_t v[4][D / 64];
+            uint32_t vs[4];
 #pragma unroll
-            for (int w = 0; w < Kv4Frag<D>::VW; ++w) {      // one word a key = four 16-row tiles
+            for (int x = 0; x < 4; ++x) {
+              const int row = 16 * h + 2 * t + (x & 1) + 8 * (x >> 1);
+              const uint8_t* src = stage + S::kV + kv4_v_offset<D>(row, g * (D / 16));
+              if constexpr (D == 128) {
+                const uint2 u = *reinterpret_cast<const uint2*>(src);
+                v[x][0] = u.x; v[x][1] = u.y;
+                vs[x] = stage[S::kVs + row * 8 + g];
+              } else {
+                v[x][0] = *reinterpret_cast<const uint32_t*>(src);
+                vs[x] = stage[S::kVs + row * 4 + g / 2];
+              }
+            }
+            const __half2 s01 = scales_h2(vs[0] | (vs[1] << 8));
+            const __half2 s23 = scales_h2(vs[2] | (vs[3] << 8));
+#pragma unroll
+            for (int w = 0; w < D / 64; ++w) {              // one word a key = four 16-row tiles
               // pairs along the keys: low nibbles (even channels, MMA rows g) and high ones (odd, g + 8)
-              const uint32_t lo01 = (vmem[h][0][w] & 0x0f0f0f0fu) | ((vmem[h][1][w] << 4) & 0xf0f0f0f0u);
-              const uint32_t hi01 = ((vmem[h][0][w] >> 4) & 0x0f0f0f0fu) | (vmem[h][1][w] & 0xf0f0f0f0u);
-              const uint32_t lo23 = (vmem[h][2][w] & 0x0f0f0f0fu) | ((vmem[h][3][w] << 4) & 0xf0f0f0f0u);
-              const uint32_t hi23 = ((vmem[h][2][w] >> 4) & 0x0f0f0f0fu) | (vmem[h][3][w] & 0xf0f0f0f0u);
+              const uint32_t lo01 = (v[0][w] & 0x0f0f0f0fu) | ((v[1][w] << 4) & 0xf0f0f0f0u);
+              const uint32_t hi01 = ((v[0][w] >> 4) & 0x0f0f0f0fu) | (v[1][w] & 0xf0f0f0f0u);
+              const uint32_t lo23 = (v[2][w] & 0x0f0f0f0fu) | ((v[3][w] << 4) & 0xf0f0f0f0u);
+              const uint32_t hi23 = ((v[2][w] >> 4) & 0x0f0f0f0fu) | (v[3][w] & 0xf0f0f0f0u);
               __half2 a0[4], a1[4], a2[4], a3[4];
               e2m1x8(lo01, a0);
               e2m1x8(hi01, a1);
@@ -417,6 +474,7 @@ attention_kv4_kernel(Kv4Args p) {
             }
           }
         }
+        __syncwarp();                                       // the ring is read; O takes its place
         // ---- join the four warps
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) {
@@ -429,7 +487,7 @@ attention_kv4_kernel(Kv4Args p) {
             if (g == 0) { sm_m[warp][row] = m[nb][c]; sm_l[warp][row] = x; }
 #pragma unroll
             for (int k = 0; k < KS; ++k)
-              *reinterpret_cast<float2*>(&sm_o[warp][row][g * M::kGroup + 2 * k]) =
+              *reinterpret_cast<float2*>(sm_o(warp, row) + g * M::kGroup + 2 * k) =
                   make_float2(o[nb][k][c], o[nb][k][2 + c]);
           }
         }
@@ -452,7 +510,7 @@ attention_kv4_kernel(Kv4Args p) {
 #pragma unroll
             for (int x = 0; x < D / 32; ++x) {
               const int d = lane * (D / 32) + x;
-              acc[x] += sm_o[w][row][(d / (D / 8)) * M::kGroup + d % (D / 8)] * c;
+              acc[x] += sm_o(w, row)[(d / (D / 8)) * M::kGroup + d % (D / 8)] * c;
             }
           }
           if (whole) {
@@ -493,6 +551,7 @@ kv4_merge_kernel(Kv4Args p) {
   before = block_sum_i64(before, scratch);
   all = block_sum_i64(all, scratch);
   const Kv4Req r = kv4_request(p, b);
+  pdl_wait();                               // in every block: this grid ends only after the one before it
   if (i * R >= r.len * G) return;
   for (int x = 0; x < i; ++x) {
     const Kv4Span s = kv4_span<R>(p, r, G, x);
@@ -507,34 +566,62 @@ kv4_merge_kernel(Kv4Args p) {
   if (w0 == w1) return;
   const int rows = min(R, r.len * G - i * R);
   for (int row = warp; row < rows; row += kKvWarps) {
+    const auto at = [&](int64_t w) { return p.part + ((w * 2 + (w == w0 ? 1 : 0)) * R + row) * (D + 2); };
     float mx = -INFINITY;
-    for (int64_t w = w0; w <= w1; ++w) mx = fmaxf(mx, p.part[((w * 2 + (w == w0 ? 1 : 0)) * R + row) * (D + 2)]);
+    for (int64_t w = w0 + lane; w <= w1; w += 32) mx = fmaxf(mx, at(w)[0]);
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
+    const float ref = mx == -INFINITY ? 0.f : mx;
     float acc[PER], sum = 0.f;
 #pragma unroll
     for (int x = 0; x < PER; ++x) acc[x] = 0.f;
-    for (int64_t w = w0; w <= w1; ++w) {
-      const float* src = p.part + ((w * 2 + (w == w0 ? 1 : 0)) * R + row) * (D + 2);
-      const float c = kv_ex2(src[0] - (mx == -INFINITY ? 0.f : mx));
-      sum += src[1] * c;
+    for (int64_t w32 = w0; w32 <= w1; w32 += 32) {          // a lane forms the weight of one worker
+      float c = 0.f;
+      if (w32 + lane <= w1) {
+        const float* src = at(w32 + lane);
+        c = kv_ex2(src[0] - ref);
+        sum += src[1] * c;
+      }
+      const int n = static_cast<int>(min(w1 - w32 + 1, static_cast<int64_t>(32)));
+#pragma unroll 8
+      for (int w = 0; w < n; ++w) {
+        const float cw = __shfl_sync(0xffffffffu, c, w);
+        const float* src = at(w32 + w) + 2 + lane * PER;
 #pragma unroll
-      for (int x = 0; x < PER; ++x) acc[x] += src[2 + lane * PER + x] * c;
+        for (int x = 0; x < PER; x += 2) {
+          const float2 v = *reinterpret_cast<const float2*>(src + x);
+          acc[x] += v.x * cw;
+          acc[x + 1] += v.y * cw;
+        }
+      }
     }
+    sum = warp_sum(sum);
     const int tok = (i * R + row) / G, head = kvh * G + (i * R + row) % G;
     kv4_write_row<D>(p, acc, sum, static_cast<int64_t>(r.begin) + tok, head, lane);
   }
 }
 
-constexpr int kKvCtasPerSm = 3;
-
 template <int D, int NB>
 static int launch_kv4(const Kv4Args& a, cudaStream_t st) {
   constexpr int R = 8 * NB;
-  attention_kv4_kernel<D, NB><<<a.workers, 32 * kKvWarps, 0, st>>>(a);
+  constexpr int smem = kKvWarps * Kv4Ring<D>::kWarp;
+  static SmemConfig config;
+  if (int rc = config.ensure(attention_kv4_kernel<D, NB>, smem)) return rc;
+  attention_kv4_kernel<D, NB><<<a.workers, 32 * kKvWarps, smem, st>>>(a);
+  if (cudaGetLastError() != cudaSuccess) return MSL_ERR_CUDA;
   const int G = a.hq / a.hkv;
   const int64_t blocks = (static_cast<int64_t>(a.max_q_len) * G + R - 1) / R;
-  const dim3 grid(static_cast<unsigned>(blocks * a.hkv), a.batch);
-  kv4_merge_kernel<D, NB><<<grid, 32 * kKvWarps, 0, st>>>(a);
-  return cudaGetLastError() == cudaSuccess ? MSL_OK : MSL_ERR_CUDA;
+  // The merge forms its schedule while the attention runs and waits for it on the device (programmatic launch).
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(blocks * a.hkv), a.batch);
+  cfg.blockDim = dim3(32 * kKvWarps);
+  cfg.stream = st;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kv4_merge_kernel<D, NB>, a) == cudaSuccess ? MSL_OK : MSL_ERR_CUDA;
 }
 
 // Query rows a CTA holds: one MMA column block of 8 where the group's rows fit, else two.
@@ -605,11 +692,14 @@ extern "C" int msl_attention_kv4(const void* q, int64_t ld_q, const void* k_cach
     return MSL_ERR_ALIGN;
   if (workspace_bytes < plan.bytes) return MSL_ERR_CAPACITY;
   const auto u8 = [](const void* x) { return static_cast<const uint8_t*>(x); };
+  int page_shift = -1;
+  if ((page_size & (page_size - 1)) == 0)
+    for (page_shift = 0; (1 << page_shift) < page_size; ++page_shift) {}
   const Kv4Args a{static_cast<const __nv_bfloat16*>(q), ld_q, u8(k_cache), u8(k_sf), u8(v_cache), u8(v_sf),
                   page_table, max_pages, seq_lens, cu_seqlens_q, k_scale, v_scale, softmax_scale, batch, max_q_len,
                   tokens, hq, hkv, page_size, window, cache_rows, static_cast<__nv_bfloat16*>(out), ld_out,
                   static_cast<const __nv_bfloat16*>(gate), ld_gate, static_cast<float*>(workspace),
-                  sm_count() * kKvCtasPerSm, plan.splits, status};
+                  sm_count() * kKvCtasPerSm, plan.splits, page_shift, status};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (!plan.few) return launch_kv4_tc(a, head_dim, st);
   if (kv4_row_blocks(static_cast<int64_t>(max_q_len) * G) == 1)

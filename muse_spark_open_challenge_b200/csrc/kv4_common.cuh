@@ -28,6 +28,7 @@ struct Kv4Args {
   float* part;                  // partial results (workspace)
   int workers;                  // few rows: CTAs that share the key tiles
   int kv_splits;                // many rows: slices of a query block's keys
+  int page_shift;               // log2 of the page size, -1: not a power of two
   int* status;
 };
 
@@ -54,10 +55,14 @@ __device__ __forceinline__ __half2 scales_h2(uint32_t two) {
   asm("{.reg .b16 x;\n\tcvt.u16.u32 x, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, x;}" : "=r"(h) : "r"(two));
   return __hmin2(bits_h2(h), __half2half2(__ushort_as_half(0x5F00)));   // 448
 }
+// Programmatic launch: the next kernel's blocks may start; wait until the kernel before has ended and its writes show.
+__device__ __forceinline__ void pdl_launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 // The cache row of key `key` (-1: hidden from every row of the block, or no valid page).
 __device__ __forceinline__ int kv4_row(const Kv4Args& p, const int* table, int key, int lo, int hi) {
   if (key < lo || key >= hi) return -1;
-  const int idx = key / p.page_size;
+  const int idx = p.page_shift >= 0 ? key >> p.page_shift : key / p.page_size;
   const int page = idx < p.max_pages ? table[idx] : -1;
   const int64_t row = static_cast<int64_t>(page) * p.page_size + (key - idx * p.page_size);
   if (page < 0 || row >= p.cache_rows) {
