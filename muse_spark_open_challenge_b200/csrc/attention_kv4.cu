@@ -25,9 +25,6 @@
 
 namespace msl {
 
-constexpr int kKvWarps = 4;
-constexpr int kKvTile = 32 * kKvWarps;     // keys of a tile
-constexpr int kKvCtasPerSm = 3;
 constexpr float kKvTau = 8.0f;             // the running maximum may lag by 2^8: P stays within f16
 
 // A request as the schedule sees it: q rows [begin, begin + len), `seq` cached tokens.
@@ -55,8 +52,8 @@ __device__ __forceinline__ Kv4Span kv4_span(const Kv4Args& p, const Kv4Req& r, i
                                       static_cast<int64_t>(p.max_pages) * p.page_size));
   const int lo = p.window ? max(0, r.seq + low_tok - p.window + 1) : 0;
   Kv4Span s;
-  s.first = lo / kKvTile;
-  s.last = max(s.first + 1, (hi + kKvTile - 1) / kKvTile);   // a row block with nothing to see still writes its zeros
+  s.first = lo >> p.tile_shift;
+  s.last = max(s.first + 1, (hi + (1 << p.tile_shift) - 1) >> p.tile_shift);   // with nothing to see: zeros are written
   return s;
 }
 template <int R>
@@ -67,30 +64,31 @@ __device__ __forceinline__ int64_t kv4_tiles(const Kv4Args& p, const Kv4Req& r, 
     const Kv4Span s = kv4_span<R>(p, r, G, i);
     sum += s.last - s.first;
   }
-  return sum * p.hkv;
+  return sum * (p.hkv / p.heads);
 }
 
+template <int W>
 __device__ __forceinline__ int64_t block_sum_i64(int64_t v, int64_t* scratch) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = v;
   __syncthreads();
   int64_t s = 0;
-  for (int w = 0; w < kKvWarps; ++w) s += scratch[w];
+  for (int w = 0; w < W; ++w) s += scratch[w];
   __syncthreads();
   return s;
 }
 
 __device__ __forceinline__ void mma_16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
                                           uint32_t b0, uint32_t b1) {
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
       "{%0, %1, %2, %3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
   uint32_t o;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(o) : "r"(v));
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(o) : "r"(v));
   return o;
 }
 
@@ -103,7 +101,7 @@ struct Kv4Ring {
   static constexpr int kRowBytes = D / 2, kChunks = D / 32, kSfBytes = D / 16;
   static constexpr int kV = 32 * kRowBytes, kKs = 2 * kV, kVs = kKs + 32 * kSfBytes, kHeld = kVs + 32 * kSfBytes;
   static constexpr int kStage = kHeld + 16;
-  static constexpr int kStages = 4;
+  static constexpr int kStages = 3;
   static constexpr int kWarp = kStages * kStage;
 };
 template <int D>
@@ -124,25 +122,38 @@ __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commi
 template <int N>
 __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
+// Where a lane's copies start: the KV head's bytes of cache row 0, and the lane's 16-byte unit of them.
+struct Kv4Source {
+  const uint8_t *k, *v, *ks, *vs;
+  int64_t pitch, sf_pitch;                  // bytes of a cache row (all heads)
+};
+template <int D>
+__device__ __forceinline__ Kv4Source kv4_source(const Kv4Args& p, int kvh, int lane) {
+  using S = Kv4Ring<D>;
+  const int at = kvh * S::kRowBytes + (lane % S::kChunks) * 16;
+  return {p.k + at, p.v + at, p.ks + kvh * S::kSfBytes, p.vs + kvh * S::kSfBytes,
+          static_cast<int64_t>(p.hkv) * S::kRowBytes, static_cast<int64_t>(p.hkv) * S::kSfBytes};
+}
+
 // Start copying the 32 keys whose cache rows the lanes hold (-1: zeros).
 template <int D>
-__device__ __forceinline__ void kv4_issue(const Kv4Args& p, uint8_t* stage, int kvh, int row, int lane) {
+__device__ __forceinline__ void kv4_issue(const Kv4Source& src, uint8_t* stage, int row, int lane) {
   using S = Kv4Ring<D>;
   const uint32_t base = smem_u32(stage);
   const uint32_t mask = __ballot_sync(0xffffffffu, row >= 0);
+  const int safe = max(row, 0);
 #pragma unroll
   for (int i = 0; i < S::kChunks; ++i) {
-    const int r = (32 / S::kChunks) * i + lane / S::kChunks, c = lane % S::kChunks;
-    const int from = __shfl_sync(0xffffffffu, row, r);
-    const int64_t off = (static_cast<int64_t>(max(from, 0)) * p.hkv + kvh) * S::kRowBytes + c * 16;
-    const int bytes = from >= 0 ? 16 : 0;
-    cp_async16(base + r * S::kRowBytes + c * 16, p.k + off, bytes);
-    cp_async16(base + S::kV + kv4_v_offset<D>(r, c * 16), p.v + off, bytes);
+    constexpr int kRows = 32 / S::kChunks;                  // rows a round covers
+    const int r = kRows * i + lane / S::kChunks, c = lane % S::kChunks;
+    const int from = __shfl_sync(0xffffffffu, safe, r);
+    const int bytes = (mask >> r) & 1u ? 16 : 0;
+    cp_async16(base + r * S::kRowBytes + c * 16, src.k + from * src.pitch, bytes);
+    cp_async16(base + S::kV + kv4_v_offset<D>(r, c * 16), src.v + from * src.pitch, bytes);
   }
-  const int64_t off = (static_cast<int64_t>(max(row, 0)) * p.hkv + kvh) * S::kSfBytes;
   const int bytes = row >= 0 ? S::kSfBytes : 0;
-  cp_async_small<S::kSfBytes>(base + S::kKs + lane * S::kSfBytes, p.ks + off, bytes);
-  cp_async_small<S::kSfBytes>(base + S::kVs + lane * S::kSfBytes, p.vs + off, bytes);
+  cp_async_small<S::kSfBytes>(base + S::kKs + lane * S::kSfBytes, src.ks + safe * src.sf_pitch, bytes);
+  cp_async_small<S::kSfBytes>(base + S::kVs + lane * S::kSfBytes, src.vs + safe * src.sf_pitch, bytes);
   if (lane == 0) *reinterpret_cast<uint32_t*>(stage + S::kHeld) = mask;
 }
 
@@ -174,8 +185,17 @@ struct Kv4Merge {
   static constexpr int kRow = 8 * kGroup + 8;
 };
 
+// W warps a CTA.  p.heads of them (a power of two) take one KV head each, the W / p.heads groups of them 32 keys each:
+// a cache row's heads lie side by side, and fetching them together is what keeps DRAM traffic at the bytes needed.
 template <int D, int NB>
-__global__ void __launch_bounds__(32 * kKvWarps, kKvCtasPerSm)
+struct Kv4Shape {
+  static constexpr bool kSlim = D == 64 || NB == 1;        // fits 128 registers
+  static constexpr int kWarps = kSlim ? 8 : 4;
+  static constexpr int kCtas = kSlim ? 2 : 3;              // per SM
+};
+
+template <int D, int NB, int W>
+__global__ void __launch_bounds__(32 * W, Kv4Shape<D, NB>::kCtas)
 attention_kv4_kernel(Kv4Args p) {
   constexpr int R = 8 * NB;
   constexpr int KS = D / 16;               // MMA steps of Q K^T, and 16-row tiles of O^T
@@ -184,8 +204,8 @@ attention_kv4_kernel(Kv4Args p) {
   static_assert(R * M::kRow * 4 <= S::kWarp, "a warp's O takes the place of its ring");
   extern __shared__ __align__(128) uint8_t kv4_smem[];
   const auto sm_o = [&](int w, int row) { return reinterpret_cast<float*>(kv4_smem + w * S::kWarp) + row * M::kRow; };
-  __shared__ float sm_m[kKvWarps][R], sm_l[kKvWarps][R];
-  __shared__ int64_t scratch[kKvWarps];
+  __shared__ float sm_m[W][R], sm_l[W][R];
+  __shared__ int64_t scratch[W];
   __shared__ int sm_b;
   __shared__ int64_t sm_at;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
@@ -207,7 +227,7 @@ attention_kv4_kernel(Kv4Args p) {
   if (lane == 31) scratch[warp] = inc;
   __syncthreads();
   int64_t total = 0;
-  for (int w = 0; w < kKvWarps; ++w) {
+  for (int w = 0; w < W; ++w) {
     if (w < warp) inc += scratch[w];
     total += scratch[w];
   }
@@ -231,6 +251,8 @@ attention_kv4_kernel(Kv4Args p) {
   int64_t skip = at - sm_at;                                // tiles of request b before this range
   const float scale_log2 = p.softmax_scale * (*p.k_scale) * 1.4426950408889634f;
 
+  const int groups = p.hkv / p.heads, my_head = warp & (p.heads - 1), n_sub = W / p.heads;
+
   for (; at < end && b < p.batch; ++b) {
     const Kv4Req r = kv4_request(p, b);
     const int blocks = (r.len * G + R - 1) / R;
@@ -238,8 +260,9 @@ attention_kv4_kernel(Kv4Args p) {
     for (int i = 0; i < blocks && at < end; ++i) {
       const Kv4Span span = kv4_span<R>(p, r, G, i);
       const int n_span = span.last - span.first;
-      if (skip >= static_cast<int64_t>(n_span) * p.hkv) { skip -= static_cast<int64_t>(n_span) * p.hkv; continue; }
-      for (int kvh = static_cast<int>(skip / n_span); kvh < p.hkv && at < end; ++kvh) {
+      if (skip >= static_cast<int64_t>(n_span) * groups) { skip -= static_cast<int64_t>(n_span) * groups; continue; }
+      for (int group = static_cast<int>(skip / n_span); group < groups && at < end; ++group) {
+        const int kvh = group * p.heads + my_head;
         const int off = static_cast<int>(skip % n_span);
         skip = 0;
         const int n = static_cast<int>(min(end - at, static_cast<int64_t>(n_span - off)));
@@ -299,27 +322,29 @@ attention_kv4_kernel(Kv4Args p) {
             for (int c = 0; c < 4; ++c) o[nb][k][c] = 0.f;
         }
         // ---- the keys, 32 a step
-        const int key_first = (span.first + off) * kKvTile + warp * 32;
+        const int tile = 1 << p.tile_shift;
+        const int key_first = (span.first + off) * tile + (warp / p.heads) * 32;
         const auto page_of = [&](int j) {
-          return j < n ? kv4_page(p, table, key_first + j * kKvTile + lane, lo, hi) : Kv4Page{INT_MIN, 0};
+          return j < n ? kv4_page(p, table, key_first + j * tile + lane, lo, hi) : Kv4Page{INT_MIN, 0};
         };
+        const Kv4Source source = kv4_source<D>(p, kvh, lane);
         Kv4Page ahead[S::kStages];
 #pragma unroll
         for (int j = 0; j < S::kStages; ++j) ahead[j] = page_of(j);
 #pragma unroll
         for (int j = 0; j < S::kStages - 1; ++j) {
-          if (j < n) kv4_issue<D>(p, ring + j * S::kStage, kvh, kv4_row_of(p, ahead[j]), lane);
+          if (j < n) kv4_issue<D>(source, ring + j * S::kStage, kv4_row_of(p, ahead[j]), lane);
           cp_async_commit();
         }
         Kv4Page page_next = ahead[S::kStages - 1];          // of step j + kStages - 1
         int slot = 0;
         for (int j = 0; j < n; ++j) {
-          const int key0 = key_first + j * kKvTile;
+          const int key0 = key_first + j * tile;
           uint8_t* stage = ring + slot * S::kStage;
           cp_async_wait<S::kStages - 2>();
           __syncwarp();                                     // every lane's copies are in, and the last slot is free
           if (j + S::kStages - 1 < n)
-            kv4_issue<D>(p, ring + (slot == 0 ? S::kStages - 1 : slot - 1) * S::kStage, kvh, kv4_row_of(p, page_next), lane);
+            kv4_issue<D>(source, ring + (slot == 0 ? S::kStages - 1 : slot - 1) * S::kStage, kv4_row_of(p, page_next), lane);
           cp_async_commit();
           page_next = page_of(j + S::kStages);
           slot = slot + 1 == S::kStages ? 0 : slot + 1;
@@ -475,7 +500,7 @@ attention_kv4_kernel(Kv4Args p) {
           }
         }
         __syncwarp();                                       // the ring is read; O takes its place
-        // ---- join the four warps
+        // ---- join the warps of a head
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) {
 #pragma unroll
@@ -495,16 +520,16 @@ attention_kv4_kernel(Kv4Args p) {
         const bool whole = n == n_span;
         // a worker has at most two partial results: the rest of an item that an earlier worker began (slot 0) and
         // the beginning of one that a later worker ends (slot 1)
-        float* part = p.part + (static_cast<int64_t>(blockIdx.x) * 2 + (off == 0 ? 1 : 0)) * R * (D + 2);
-        for (int row = warp; row < rows; row += kKvWarps) {
+        float* part = p.part + (static_cast<int64_t>(blockIdx.x) * 2 + (off == 0 ? 1 : 0)) * p.heads * R * (D + 2);
+        for (int job = warp; job < p.heads * rows; job += W) {
+          const int h = job & (p.heads - 1), row = job / p.heads;
           float mx = -INFINITY;
-#pragma unroll
-          for (int w = 0; w < kKvWarps; ++w) mx = fmaxf(mx, sm_m[w][row]);
+          for (int x = 0; x < n_sub; ++x) mx = fmaxf(mx, sm_m[x * p.heads + h][row]);
           float acc[D / 32], sum = 0.f;
 #pragma unroll
           for (int x = 0; x < D / 32; ++x) acc[x] = 0.f;
-#pragma unroll
-          for (int w = 0; w < kKvWarps; ++w) {
+          for (int y = 0; y < n_sub; ++y) {
+            const int w = y * p.heads + h;
             const float c = kv_ex2(sm_m[w][row] - (mx == -INFINITY ? 0.f : mx));
             sum += sm_l[w][row] * c;
 #pragma unroll
@@ -514,10 +539,10 @@ attention_kv4_kernel(Kv4Args p) {
             }
           }
           if (whole) {
-            const int tok = (i * R + row) / G, head = kvh * G + (i * R + row) % G;
+            const int tok = (i * R + row) / G, head = (group * p.heads + h) * G + (i * R + row) % G;
             kv4_write_row<D>(p, acc, sum, static_cast<int64_t>(r.begin) + tok, head, lane);
           } else {
-            float* dst = part + row * (D + 2);
+            float* dst = part + (h * R + row) * (D + 2);
             if (lane == 0) { dst[0] = mx; dst[1] = sum; }
 #pragma unroll
             for (int x = 0; x < D / 32; x += 2)
@@ -534,11 +559,12 @@ attention_kv4_kernel(Kv4Args p) {
 
 // Joins the partial results of work items that several workers share.  One CTA per (row block and KV head,
 // request), one warp per row; items that one worker covered are final already.
+constexpr int kMergeWarps = 4;
 template <int D, int NB>
-__global__ void __launch_bounds__(32 * kKvWarps)
+__global__ void __launch_bounds__(32 * kMergeWarps)
 kv4_merge_kernel(Kv4Args p) {
   constexpr int R = 8 * NB, PER = D / 32;
-  __shared__ int64_t scratch[kKvWarps];
+  __shared__ int64_t scratch[kMergeWarps];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int G = p.hq / p.hkv;
   const int b = blockIdx.y, i = blockIdx.x / p.hkv, kvh = blockIdx.x % p.hkv;
@@ -548,25 +574,27 @@ kv4_merge_kernel(Kv4Args p) {
     all += n;
     if (x < b) before += n;
   }
-  before = block_sum_i64(before, scratch);
-  all = block_sum_i64(all, scratch);
+  before = block_sum_i64<kMergeWarps>(before, scratch);
+  all = block_sum_i64<kMergeWarps>(all, scratch);
   const Kv4Req r = kv4_request(p, b);
   pdl_wait();                               // in every block: this grid ends only after the one before it
   if (i * R >= r.len * G) return;
   for (int x = 0; x < i; ++x) {
     const Kv4Span s = kv4_span<R>(p, r, G, x);
-    before += static_cast<int64_t>(s.last - s.first) * p.hkv;
+    before += static_cast<int64_t>(s.last - s.first) * (p.hkv / p.heads);
   }
   const Kv4Span span = kv4_span<R>(p, r, G, i);
   const int n_span = span.last - span.first;
-  const int64_t t0 = before + static_cast<int64_t>(kvh) * n_span, t1 = t0 + n_span;   // this item's tiles
+  const int64_t t0 = before + static_cast<int64_t>(kvh / p.heads) * n_span, t1 = t0 + n_span;   // this item's tiles
   // tile t belongs to the largest w with floor(all * w / workers) <= t
   const int64_t workers = min(static_cast<int64_t>(p.workers), all);
   const int64_t w0 = ((t0 + 1) * workers - 1) / all, w1 = (t1 * workers - 1) / all;
   if (w0 == w1) return;
   const int rows = min(R, r.len * G - i * R);
-  for (int row = warp; row < rows; row += kKvWarps) {
-    const auto at = [&](int64_t w) { return p.part + ((w * 2 + (w == w0 ? 1 : 0)) * R + row) * (D + 2); };
+  for (int row = warp; row < rows; row += kMergeWarps) {
+    const auto at = [&](int64_t w) {
+      return p.part + (((w * 2 + (w == w0 ? 1 : 0)) * p.heads + (kvh & (p.heads - 1))) * R + row) * (D + 2);
+    };
     float mx = -INFINITY;
     for (int64_t w = w0 + lane; w <= w1; w += 32) mx = fmaxf(mx, at(w)[0]);
 #pragma unroll
@@ -601,13 +629,31 @@ kv4_merge_kernel(Kv4Args p) {
   }
 }
 
+// KV heads a CTA of `warps` warps takes at once: the largest power of two that divides them.
+static int kv4_heads(int hkv, int warps) {
+  int h = 1;
+  while (h < warps && hkv % (2 * h) == 0) h *= 2;
+  return h;
+}
+
 template <int D, int NB>
-static int launch_kv4(const Kv4Args& a, cudaStream_t st) {
-  constexpr int R = 8 * NB;
-  constexpr int smem = kKvWarps * Kv4Ring<D>::kWarp;
+static int64_t kv4_few_workspace(int hkv) {
+  using Shape = Kv4Shape<D, NB>;
+  return static_cast<int64_t>(sm_count()) * Shape::kCtas * 2 * kv4_heads(hkv, Shape::kWarps) * 8 * NB * (D + 2) * 4;
+}
+
+template <int D, int NB>
+static int launch_kv4(Kv4Args a, cudaStream_t st) {
+  using Shape = Kv4Shape<D, NB>;
+  constexpr int R = 8 * NB, W = Shape::kWarps;
+  constexpr int smem = W * Kv4Ring<D>::kWarp;
   static SmemConfig config;
-  if (int rc = config.ensure(attention_kv4_kernel<D, NB>, smem)) return rc;
-  attention_kv4_kernel<D, NB><<<a.workers, 32 * kKvWarps, smem, st>>>(a);
+  if (int rc = config.ensure(attention_kv4_kernel<D, NB, W>, smem)) return rc;
+  a.workers = sm_count() * Shape::kCtas;
+  a.heads = kv4_heads(a.hkv, W);
+  a.tile_shift = 5;
+  while ((1 << a.tile_shift) < 32 * (W / a.heads)) ++a.tile_shift;
+  attention_kv4_kernel<D, NB, W><<<a.workers, 32 * W, smem, st>>>(a);
   if (cudaGetLastError() != cudaSuccess) return MSL_ERR_CUDA;
   const int G = a.hq / a.hkv;
   const int64_t blocks = (static_cast<int64_t>(a.max_q_len) * G + R - 1) / R;
@@ -617,7 +663,7 @@ static int launch_kv4(const Kv4Args& a, cudaStream_t st) {
   attr.val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(blocks * a.hkv), a.batch);
-  cfg.blockDim = dim3(32 * kKvWarps);
+  cfg.blockDim = dim3(32 * kMergeWarps);
   cfg.stream = st;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
@@ -642,8 +688,9 @@ static Kv4Plan kv4_plan(int batch, int max_q_len, int tokens, int hq, int hkv, i
   const int64_t rows = static_cast<int64_t>(max_q_len) * (hq / hkv);
   plan.few = rows <= kKvFewRows;
   if (plan.few) {
-    const int64_t workers = static_cast<int64_t>(sm_count()) * kKvCtasPerSm;
-    plan.bytes = workers * 2 * 8 * kv4_row_blocks(rows) * (head_dim + 2) * 4;
+    const bool one = kv4_row_blocks(rows) == 1;
+    plan.bytes = head_dim == 128 ? (one ? kv4_few_workspace<128, 1>(hkv) : kv4_few_workspace<128, 2>(hkv))
+                                 : (one ? kv4_few_workspace<64, 1>(hkv) : kv4_few_workspace<64, 2>(hkv));
   } else {
     plan.splits = msl_attention_split_plan(batch, max_q_len, hq, hkv, max_pages, page_size, window);
     plan.bytes = kv4_tc_workspace(plan.splits, tokens, hq, head_dim);
@@ -699,7 +746,7 @@ extern "C" int msl_attention_kv4(const void* q, int64_t ld_q, const void* k_cach
                   page_table, max_pages, seq_lens, cu_seqlens_q, k_scale, v_scale, softmax_scale, batch, max_q_len,
                   tokens, hq, hkv, page_size, window, cache_rows, static_cast<__nv_bfloat16*>(out), ld_out,
                   static_cast<const __nv_bfloat16*>(gate), ld_gate, static_cast<float*>(workspace),
-                  sm_count() * kKvCtasPerSm, plan.splits, page_shift, status};
+                  0, 0, 0, plan.splits, page_shift, status};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (!plan.few) return launch_kv4_tc(a, head_dim, st);
   if (kv4_row_blocks(static_cast<int64_t>(max_q_len) * G) == 1)

@@ -26,7 +26,9 @@ struct Kv4Args {
   const __nv_bfloat16* gate;
   int64_t ld_gate;
   float* part;                  // partial results (workspace)
-  int workers;                  // few rows: CTAs that share the key tiles
+  int workers;                  // few rows: CTAs that share the key tiles,
+  int heads;                    //   KV heads a CTA takes at once,
+  int tile_shift;               //   log2 of a tile's keys
   int kv_splits;                // many rows: slices of a query block's keys
   int page_shift;               // log2 of the page size, -1: not a power of two
   int* status;
