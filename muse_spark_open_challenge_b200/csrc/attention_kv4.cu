@@ -44,7 +44,7 @@ struct Kv4Span {
   int first, last;
 };
 template <int R>
-__device__ __forceinline__ Kv4Span kv4_span(const Kv4Args& p, const Kv4Req& r, int G, int i) {
+__device__ __forceinline__ Kv4Span kv4_span(const Kv4Args& p, const Kv4Req& r, int G, int i, int tile_shift) {
   const int last_tok = min(r.len - 1, (R * i + R - 1) / G);
   const int low_tok = R * i / G;
   // keys past the table's row have no page: they are not walked (the kernel reports them)
@@ -52,20 +52,27 @@ __device__ __forceinline__ Kv4Span kv4_span(const Kv4Args& p, const Kv4Req& r, i
                                       static_cast<int64_t>(p.max_pages) * p.page_size));
   const int lo = p.window ? max(0, r.seq + low_tok - p.window + 1) : 0;
   Kv4Span s;
-  s.first = lo >> p.tile_shift;
-  s.last = max(s.first + 1, (hi + (1 << p.tile_shift) - 1) >> p.tile_shift);   // with nothing to see: zeros are written
+  s.first = lo >> tile_shift;
+  s.last = max(s.first + 1, (hi + (1 << tile_shift) - 1) >> tile_shift);   // with nothing to see: zeros are written
   return s;
 }
+// Tiles of a request (all row blocks and KV heads) when a CTA takes `heads` KV heads at once, 2^tile_shift keys a tile.
 template <int R>
-__device__ __forceinline__ int64_t kv4_tiles(const Kv4Args& p, const Kv4Req& r, int G) {
+__device__ __forceinline__ int64_t kv4_tiles(const Kv4Args& p, const Kv4Req& r, int G, int heads, int tile_shift) {
   const int blocks = (r.len * G + R - 1) / R;
   int64_t sum = 0;
   for (int i = 0; i < blocks; ++i) {
-    const Kv4Span s = kv4_span<R>(p, r, G, i);
+    const Kv4Span s = kv4_span<R>(p, r, G, i, tile_shift);
     sum += s.last - s.first;
   }
-  return sum * (p.hkv / p.heads);
+  return sum * (p.hkv / heads);
 }
+// A CTA takes p.heads KV heads of 32 W / p.heads keys at once where every worker has at least kKvLong tiles (below), and
+// one head of 32 W keys otherwise: the heads of a cache row lie side by side, so taking them together fetches whole rows
+// (a 64-byte piece of one costs as much DRAM time as 128 bytes), but it also leaves p.heads times as many partial
+// results per item to join, which a short step cannot hide.  64 requests x 8192 keys, 8 heads: 291 -> 174 us with all
+// heads at once; 1 x 4096: 18 -> 40 us.
+constexpr int kKvLong = 8;
 
 template <int W>
 __device__ __forceinline__ int64_t block_sum_i64(int64_t v, int64_t* scratch) {
@@ -216,8 +223,16 @@ attention_kv4_kernel(Kv4Args p) {
   // ---- this worker's range of tiles
   const int per = (p.batch + blockDim.x - 1) / blockDim.x;
   const int b0 = min(tid * per, p.batch), b1 = min(b0 + per, p.batch);
-  int64_t mine = 0;
-  for (int b = b0; b < b1; ++b) mine += kv4_tiles<R>(p, kv4_request(p, b), G);
+  constexpr int kWide = W == 8 ? 8 : 7;                     // log2 of a one-head tile's keys, 32 W
+  int64_t mine_all = 0, mine = 0;                           // tiles with p.heads heads a CTA, and with one
+  for (int b = b0; b < b1; ++b) {
+    const Kv4Req r = kv4_request(p, b);
+    mine_all += kv4_tiles<R>(p, r, G, p.heads, p.tile_shift);
+    mine += kv4_tiles<R>(p, r, G, 1, kWide);
+  }
+  const bool together = block_sum_i64<W>(mine_all, scratch) >= static_cast<int64_t>(kKvLong) * p.workers;
+  const int heads = together ? p.heads : 1, tile_shift = together ? p.tile_shift : kWide;
+  if (together) mine = mine_all;
   int64_t inc = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -239,7 +254,7 @@ attention_kv4_kernel(Kv4Args p) {
     int64_t base = inc - mine;
     int b = b0;
     for (; b < b1 - 1; ++b) {
-      const int64_t n = kv4_tiles<R>(p, kv4_request(p, b), G);
+      const int64_t n = kv4_tiles<R>(p, kv4_request(p, b), G, heads, tile_shift);
       if (at < base + n) break;
       base += n;
     }
@@ -251,18 +266,18 @@ attention_kv4_kernel(Kv4Args p) {
   int64_t skip = at - sm_at;                                // tiles of request b before this range
   const float scale_log2 = p.softmax_scale * (*p.k_scale) * 1.4426950408889634f;
 
-  const int groups = p.hkv / p.heads, my_head = warp & (p.heads - 1), n_sub = W / p.heads;
+  const int groups = p.hkv / heads, my_head = warp & (heads - 1), n_sub = W / heads;
 
   for (; at < end && b < p.batch; ++b) {
     const Kv4Req r = kv4_request(p, b);
     const int blocks = (r.len * G + R - 1) / R;
     const int* table = p.page_table + static_cast<int64_t>(b) * p.max_pages;
     for (int i = 0; i < blocks && at < end; ++i) {
-      const Kv4Span span = kv4_span<R>(p, r, G, i);
+      const Kv4Span span = kv4_span<R>(p, r, G, i, tile_shift);
       const int n_span = span.last - span.first;
       if (skip >= static_cast<int64_t>(n_span) * groups) { skip -= static_cast<int64_t>(n_span) * groups; continue; }
       for (int group = static_cast<int>(skip / n_span); group < groups && at < end; ++group) {
-        const int kvh = group * p.heads + my_head;
+        const int kvh = group * heads + my_head;
         const int off = static_cast<int>(skip % n_span);
         skip = 0;
         const int n = static_cast<int>(min(end - at, static_cast<int64_t>(n_span - off)));
@@ -322,8 +337,8 @@ attention_kv4_kernel(Kv4Args p) {
             for (int c = 0; c < 4; ++c) o[nb][k][c] = 0.f;
         }
         // ---- the keys, 32 a step
-        const int tile = 1 << p.tile_shift;
-        const int key_first = (span.first + off) * tile + (warp / p.heads) * 32;
+        const int tile = 1 << tile_shift;
+        const int key_first = (span.first + off) * tile + (warp / heads) * 32;
         const auto page_of = [&](int j) {
           return j < n ? kv4_page(p, table, key_first + j * tile + lane, lo, hi) : Kv4Page{INT_MIN, 0};
         };
@@ -521,15 +536,15 @@ attention_kv4_kernel(Kv4Args p) {
         // a worker has at most two partial results: the rest of an item that an earlier worker began (slot 0) and
         // the beginning of one that a later worker ends (slot 1)
         float* part = p.part + (static_cast<int64_t>(blockIdx.x) * 2 + (off == 0 ? 1 : 0)) * p.heads * R * (D + 2);
-        for (int job = warp; job < p.heads * rows; job += W) {
-          const int h = job & (p.heads - 1), row = job / p.heads;
+        for (int job = warp; job < heads * rows; job += W) {
+          const int h = job & (heads - 1), row = job / heads;
           float mx = -INFINITY;
-          for (int x = 0; x < n_sub; ++x) mx = fmaxf(mx, sm_m[x * p.heads + h][row]);
+          for (int x = 0; x < n_sub; ++x) mx = fmaxf(mx, sm_m[x * heads + h][row]);
           float acc[D / 32], sum = 0.f;
 #pragma unroll
           for (int x = 0; x < D / 32; ++x) acc[x] = 0.f;
           for (int y = 0; y < n_sub; ++y) {
-            const int w = y * p.heads + h;
+            const int w = y * heads + h;
             const float c = kv_ex2(sm_m[w][row] - (mx == -INFINITY ? 0.f : mx));
             sum += sm_l[w][row] * c;
 #pragma unroll
@@ -539,7 +554,7 @@ attention_kv4_kernel(Kv4Args p) {
             }
           }
           if (whole) {
-            const int tok = (i * R + row) / G, head = (group * p.heads + h) * G + (i * R + row) % G;
+            const int tok = (i * R + row) / G, head = (group * heads + h) * G + (i * R + row) % G;
             kv4_write_row<D>(p, acc, sum, static_cast<int64_t>(r.begin) + tok, head, lane);
           } else {
             float* dst = part + (h * R + row) * (D + 2);
@@ -557,75 +572,98 @@ attention_kv4_kernel(Kv4Args p) {
   }
 }
 
-// Joins the partial results of work items that several workers share.  One CTA per (row block and KV head,
-// request), one warp per row; items that one worker covered are final already.
-constexpr int kMergeWarps = 4;
-template <int D, int NB>
+// Joins the partial results of work items that several workers share; items that one worker covered are final already.
+// One CTA per (row block and KV head, request, and, where there are few of them, row).  Its warps share out the rows
+// and, with warps to spare, the partial results of a row.
+constexpr int kMergeWarps = 8;
+template <int D, int NB, int W>
 __global__ void __launch_bounds__(32 * kMergeWarps)
 kv4_merge_kernel(Kv4Args p) {
   constexpr int R = 8 * NB, PER = D / 32;
   __shared__ int64_t scratch[kMergeWarps];
+  __shared__ float sm_o[kMergeWarps][D], sm_l[kMergeWarps];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int G = p.hq / p.hkv;
   const int b = blockIdx.y, i = blockIdx.x / p.hkv, kvh = blockIdx.x % p.hkv;
-  int64_t before = 0, all = 0;
+  constexpr int kWide = W == 8 ? 8 : 7;
+  int64_t before = 0, all = 0, before_all = 0, all_all = 0;
   for (int x = tid; x < p.batch; x += blockDim.x) {
-    const int64_t n = kv4_tiles<R>(p, kv4_request(p, x), G);
+    const Kv4Req r = kv4_request(p, x);
+    const int64_t n = kv4_tiles<R>(p, r, G, 1, kWide), m = kv4_tiles<R>(p, r, G, p.heads, p.tile_shift);
     all += n;
-    if (x < b) before += n;
+    all_all += m;
+    if (x < b) { before += n; before_all += m; }
   }
-  before = block_sum_i64<kMergeWarps>(before, scratch);
-  all = block_sum_i64<kMergeWarps>(all, scratch);
+  all_all = block_sum_i64<kMergeWarps>(all_all, scratch);
+  const bool together = all_all >= static_cast<int64_t>(kKvLong) * p.workers;   // the attention kernel's choice
+  const int heads = together ? p.heads : 1, tile_shift = together ? p.tile_shift : kWide;
+  all = together ? all_all : block_sum_i64<kMergeWarps>(all, scratch);
+  before = block_sum_i64<kMergeWarps>(together ? before_all : before, scratch);
   const Kv4Req r = kv4_request(p, b);
   pdl_wait();                               // in every block: this grid ends only after the one before it
   if (i * R >= r.len * G) return;
   for (int x = 0; x < i; ++x) {
-    const Kv4Span s = kv4_span<R>(p, r, G, x);
-    before += static_cast<int64_t>(s.last - s.first) * (p.hkv / p.heads);
+    const Kv4Span s = kv4_span<R>(p, r, G, x, tile_shift);
+    before += static_cast<int64_t>(s.last - s.first) * (p.hkv / heads);
   }
-  const Kv4Span span = kv4_span<R>(p, r, G, i);
+  const Kv4Span span = kv4_span<R>(p, r, G, i, tile_shift);
   const int n_span = span.last - span.first;
-  const int64_t t0 = before + static_cast<int64_t>(kvh / p.heads) * n_span, t1 = t0 + n_span;   // this item's tiles
+  const int64_t t0 = before + static_cast<int64_t>(kvh / heads) * n_span, t1 = t0 + n_span;   // this item's tiles
   // tile t belongs to the largest w with floor(all * w / workers) <= t
   const int64_t workers = min(static_cast<int64_t>(p.workers), all);
-  const int64_t w0 = ((t0 + 1) * workers - 1) / all, w1 = (t1 * workers - 1) / all;
+  const int w0 = static_cast<int>(((t0 + 1) * workers - 1) / all), w1 = static_cast<int>((t1 * workers - 1) / all);
   if (w0 == w1) return;
   const int rows = min(R, r.len * G - i * R);
-  for (int row = warp; row < rows; row += kMergeWarps) {
-    const auto at = [&](int64_t w) {
-      return p.part + (((w * 2 + (w == w0 ? 1 : 0)) * p.heads + (kvh & (p.heads - 1))) * R + row) * (D + 2);
+  // rows_par rows at a time, `share` warps a row
+  const int here = gridDim.z == 1 ? rows : 1;
+  const int rows_par = here > 4 ? 8 : here > 2 ? 4 : here, share = kMergeWarps / rows_par;
+  const int mine = warp % share;
+  for (int row0 = blockIdx.z; row0 < rows; row0 += gridDim.z * rows_par) {
+    const int row = row0 + warp / share;
+    const bool live = row < rows;
+    const auto at = [&](int w) {
+      return p.part + ((static_cast<int64_t>(w * 2 + (w == w0 ? 1 : 0)) * p.heads + (kvh & (heads - 1))) * R + row) * (D + 2);
     };
-    float mx = -INFINITY;
-    for (int64_t w = w0 + lane; w <= w1; w += 32) mx = fmaxf(mx, at(w)[0]);
-#pragma unroll
-    for (int d = 16; d > 0; d >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
-    const float ref = mx == -INFINITY ? 0.f : mx;
-    float acc[PER], sum = 0.f;
+    float sum = 0.f, acc[PER];
 #pragma unroll
     for (int x = 0; x < PER; ++x) acc[x] = 0.f;
-    for (int64_t w32 = w0; w32 <= w1; w32 += 32) {          // a lane forms the weight of one worker
-      float c = 0.f;
-      if (w32 + lane <= w1) {
-        const float* src = at(w32 + lane);
-        c = kv_ex2(src[0] - ref);
-        sum += src[1] * c;
-      }
-      const int n = static_cast<int>(min(w1 - w32 + 1, static_cast<int64_t>(32)));
+    if (live) {
+      float mx = -INFINITY;
+      for (int w = w0 + lane; w <= w1; w += 32) mx = fmaxf(mx, at(w)[0]);
+#pragma unroll
+      for (int d = 16; d > 0; d >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
+      const float ref = mx == -INFINITY ? 0.f : mx;
 #pragma unroll 8
-      for (int w = 0; w < n; ++w) {
-        const float cw = __shfl_sync(0xffffffffu, c, w);
-        const float* src = at(w32 + w) + 2 + lane * PER;
+      for (int w = w0 + mine; w <= w1; w += share) {
+        const float* src = at(w);
+        const float c = kv_ex2(src[0] - ref);
+        sum += src[1] * c;
 #pragma unroll
         for (int x = 0; x < PER; x += 2) {
-          const float2 v = *reinterpret_cast<const float2*>(src + x);
-          acc[x] += v.x * cw;
-          acc[x + 1] += v.y * cw;
+          const float2 v = *reinterpret_cast<const float2*>(src + 2 + lane * PER + x);
+          acc[x] += v.x * c;
+          acc[x + 1] += v.y * c;
         }
       }
     }
-    sum = warp_sum(sum);
-    const int tok = (i * R + row) / G, head = kvh * G + (i * R + row) % G;
-    kv4_write_row<D>(p, acc, sum, static_cast<int64_t>(r.begin) + tok, head, lane);
+    if (share > 1) {                                        // uniform
+#pragma unroll
+      for (int x = 0; x < PER; ++x) sm_o[warp][lane * PER + x] = acc[x];
+      if (lane == 0) sm_l[warp] = sum;
+      __syncthreads();
+      if (mine == 0) {
+        for (int y = 1; y < share; ++y) {                   // all relative to the same maximum
+          sum += sm_l[warp + y];
+#pragma unroll
+          for (int x = 0; x < PER; ++x) acc[x] += sm_o[warp + y][lane * PER + x];
+        }
+      }
+      __syncthreads();
+    }
+    if (live && mine == 0) {
+      const int tok = (i * R + row) / G, head = kvh * G + (i * R + row) % G;
+      kv4_write_row<D>(p, acc, sum, static_cast<int64_t>(r.begin) + tok, head, lane);
+    }
   }
 }
 
@@ -662,12 +700,14 @@ static int launch_kv4(Kv4Args a, cudaStream_t st) {
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr.val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(blocks * a.hkv), a.batch);
+  // few items: a CTA a row, whose warps share its many partial results
+  const int64_t items = blocks * a.hkv * a.batch;
+  cfg.gridDim = dim3(static_cast<unsigned>(blocks * a.hkv), a.batch, items <= sm_count() / 2 ? R : 1);
   cfg.blockDim = dim3(32 * kMergeWarps);
   cfg.stream = st;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kv4_merge_kernel<D, NB>, a) == cudaSuccess ? MSL_OK : MSL_ERR_CUDA;
+  return cudaLaunchKernelEx(&cfg, kv4_merge_kernel<D, NB, W>, a) == cudaSuccess ? MSL_OK : MSL_ERR_CUDA;
 }
 
 // Query rows a CTA holds: one MMA column block of 8 where the group's rows fit, else two.
