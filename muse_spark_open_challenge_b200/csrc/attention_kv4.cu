@@ -132,14 +132,14 @@ __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_gr
 // Where a lane's copies start: the KV head's bytes of cache row 0, and the lane's 16-byte unit of them.
 struct Kv4Source {
   const uint8_t *k, *v, *ks, *vs;
-  int64_t pitch, sf_pitch;                  // bytes of a cache row (all heads)
+  int pitch, sf_pitch;                      // bytes of a cache row (all heads)
 };
 template <int D>
 __device__ __forceinline__ Kv4Source kv4_source(const Kv4Args& p, int kvh, int lane) {
   using S = Kv4Ring<D>;
   const int at = kvh * S::kRowBytes + (lane % S::kChunks) * 16;
   return {p.k + at, p.v + at, p.ks + kvh * S::kSfBytes, p.vs + kvh * S::kSfBytes,
-          static_cast<int64_t>(p.hkv) * S::kRowBytes, static_cast<int64_t>(p.hkv) * S::kSfBytes};
+          p.hkv * S::kRowBytes, p.hkv * S::kSfBytes};
 }
 
 // Start copying the 32 keys whose cache rows the lanes hold (-1: zeros).
@@ -148,19 +148,34 @@ __device__ __forceinline__ void kv4_issue(const Kv4Source& src, uint8_t* stage, 
   using S = Kv4Ring<D>;
   const uint32_t base = smem_u32(stage);
   const uint32_t mask = __ballot_sync(0xffffffffu, row >= 0);
-  const int safe = max(row, 0);
+  constexpr int kRows = 32 / S::kChunks;                    // rows a round covers
+  const int c = lane % S::kChunks;
+  if (mask == 0xffffffffu) {
 #pragma unroll
-  for (int i = 0; i < S::kChunks; ++i) {
-    constexpr int kRows = 32 / S::kChunks;                  // rows a round covers
-    const int r = kRows * i + lane / S::kChunks, c = lane % S::kChunks;
-    const int from = __shfl_sync(0xffffffffu, safe, r);
-    const int bytes = (mask >> r) & 1u ? 16 : 0;
-    cp_async16(base + r * S::kRowBytes + c * 16, src.k + from * src.pitch, bytes);
-    cp_async16(base + S::kV + kv4_v_offset<D>(r, c * 16), src.v + from * src.pitch, bytes);
+    for (int i = 0; i < S::kChunks; ++i) {
+      const int r = kRows * i + lane / S::kChunks;
+      const int64_t from = __shfl_sync(0xffffffffu, row, r);
+      cp_async16(base + r * S::kRowBytes + c * 16, src.k + from * src.pitch, 16);
+      cp_async16(base + S::kV + kv4_v_offset<D>(r, c * 16), src.v + from * src.pitch, 16);
+    }
+    const int64_t from = row;
+    cp_async_small<S::kSfBytes>(base + S::kKs + lane * S::kSfBytes, src.ks + from * src.sf_pitch, S::kSfBytes);
+    cp_async_small<S::kSfBytes>(base + S::kVs + lane * S::kSfBytes, src.vs + from * src.sf_pitch, S::kSfBytes);
+  } else {
+#pragma unroll
+    for (int i = 0; i < S::kChunks; ++i) {
+      const int r = kRows * i + lane / S::kChunks;
+      const int got = __shfl_sync(0xffffffffu, row, r);
+      const int64_t from = max(got, 0);
+      const int bytes = got >= 0 ? 16 : 0;
+      cp_async16(base + r * S::kRowBytes + c * 16, src.k + from * src.pitch, bytes);
+      cp_async16(base + S::kV + kv4_v_offset<D>(r, c * 16), src.v + from * src.pitch, bytes);
+    }
+    const int64_t from = max(row, 0);
+    const int bytes = row >= 0 ? S::kSfBytes : 0;
+    cp_async_small<S::kSfBytes>(base + S::kKs + lane * S::kSfBytes, src.ks + from * src.sf_pitch, bytes);
+    cp_async_small<S::kSfBytes>(base + S::kVs + lane * S::kSfBytes, src.vs + from * src.sf_pitch, bytes);
   }
-  const int bytes = row >= 0 ? S::kSfBytes : 0;
-  cp_async_small<S::kSfBytes>(base + S::kKs + lane * S::kSfBytes, src.ks + safe * src.sf_pitch, bytes);
-  cp_async_small<S::kSfBytes>(base + S::kVs + lane * S::kSfBytes, src.vs + safe * src.sf_pitch, bytes);
   if (lane == 0) *reinterpret_cast<uint32_t*>(stage + S::kHeld) = mask;
 }
 
@@ -406,13 +421,7 @@ attention_kv4_kernel(Kv4Args p) {
               }
             }
           }
-          // ---- scores in log2 units, masked where some row does not see a key
-#pragma unroll
-          for (int h = 0; h < 2; ++h)
-#pragma unroll
-            for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-              for (int c = 0; c < 4; ++c) s[h][nb][c] *= qs[nb][c & 1];
+          // ---- mask where some row does not see a key
           if (partial) {
 #pragma unroll
             for (int h = 0; h < 2; ++h)
@@ -436,7 +445,8 @@ attention_kv4_kernel(Kv4Args p) {
           for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
-              float x = fmaxf(fmaxf(s[0][nb][c], s[0][nb][2 + c]), fmaxf(s[1][nb][c], s[1][nb][2 + c]));
+              // in log2 units (the scale is positive)
+              const float x = fmaxf(fmaxf(s[0][nb][c], s[0][nb][2 + c]), fmaxf(s[1][nb][c], s[1][nb][2 + c])) * qs[nb][c];
               top[nb][c] = x;
               move |= x > m[nb][c] + kKvTau || (m[nb][c] == -INFINITY && x > -INFINITY);
             }
@@ -465,7 +475,8 @@ attention_kv4_kernel(Kv4Args p) {
             for (int h = 0; h < 2; ++h)
 #pragma unroll
               for (int x = 0; x < 2; ++x) {
-                const float e0 = kv_ex2(s[h][nb][2 * x] - n0), e1 = kv_ex2(s[h][nb][2 * x + 1] - n1);
+                const float e0 = kv_ex2(fmaf(s[h][nb][2 * x], qs[nb][0], -n0));
+                const float e1 = kv_ex2(fmaf(s[h][nb][2 * x + 1], qs[nb][1], -n1));
                 l[nb][0] += e0;
                 l[nb][1] += e1;
                 pf[h][nb][x] = transpose8x8(h2_bits(__floats2half2_rn(e0, e1)));
@@ -760,7 +771,7 @@ extern "C" int msl_attention_kv4(const void* q, int64_t ld_q, const void* k_cach
                                  void* out, int64_t ld_out, const void* gate, int64_t ld_gate, void* workspace,
                                  int64_t workspace_bytes, int* status, void* stream) {
   if (batch <= 0 || max_q_len <= 0 || tokens < 0 || hq <= 0 || hkv <= 0 || hq % hkv || page_size <= 0 || window < 0 ||
-      max_pages <= 0 || cache_rows <= 0 || cache_rows > 0x7fffffff)
+      max_pages <= 0 || cache_rows <= 0 || cache_rows > 0x7fffffff || !(softmax_scale > 0.f))
     return MSL_ERR_ARG;
   if (head_dim != 64 && head_dim != 128) return MSL_ERR_UNSUPPORTED;
   const int G = hq / hkv;

@@ -81,14 +81,14 @@ def test_rows_refuses(lib):
 
 def attention_call(lib, **kw):
     a = dict(q=FAKE, ld_q=512, k=FAKE, kf=FAKE, v=FAKE, vf=FAKE, table=FAKE, max_pages=4, seq=FAKE, cu=FAKE, ks=FAKE,
-             vs=FAKE, batch=2, longest=3, tokens=6, hq=8, hkv=2, dim=64, page=16, window=0, rows=64, out=FAKE, ld_out=512,
+             vs=FAKE, scale=0.125, batch=2, longest=3, tokens=6, hq=8, hkv=2, dim=64, page=16, window=0, rows=64, out=FAKE, ld_out=512,
              gate=NULL, ld_gate=0, work=FAKE, bytes=None)
     a.update(kw)
     if a["bytes"] is None:
         a["bytes"] = lib.msl_attention_kv4_workspace(a["batch"], a["longest"], a["tokens"], a["hq"], a["hkv"], a["dim"],
                                                      a["max_pages"], a["page"], a["window"])
     return lib.msl_attention_kv4(a["q"], a["ld_q"], a["k"], a["kf"], a["v"], a["vf"], a["table"], a["max_pages"], a["seq"],
-                                 a["cu"], a["ks"], a["vs"], 0.125, a["batch"], a["longest"], a["tokens"], a["hq"],
+                                 a["cu"], a["ks"], a["vs"], a["scale"], a["batch"], a["longest"], a["tokens"], a["hq"],
                                  a["hkv"], a["dim"], a["page"], a["window"], a["rows"], a["out"], a["ld_out"], a["gate"],
                                  a["ld_gate"], a["work"], a["bytes"], NULL, NULL)
 
@@ -97,7 +97,8 @@ def test_attention_refuses(lib):
     for name in ("q", "k", "kf", "v", "vf", "table", "seq", "cu", "ks", "vs", "out", "work"):
         assert attention_call(lib, **{name: NULL}) == -1, name
     for name, bad in (("batch", 0), ("longest", 0), ("tokens", -1), ("hq", 7), ("hkv", 0), ("page", 0), ("window", -1),
-                      ("rows", 0), ("rows", 1 << 31), ("max_pages", 0), ("ld_q", 504), ("ld_out", 504)):
+                      ("rows", 0), ("rows", 1 << 31), ("max_pages", 0), ("ld_q", 504), ("ld_out", 504), ("scale", 0.0), ("scale", -1.0),
+                      ("scale", float("nan"))):
         assert attention_call(lib, bytes=1 << 30, **{name: bad}) == -1, name
     assert attention_call(lib, gate=FAKE, ld_gate=504) == -1
     assert attention_call(lib, dim=96, bytes=1 << 30, ld_q=768, ld_out=768) == -7
