@@ -34,8 +34,8 @@ struct TcSmem {
   static constexpr int kRing = 2 * kTile;
   static constexpr int kHeld = kRing + kStages * kTile;    // 8 x 4 words: the keys of a tile that have a page
   static constexpr int kBar = kHeld + 8 * 16;
-  // q_full, full[stages], empty[stages], s_full[2], p_lo[2], p_hi[2], pv_done[2], turn[8]
-  static constexpr int kNumBars = 1 + 2 * kStages + 16;
+  // q_full, full[stages], empty[stages], s_full[2], p_lo[2], p_hi[2], pv_done[2]
+  static constexpr int kNumBars = 1 + 2 * kStages + 8;
   static constexpr int kTotal = kBar + kNumBars * 8 + 16;
 };
 
@@ -75,22 +75,36 @@ __device__ __forceinline__ void tc_mask(uint32_t (&s)[32], int col0, int lim_hi,
     if (!(col <= lim_hi && col > lim_lo && ((held >> i) & 1u))) s[i] = 0xff800000u;
   }
 }
-// 64 columns of a row of S: exponentials summed into l and packed as f16 pairs in key order.
-__device__ __forceinline__ void tc_softmax_half(const uint32_t (&s0)[32], const uint32_t (&s1)[32], float scale_log2,
-                                                float neg_m, float& l, uint32_t (&packed)[32]) {
+// Two fp32 values an instruction: the FMA pipe takes half the issue slots.
+__device__ __forceinline__ uint64_t f32x2(float a, float b) {
+  uint64_t d;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(a), "f"(b));
+  return d;
+}
+__device__ __forceinline__ float2 unpack_f32x2(uint64_t v) {
+  float2 d;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(d.x), "=f"(d.y) : "l"(v));
+  return d;
+}
+__device__ __forceinline__ uint64_t fma_f32x2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t add_f32x2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+// 32 columns of a row of S: exponentials summed (four chains) and packed as f16 pairs in key order.
+__device__ __forceinline__ void tc_exp32(const uint32_t (&s)[32], uint64_t scale, uint64_t neg_m, uint64_t (&sum)[2],
+                                         uint32_t* packed) {
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const uint32_t(&s)[32] = h ? s1 : s0;
-    float part[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int i = 0; i < 32; i += 2) {
-      const float a = kv_ex2(fmaf(__uint_as_float(s[i]), scale_log2, neg_m));
-      const float b = kv_ex2(fmaf(__uint_as_float(s[i + 1]), scale_log2, neg_m));
-      part[(i / 2) & 3] += a;
-      part[(i / 2 + 2) & 3] += b;
-      packed[16 * h + i / 2] = h2_bits(__floats2half2_rn(a, b));
-    }
-    l += (part[0] + part[1]) + (part[2] + part[3]);
+  for (int i = 0; i < 32; i += 2) {
+    const float2 x = unpack_f32x2(fma_f32x2(f32x2(__uint_as_float(s[i]), __uint_as_float(s[i + 1])), scale, neg_m));
+    const float a = kv_ex2(x.x), b = kv_ex2(x.y);
+    sum[(i / 2) & 1] = add_f32x2(sum[(i / 2) & 1], f32x2(a, b));
+    packed[i / 2] = h2_bits(__floats2half2_rn(a, b));
   }
 }
 
@@ -161,7 +175,6 @@ attention_kv4_tc_kernel(Kv4Args p) {
   uint64_t* p_lo = s_full + 2;
   uint64_t* p_hi = p_lo + 2;
   uint64_t* pv_done = p_hi + 2;
-  uint64_t* turn = pv_done + 2;                            // [group][warp in group]: the exponential unit's turn
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + S::kNumBars);
   volatile uint32_t* abort_flag = tmem_slot + 1;
   uint32_t* held = reinterpret_cast<uint32_t*>(smem + S::kHeld);
@@ -229,7 +242,6 @@ attention_kv4_tc_kernel(Kv4Args p) {
       mbar_init(&p_hi[i], 4);
       mbar_init(&pv_done[i], 1);
     }
-    for (int i = 0; i < 8; ++i) mbar_init(&turn[i], 1);
     *abort_flag = 0;
     mbar_fence_init();
   }
@@ -345,7 +357,7 @@ attention_kv4_tc_kernel(Kv4Args p) {
     reg_alloc<176>();
     const int sub = warp >> 2;                             // query sub-tile of this group
     const int r = (warp & 3) * 32 + lane;                  // row = TMEM lane
-    const int n_mine = n_sub[sub], n_other = n_sub[sub ^ 1];
+    const int n_mine = n_sub[sub];
     const int tq = r / G, g = r - tq * G;
     const bool row_valid = r < rows_valid[sub];
     const int first_tok = q0 + sub * TQ;
@@ -414,55 +426,49 @@ attention_kv4_tc_kernel(Kv4Args p) {
       // A row's reference maximum moves when the row exceeds it by more than tau, or finds its first visible key.  Each
       // row decides for itself, so that its bits do not depend on its neighbours; the warp rescales together.
       const bool move = m_cand > m_run + kTcTau || (m_run == -INFINITY && m_cand > -INFINITY);
-      const bool event = __any_sync(0xffffffffu, move);
       float corr = 1.0f;
-      if (move) {
-        corr = kv_ex2(m_run - m_cand);                      // 0 when m_run = -inf
-        m_run = m_cand;
+      if (__any_sync(0xffffffffu, move)) {
+        if (move) {
+          corr = kv_ex2(m_run - m_cand);                    // 0 when m_run = -inf
+          m_run = m_cand;
+        }
+        if (j > 0) {
+          // O moves to the new maximum before any of this tile's P is used.  S(j) was ready only after P V(j-1) had
+          // finished (the tensor pipe ran it first), so O is quiet.  Small pieces: the scores hold the registers.
+#pragma unroll 1
+          for (int c = 0; c < D; c += 16) {
+            uint32_t oa[16];
+            tmem_ld16(tmem_o + c, oa);
+            tmem_ld_wait();
+#pragma unroll
+            for (int i = 0; i < 16; ++i) oa[i] = __float_as_uint(__uint_as_float(oa[i]) * corr);
+            tmem_st16(tmem_o + c, oa);
+          }
+        }
       }
       const float m_use = (m_run == -INFINITY) ? 0.f : m_run;
-      const bool resc = j > 0 && event;                     // warp-uniform
-      // The two warps that share a scheduler (one of each group) take turns at the exponential pass.  Order: group 0
-      // tile 0, group 1 tile 0, group 0 tile 1, ...; a turn is skipped where the partner has no such tile.
-      if (sub == 0 ? (j >= 1 && j - 1 < n_other) : (j < n_other)) {
-        if (*abort_flag || !mbar_wait(&turn[sub * 4 + (warp & 3)], (sub == 0 ? j - 1 : j) & 1)) { ok = false; break; }
-      }
-      const float neg_m = kTcShift - m_use;
-      float l_tile = 0.f;
-      uint32_t pk[32], pk2[32];
-      tc_softmax_half(sa, sb, scale_log2, neg_m, l_tile, pk);
-      if (!resc) {
-        tc_st32(tmem_s, pk);
-        tmem_st_wait();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&p_lo[sub]);
-      }
-      __syncwarp();
-      if (lane == 0 && (sub == 0 ? (j < n_other) : (j + 1 < n_other))) mbar_arrive(&turn[(sub ^ 1) * 4 + (warp & 3)]);
-      tc_softmax_half(sc, sd, scale_log2, neg_m, l_tile, pk2);
-      if (resc) {
-        // O moves to the new maximum before any of this tile's P is used.  S(j) was ready only after P V(j-1) had
-        // finished (the tensor pipe ran it first), so O is quiet.
-#pragma unroll
-        for (int c = 0; c < D; c += 32) {
-          uint32_t oa[32];
-          tmem_ld32(tmem_o + c, oa);
-          tmem_ld_wait();
-#pragma unroll
-          for (int i = 0; i < 32; ++i) oa[i] = __float_as_uint(__uint_as_float(oa[i]) * corr);
-          tc_st32(tmem_o + c, oa);
-        }
+      const uint64_t scale2 = f32x2(scale_log2, scale_log2), neg_m2 = f32x2(kTcShift - m_use, kTcShift - m_use);
+      uint64_t sum[2] = {0, 0};                             // two pairs of +0
+      {
+        uint32_t pk[32];
+        tc_exp32(sa, scale2, neg_m2, sum, pk);
+        tc_exp32(sb, scale2, neg_m2, sum, pk + 16);
         tc_st32(tmem_s, pk);
       }
-      tc_st32(tmem_s + 32, pk2);
-      tmem_st_wait();                                       // P and a rescaled O
+      uint32_t pk[32];
+      tc_exp32(sc, scale2, neg_m2, sum, pk);                // the first half's stores land meanwhile
+      tmem_st_wait();                                       // P's first half and a rescaled O
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) {
-        if (resc) mbar_arrive(&p_lo[sub]);
-        mbar_arrive(&p_hi[sub]);
-      }
+      if (lane == 0) mbar_arrive(&p_lo[sub]);
+      tc_exp32(sd, scale2, neg_m2, sum, pk + 16);
+      tc_st32(tmem_s + 32, pk);
+      tmem_st_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&p_hi[sub]);
+      const float2 total = unpack_f32x2(add_f32x2(sum[0], sum[1]));
+      const float l_tile = total.x + total.y;
       l_run = l_run * corr + l_tile;
     }
     // ---------------------------------------------------------------- epilogue
