@@ -5,10 +5,7 @@
 // an element is an E2M1 code c, element 2 i in the low nibble of byte i, and stands for c * s * scale with
 // one fp32 scale for the keys and one for the values.  Codes u8 [rows][hkv][D / 2], scales e4m3
 // [rows][hkv][D / 16]: 4.5 bits an element against the 8 of the FP8 cache.
-#include <cuda_fp16.h>
-
-#include "msl_common.cuh"
-#include "msl_host.h"
+#include "kv4_common.cuh"
 
 namespace msl {
 
@@ -132,11 +129,15 @@ __global__ void __launch_bounds__(kPlanThreads) page_plan_kernel(PlanArgs p) {
 
 // ============================================================================ store
 // Lanes own 8 consecutive channels of a head, D / 8 lanes a head; two neighbouring lanes share a block of 16.
-// Queries are rounded to bf16 once, so fp32 serves them.  Keys and values end on a coarse grid, where an
-// error of one fp32 ulp next to a border moves a value by a whole step: their norm, rotation and borders are
-// held in 64 bits (this GPU runs them at half the fp32 rate), and codes come from comparisons with
-// border * (s * scale), a product of 24 + 4 + 3 bits that is exact in 64, so that ties are seen as ties.
+// Queries are rounded to bf16 once, so fp32 serves them.  Keys and values end on a coarse grid, where an error of one
+// fp32 ulp next to a border moves a value by a whole step.  So borders are decided on values held in 64 bits, where it
+// matters: norm and rotation of the keys run in 64 bits (at half the fp32 rate on this GPU; a value is 64 bits exact as
+// far as the grid can tell), a code is formed in fp32 from the value nudged up and down by 2^-20, and where the two
+// disagree the border is compared in 64 bits (s * scale has 24 + 4 bits, a border of the grid 3: exact, so ties are
+// seen as ties).  Comparing every value with the seven borders in 64 bits: 139 us for 16384 tokens of 32 + 8 + 8 heads
+// x 128, issue bound (6700 warp instructions a token).
 constexpr int kStoreThreads = 256;
+constexpr int kStoreTok = 2;
 
 // bf16 bits -> double, exact for finite values; infinities and NaN become finite, +-2^128 and above: the
 // format has no code for them, and they saturate like any value beyond its range.
@@ -146,9 +147,8 @@ __device__ __forceinline__ double bf16_bits_to_f64(uint32_t b) {
   return d * __hiloint2double((1023 + 896) << 20, 0);
 }
 
-__device__ __forceinline__ double shfl_xor_f64(double v, int o) {
-  return __hiloint2double(__shfl_xor_sync(0xffffffffu, __double2hiint(v), o),
-                          __shfl_xor_sync(0xffffffffu, __double2loint(v), o));
+__device__ __forceinline__ double shfl_xor_f64(uint32_t mask, double v, int o) {
+  return __hiloint2double(__shfl_xor_sync(mask, __double2hiint(v), o), __shfl_xor_sync(mask, __double2loint(v), o));
 }
 
 // Nearest E4M3 of x in [0, 448], ties to even: rounding to odd in fp32 first keeps the second rounding right.
@@ -159,6 +159,42 @@ __device__ __forceinline__ uint32_t e4m3_of_f64(double x) {
 }
 __device__ __forceinline__ float e4m3_to_f32(uint32_t b) {
   return __half2float(__half(__nv_cvt_fp8_to_halfraw(static_cast<__nv_fp8_storage_t>(b), __NV_E4M3)));
+}
+
+// Nearest E2M1 codes of u[i] * f (saturating), element i in nibble i.  u + 0 keeps a zero's code 0 whatever its sign.
+__device__ __forceinline__ uint32_t e2m1_of_8(const float (&u)[8], float f) {
+  float v[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = fmaf(u[i], f, 0.0f);
+  uint32_t w;
+  asm("{.reg .b8 a, b, c, d;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\n\tcvt.rn.satfinite.e2m1x2.f32 b, %4, %3;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 c, %6, %5;\n\tcvt.rn.satfinite.e2m1x2.f32 d, %8, %7;\n\t"
+      "mov.b32 %0, {a, b, c, d};}"
+      : "=r"(w)
+      : "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]));
+  return w;
+}
+
+// (cos, sin) of an angle of any size, good to about 1e-14: quarter turns are taken off in 64 bits (pi / 2 as a sum of
+// two doubles), what is left has at most pi / 4, where the Taylor series to r^14 serves.
+__device__ __forceinline__ double2 cos_sin_f64(double a) {
+  const double n = rint(a * 0.63661977236758134);
+  const double r = fma(-n, 6.123233995736766e-17, fma(-n, 1.5707963267948966, a));
+  const double q = r * r;
+  double s = 1.0 / 6227020800.0, c = -1.0 / 87178291200.0;
+  s = fma(s, q, -1.0 / 39916800.0); c = fma(c, q, 1.0 / 479001600.0);
+  s = fma(s, q, 1.0 / 362880.0); c = fma(c, q, -1.0 / 3628800.0);
+  s = fma(s, q, -1.0 / 5040.0); c = fma(c, q, 1.0 / 40320.0);
+  s = fma(s, q, 1.0 / 120.0); c = fma(c, q, -1.0 / 720.0);
+  s = fma(s, q, -1.0 / 6.0); c = fma(c, q, 1.0 / 24.0);
+  c = fma(c, q, -0.5);
+  s = fma(s * q, r, r);
+  c = fma(c, q, 1.0);
+  // n mod 4 from the low bits of n + 1.5 * 2^52
+  const int k = __double2loint(n + 6755399441055744.0) & 3;
+  const double x = (k & 1) ? s : c, y = (k & 1) ? c : s;
+  return make_double2((k == 1 || k == 2) ? -x : x, (k & 2) ? -y : y);
 }
 
 struct StoreArgs {
@@ -176,128 +212,199 @@ struct StoreArgs {
   int* status;
 };
 
+// Block x takes tokens [kStoreTok x, + kStoreTok) with all their heads, 256 lanes at a time; the rotations of its tokens
+// are formed once, while the first loads are in flight.
 template <int D>
 __global__ void __launch_bounds__(kStoreThreads)
 qk_rope_store_kv4_kernel(StoreArgs p) {
   constexpr int LPH = D / 8;
-  __shared__ double2 rot[D / 2];          // (cos, sin) of position * inv_freq[j]
-  const int t = blockIdx.x;
+  // (cos, sin) of position * inv_freq[4 lane + i] at [i][lane]: a warp's reads are contiguous
+  __shared__ double2 rot[kStoreTok][4][LPH];
+  __shared__ float2 rot32[kStoreTok][4][LPH];
   const int lanes = (p.hq + 2 * p.hkv) * LPH;
-  const int idx = blockIdx.y * kStoreThreads + threadIdx.x;
-  const bool live = idx < lanes;
-  const int h = idx / LPH, sub = idx % LPH;
-  uint4 raw = make_uint4(0, 0, 0, 0);
-  if (live) raw = *reinterpret_cast<const uint4*>(p.qkv + t * p.ld + h * D + sub * 8);
+  const int t0 = blockIdx.x * kStoreTok, nt = min(kStoreTok, p.tokens - t0);
+  const int sub = threadIdx.x % LPH;
+  const uint32_t mask = (0xffffffffu >> (32 - LPH)) << (threadIdx.x & 31 & ~(LPH - 1));   // the lanes of this head
+  uint4 raw[kStoreTok];
+  const auto fetch = [&](int idx) {
+#pragma unroll
+    for (int tt = 0; tt < kStoreTok; ++tt)
+      raw[tt] = idx < lanes && tt < nt ? *reinterpret_cast<const uint4*>(p.qkv + (t0 + tt) * p.ld + idx * 8)
+                                       : make_uint4(0, 0, 0, 0);
+  };
+  fetch(threadIdx.x);
   if (p.inv_freq != nullptr) {
-    for (int j = threadIdx.x; j < D / 2; j += kStoreThreads) {
-      // the angle's whole turns are taken off in 64 bits: 2 pi as a sum of two doubles
-      const double a = static_cast<double>(p.positions[t]) * static_cast<double>(p.inv_freq[j]);
-      const double n = rint(a * 0.15915494309189535);
-      const double r = fma(-n, 2.4492935982947064e-16, fma(-n, 6.283185307179586, a));
-      double sn, cs;
-      sincos(r, &sn, &cs);
-      rot[j] = make_double2(cs, sn);
+    for (int x = threadIdx.x; x < kStoreTok * (D / 2); x += kStoreThreads) {
+      const int tt = x / (D / 2), j = x % (D / 2);
+      if (tt < nt) {
+        const double2 cs = cos_sin_f64(static_cast<double>(p.positions[t0 + tt]) * static_cast<double>(p.inv_freq[j]));
+        rot[tt][j % 4][j / 4] = cs;
+        rot32[tt][j % 4][j / 4] = make_float2(static_cast<float>(cs.x), static_cast<float>(cs.y));
+      }
     }
     __syncthreads();
   }
-  const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
-  const bool is_q = h < p.hq, is_v = h >= p.hq + p.hkv;
-  double z[8];
-  double ss = 0.0;
+  for (int idx = threadIdx.x; idx < lanes; idx += kStoreThreads) {   // a head's lanes stay together
+    uint4 now[kStoreTok];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    z[i] = bf16_bits_to_f64((w[i / 2] >> (16 * (i & 1))) & 0xffffu);
-    ss += z[i] * z[i];
-  }
+    for (int tt = 0; tt < kStoreTok; ++tt) now[tt] = raw[tt];
+    fetch(idx + kStoreThreads);
+    const int h = idx / LPH;
 #pragma unroll
-  for (int o = LPH / 2; o > 0; o >>= 1) ss += shfl_xor_f64(ss, o);
-  if (!is_v) {
-    const double r = 1.0 / sqrt(ss / D + 1e-5);
+    for (int tt = 0; tt < kStoreTok; ++tt) {
+      if (tt >= nt) break;
+      const int64_t t = t0 + tt;
+      const uint32_t w[4] = {now[tt].x, now[tt].y, now[tt].z, now[tt].w};
+      float v[8];
 #pragma unroll
-    for (int i = 0; i < 8; i += 2) {
-      double e = z[i] * r, o = z[i + 1] * r;
-      if (p.inv_freq != nullptr) {
-        const double2 cs = rot[(sub * 8 + i) / 2];
-        const double e2 = e * cs.x - o * cs.y;
-        o = e * cs.y + o * cs.x;
-        e = e2;
+      for (int i = 0; i < 8; ++i) v[i] = bf16_bits_to_f32((w[i / 2] >> (16 * (i & 1))) & 0xffffu);
+      if (h < p.hq) {
+        float ss = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) ss += v[i] * v[i];
+#pragma unroll
+        for (int o = LPH / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(mask, ss, o);
+        const float r = rsqrtf(ss * (1.0f / D) + 1e-5f);
+        uint32_t out[4];
+#pragma unroll
+        for (int i = 0; i < 8; i += 2) {
+          float e = v[i] * r, o = v[i + 1] * r;
+          if (p.inv_freq != nullptr) {
+            const float2 cs = rot32[tt][i / 2][sub];
+            const float e2 = e * cs.x - o * cs.y;
+            o = e * cs.y + o * cs.x;
+            e = e2;
+          }
+          out[i / 2] = pack_bf16x2(e, o);
+        }
+        *reinterpret_cast<uint4*>(p.q + (t * p.hq + h) * D + sub * 8) = make_uint4(out[0], out[1], out[2], out[3]);
+        continue;
       }
-      z[i] = e;
-      z[i + 1] = o;
+      const bool is_v = h >= p.hq + p.hkv;
+      double z[8];                                          // keys only: values are exact in v
+      if (!is_v) {
+        double ss = 0.0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          z[i] = bf16_bits_to_f64((w[i / 2] >> (16 * (i & 1))) & 0xffffu);
+          ss += z[i] * z[i];
+        }
+#pragma unroll
+        for (int o = LPH / 2; o > 0; o >>= 1) ss += shfl_xor_f64(mask, ss, o);
+        const double r = 1.0 / sqrt(ss / D + 1e-5);
+#pragma unroll
+        for (int i = 0; i < 8; i += 2) {
+          double e = z[i] * r, o = z[i + 1] * r;
+          if (p.inv_freq != nullptr) {
+            const double2 cs = rot[tt][i / 2][sub];
+            const double e2 = e * cs.x - o * cs.y;
+            o = e * cs.y + o * cs.x;
+            e = e2;
+          }
+          z[i] = e;
+          z[i + 1] = o;
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = static_cast<float>(z[i]);
+      } else {
+        // no code for infinities and NaN: the largest finite magnitude, with the sign they have
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = copysignf(fminf(fabsf(v[i]), 3.402823466e38f), v[i]);
+      }
+      const auto exact = [&](int i) { return is_v ? static_cast<double>(v[i]) : z[i]; };
+      float amax = 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) amax = fmaxf(amax, fabsf(v[i]));
+      amax = fmaxf(amax, __shfl_xor_sync(mask, amax, 1));
+      const float scale = is_v ? *p.v_scale : *p.k_scale;
+      // the block scale; within 2^-20 of a midpoint of E4M3 (or among its subnormals) it is decided in 64 bits
+      const float want = fminf(amax / (6.0f * scale), 448.0f);
+      uint32_t s8 = __nv_cvt_float_to_fp8(want, __NV_SATFINITE, __NV_E4M3);
+      const int from_mid = static_cast<int>(__float_as_uint(want) & 0xfffffu) - 0x80000;
+      if (want < 0.015625f || (from_mid >= -8 && from_mid <= 8)) {   // the same for both lanes of a block
+        double top = 0.0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) top = fmax(top, fabs(exact(i)));
+        top = fmax(top, shfl_xor_f64(3u << (threadIdx.x & 30), top, 1));
+        s8 = e4m3_of_f64(fmin(top / (6.0 * static_cast<double>(scale)), 448.0));
+      }
+      const float s = e4m3_to_f32(s8);
+      const float inv = 1.0f / (s * scale);
+      uint32_t packed = e2m1_of_8(v, inv * (1.0f + 9.5367431640625e-7f));
+      uint32_t unsure = (packed ^ e2m1_of_8(v, inv * (1.0f - 9.5367431640625e-7f)));
+      if (s8 == 0) { packed = 0; unsure = 0; }              // a block below half the smallest scale
+      if (unsure) {
+        const double c = static_cast<double>(s) * static_cast<double>(scale);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          if ((unsure >> (4 * i)) & 15u) {
+            // packed has the upper code; 4 x the border below it: 1 3 5 7 10 14 20
+            const uint32_t up = (packed >> (4 * i)) & 7u;
+            const uint32_t border4 = static_cast<uint32_t>(0x140e0a0705030100ull >> (8 * up)) & 255u;
+            const double d = fma(-0.25 * border4, c, fabs(exact(i)));
+            if (d < 0.0 || (d == 0.0 && (up & 1u))) packed -= 1u << (4 * i);   // a tie goes to the even code
+          }
+        }
+      }
+      const int64_t row = p.cache_loc[t];
+      if (row < 0) continue;                                // a padding token
+      if (row >= p.cache_rows) { report_error(p.status, MSL_ERR_CAPACITY); continue; }
+      const int64_t at = row * p.hkv + (is_v ? h - p.hq - p.hkv : h - p.hq);
+      *reinterpret_cast<uint32_t*>((is_v ? p.v : p.k) + at * (D / 2) + sub * 4) = packed;
+      if ((sub & 1) == 0) (is_v ? p.vs : p.ks)[at * (D / 16) + sub / 2] = static_cast<uint8_t>(s8);
     }
   }
-  double amax = 0.0;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) amax = fmax(amax, fabs(z[i]));
-  amax = fmax(amax, shfl_xor_f64(amax, 1));
-  if (!live) return;
-  if (is_q) {
-    uint4 o;
-    o.x = pack_bf16x2(static_cast<float>(z[0]), static_cast<float>(z[1]));
-    o.y = pack_bf16x2(static_cast<float>(z[2]), static_cast<float>(z[3]));
-    o.z = pack_bf16x2(static_cast<float>(z[4]), static_cast<float>(z[5]));
-    o.w = pack_bf16x2(static_cast<float>(z[6]), static_cast<float>(z[7]));
-    *reinterpret_cast<uint4*>(p.q + (static_cast<int64_t>(t) * p.hq + h) * D + sub * 8) = o;
-    return;
-  }
-  const int64_t row = p.cache_loc[t];
-  if (row < 0) return;                                      // a padding token
-  if (row >= p.cache_rows) { report_error(p.status, MSL_ERR_CAPACITY); return; }
-  const double scale = is_v ? *p.v_scale : *p.k_scale;
-  const uint32_t s8 = e4m3_of_f64(fmin(amax / (6.0 * scale), 448.0));
-  const double c = static_cast<double>(e4m3_to_f32(s8)) * scale;
-  uint32_t packed = 0;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const double m = fabs(z[i]);
-    uint32_t code = (m > 0.25 * c) + (m >= 0.75 * c) + (m > 1.25 * c) + (m >= 1.75 * c) + (m > 2.5 * c) +
-                    (m >= 3.5 * c) + (m > 5.0 * c);
-    if (z[i] < 0.0) code |= 8u;
-    packed |= code << (4 * i);
-  }
-  if (s8 == 0) packed = 0;                                  // a block below half the smallest scale
-  const int head = is_v ? h - p.hq - p.hkv : h - p.hq;
-  uint8_t* codes = is_v ? p.v : p.k;
-  uint8_t* scales = is_v ? p.vs : p.ks;
-  const int64_t at = row * p.hkv + head;
-  *reinterpret_cast<uint32_t*>(codes + at * (D / 2) + sub * 4) = packed;
-  if ((sub & 1) == 0) scales[at * (D / 16) + sub / 2] = static_cast<uint8_t>(s8);
 }
 
 // ============================================================================ read-back
-// out[i] = the values of cache row rows[i] (zeros for a negative index), one lane per 8 codes.
+// out[i] = the values of cache row rows[i] (zeros for a negative index), one lane per block of 16: 8 bytes of codes and
+// a scale in, 32 or 64 bytes out.
+constexpr int kRowsThreads = 256;
 template <typename OUT>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(kRowsThreads)
 kv4_rows_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, const float* __restrict__ scale,
-                const int64_t* __restrict__ rows, int64_t n, int width, int64_t cache_rows, OUT* __restrict__ out,
-                int* status) {
-  const int per_row = width / 8;
-  const int64_t idx = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-  if (idx >= n * per_row) return;
-  const int64_t i = idx / per_row;
-  const int c = static_cast<int>(idx % per_row);
-  const int64_t row = rows[i];
-  float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-  if (row >= cache_rows) report_error(status, MSL_ERR_CAPACITY);
-  if (row >= 0 && row < cache_rows) {
-    const uint32_t w = *reinterpret_cast<const uint32_t*>(codes + row * (width / 2) + c * 4);
-    const float s = e4m3_to_f32(scales[row * (width / 16) + c / 2]);
-    const float t = *scale;
-#pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      const uint32_t code = (w >> (4 * k)) & 15u, m = code & 7u;
-      // code * s is exact (2 + 4 bits), so the fp32 product with the tensor's scale rounds once
-      const float mag = m < 4 ? 0.5f * m : (m < 6 ? static_cast<float>(m - 2) : 2.0f * m - 8.0f);
-      v[k] = ((code & 8u) ? -mag : mag) * s * t;
+                const int64_t* __restrict__ rows, int64_t n, int blocks, int rows_per_cta, int64_t cache_rows,
+                OUT* __restrict__ out, int* status) {
+  const float t = *scale;
+  const int64_t first = static_cast<int64_t>(blockIdx.x) * rows_per_cta;
+  for (int x = threadIdx.x; x < rows_per_cta * blocks; x += kRowsThreads) {
+    const int64_t i = first + x / blocks;
+    if (i >= n) return;
+    const int64_t row = rows[i];
+    uint2 w = make_uint2(0, 0);
+    float s = 0.f;
+    if (row >= cache_rows) {
+      report_error(status, MSL_ERR_CAPACITY);
+    } else if (row >= 0) {
+      const int64_t at = row * blocks + x % blocks;
+      w = *reinterpret_cast<const uint2*>(codes + at * 8);
+      s = e4m3_to_f32(scales[at]);
     }
-  }
-  if constexpr (sizeof(OUT) == 2) {
-    *reinterpret_cast<uint4*>(out + idx * 8) = make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]),
-                                                          pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
-  } else {
-    float4* dst = reinterpret_cast<float4*>(out + idx * 8);
-    dst[0] = make_float4(v[0], v[1], v[2], v[3]);
-    dst[1] = make_float4(v[4], v[5], v[6], v[7]);
+    // code * s is exact (2 + 4 bits), so the fp32 product with the tensor's scale rounds once
+    float v[16];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      __half2 h[4];
+      e2m1x8(k ? w.y : w.x, h);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float2 f = __half22float2(h[j]);
+        v[8 * k + 2 * j] = f.x * s * t;
+        v[8 * k + 2 * j + 1] = f.y * s * t;
+      }
+    }
+    OUT* dst = out + (first * blocks + x) * 16;
+    if constexpr (sizeof(OUT) == 2) {
+#pragma unroll
+      for (int k = 0; k < 2; ++k)
+        reinterpret_cast<uint4*>(dst)[k] =
+            make_uint4(pack_bf16x2(v[8 * k], v[8 * k + 1]), pack_bf16x2(v[8 * k + 2], v[8 * k + 3]),
+                       pack_bf16x2(v[8 * k + 4], v[8 * k + 5]), pack_bf16x2(v[8 * k + 6], v[8 * k + 7]));
+    } else {
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        reinterpret_cast<float4*>(dst)[k] = make_float4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]);
+    }
   }
 }
 
@@ -343,8 +450,7 @@ extern "C" int msl_qk_rope_store_kv4(const void* qkv, int64_t ld, const int64_t*
   const StoreArgs a{static_cast<const __nv_bfloat16*>(qkv), ld, positions, cache_loc, inv_freq, k_scale, v_scale,
                     static_cast<__nv_bfloat16*>(q), static_cast<uint8_t*>(k_cache), static_cast<uint8_t*>(k_sf),
                     static_cast<uint8_t*>(v_cache), static_cast<uint8_t*>(v_sf), tokens, hq, hkv, cache_rows, status};
-  const int lanes = (hq + 2 * hkv) * (head_dim / 8);
-  const dim3 grid(tokens, (lanes + kStoreThreads - 1) / kStoreThreads);
+  const int grid = (tokens + kStoreTok - 1) / kStoreTok;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (head_dim == 128) qk_rope_store_kv4_kernel<128><<<grid, kStoreThreads, 0, st>>>(a);
   else qk_rope_store_kv4_kernel<64><<<grid, kStoreThreads, 0, st>>>(a);
@@ -357,16 +463,18 @@ extern "C" int msl_kv4_rows(const void* codes, const void* scales, const float* 
   if (n == 0) return MSL_OK;
   if (!codes || !scales || !scale || !rows || !out) return MSL_ERR_ARG;
   if ((width & 15) || misaligned(codes, 16) || misaligned(out, 16)) return MSL_ERR_ALIGN;
-  const int64_t blocks = (n * (width / 8) + 255) / 256;
-  if (blocks > 0x7fffffff) return MSL_ERR_UNSUPPORTED;
+  const int blocks = width / 16;
+  const int per = std::max(1, kRowsThreads / blocks);       // whole rows a CTA
+  const int64_t grid = (n + per - 1) / per;
+  if (grid > 0x7fffffff) return MSL_ERR_UNSUPPORTED;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const auto* c = static_cast<const uint8_t*>(codes);
   const auto* s = static_cast<const uint8_t*>(scales);
   if (out_mode == MSL_OUT_BF16)
-    kv4_rows_kernel<<<static_cast<unsigned>(blocks), 256, 0, st>>>(c, s, scale, rows, n, width, cache_rows,
-                                                                  static_cast<__nv_bfloat16*>(out), status);
+    kv4_rows_kernel<<<static_cast<unsigned>(grid), kRowsThreads, 0, st>>>(
+        c, s, scale, rows, n, blocks, per, cache_rows, static_cast<__nv_bfloat16*>(out), status);
   else
-    kv4_rows_kernel<<<static_cast<unsigned>(blocks), 256, 0, st>>>(c, s, scale, rows, n, width, cache_rows,
-                                                                  static_cast<float*>(out), status);
+    kv4_rows_kernel<<<static_cast<unsigned>(grid), kRowsThreads, 0, st>>>(c, s, scale, rows, n, blocks, per, cache_rows,
+                                                                         static_cast<float*>(out), status);
   return cudaGetLastError() == cudaSuccess ? MSL_OK : MSL_ERR_CUDA;
 }
