@@ -128,16 +128,16 @@ __global__ void __launch_bounds__(kPlanThreads) page_plan_kernel(PlanArgs p) {
 }
 
 // ============================================================================ store
-// Lanes own 8 consecutive channels of a head, D / 8 lanes a head; two neighbouring lanes share a block of 16.
-// Queries are rounded to bf16 once, so fp32 serves them.  Keys and values end on a coarse grid, where an error of one
-// fp32 ulp next to a border moves a value by a whole step.  So borders are decided on values held in 64 bits, where it
-// matters: norm and rotation of the keys run in 64 bits (at half the fp32 rate on this GPU; a value is 64 bits exact as
-// far as the grid can tell), a code is formed in fp32 from the value nudged up and down by 2^-20, and where the two
-// disagree the border is compared in 64 bits (s * scale has 24 + 4 bits, a border of the grid 3: exact, so ties are
-// seen as ties).  Comparing every value with the seven borders in 64 bits: 139 us for 16384 tokens of 32 + 8 + 8 heads
-// x 128, issue bound (6700 warp instructions a token).
-constexpr int kStoreThreads = 256;
-constexpr int kStoreTok = 2;
+// Lanes own 8 consecutive channels of a head, D / 8 lanes a head; two neighbouring lanes share a block of 16.  Queries
+// are rounded to bf16 once, so fp32 serves them.  Keys and values end on a coarse grid, where an error of one fp32 ulp
+// next to a border moves a value by a whole step.  So fp32 only proposes: scale and codes are formed from the value
+// nudged up and down by more than the fp32 error (below), and where the two disagree 64 bits decide: a value against
+// border * (s * scale), 3 + 4 + 24 bits and exact, so that ties are seen as ties; a key (its norm and rotation are not
+// exact in fp32) by doing its heads again in 64 bits, which one warp in a hundred has to.
+// What it is bound by is issue slots: 16384 tokens of 32 + 8 + 8 heads x 128 took 190 us with everything in 64 bits,
+// 116 with the queries in fp32.
+constexpr int kStoreThreads = 256, kStoreWarps = kStoreThreads / 32;
+constexpr int kStoreTok = 4;               // most tokens of a block
 
 // bf16 bits -> double, exact for finite values; infinities and NaN become finite, +-2^128 and above: the
 // format has no code for them, and they saturate like any value beyond its range.
@@ -161,11 +161,9 @@ __device__ __forceinline__ float e4m3_to_f32(uint32_t b) {
   return __half2float(__half(__nv_cvt_fp8_to_halfraw(static_cast<__nv_fp8_storage_t>(b), __NV_E4M3)));
 }
 
-// Nearest E2M1 codes of u[i] * f (saturating), element i in nibble i.  u + 0 keeps a zero's code 0 whatever its sign.
-__device__ __forceinline__ uint32_t e2m1_of_8(const float (&u)[8], float f) {
-  float v[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = fmaf(u[i], f, 0.0f);
+// Nearest E2M1 codes (saturating) of u[i] * f, its magnitude moved by `nudge`; element i in nibble i.  Without a nudge,
+// + 0 keeps a zero's code 0 whatever its sign.
+__device__ __forceinline__ uint32_t e2m1_pack(const float (&v)[8]) {
   uint32_t w;
   asm("{.reg .b8 a, b, c, d;\n\t"
       "cvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\n\tcvt.rn.satfinite.e2m1x2.f32 b, %4, %3;\n\t"
@@ -175,9 +173,22 @@ __device__ __forceinline__ uint32_t e2m1_of_8(const float (&u)[8], float f) {
       : "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]));
   return w;
 }
+__device__ __forceinline__ uint32_t e2m1_of_8(const float (&u)[8], float f) {
+  float v[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = fmaf(u[i], f, 0.0f);
+  return e2m1_pack(v);
+}
+__device__ __forceinline__ uint32_t e2m1_of_8(const float (&u)[8], float f, float nudge) {
+  float v[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i)   // copysign takes the magnitude alone: a downward nudge gets the other sign
+    v[i] = fmaf(u[i], f, nudge > 0.f ? copysignf(nudge, u[i]) : -copysignf(nudge, u[i]));
+  return e2m1_pack(v);
+}
 
-// (cos, sin) of an angle of any size, good to about 1e-14: quarter turns are taken off in 64 bits (pi / 2 as a sum of
-// two doubles), what is left has at most pi / 4, where the Taylor series to r^14 serves.
+// (cos, sin) of an angle of any size: quarter turns are taken off in 64 bits (pi / 2 as a sum of two doubles), what is
+// left has at most pi / 4, where a Taylor series serves: to r^14, good to about 1e-14, or in fp32 to r^10.
 __device__ __forceinline__ double2 cos_sin_f64(double a) {
   const double n = rint(a * 0.63661977236758134);
   const double r = fma(-n, 6.123233995736766e-17, fma(-n, 1.5707963267948966, a));
@@ -197,6 +208,22 @@ __device__ __forceinline__ double2 cos_sin_f64(double a) {
   return make_double2((k == 1 || k == 2) ? -x : x, (k & 2) ? -y : y);
 }
 
+__device__ __forceinline__ float2 cos_sin_f32(double a) {
+  const double n = rint(a * 0.63661977236758134);
+  const float r = static_cast<float>(fma(-n, 6.123233995736766e-17, fma(-n, 1.5707963267948966, a)));
+  const float q = r * r;
+  float s = 2.7557319e-6f, c = -2.7557319e-7f;             // 1 / 9!, -1 / 10!
+  s = fmaf(s, q, -1.9841270e-4f); c = fmaf(c, q, 2.4801587e-5f);
+  s = fmaf(s, q, 8.3333333e-3f); c = fmaf(c, q, -1.3888889e-3f);
+  s = fmaf(s, q, -1.6666667e-1f); c = fmaf(c, q, 4.1666667e-2f);
+  c = fmaf(c, q, -0.5f);
+  s = fmaf(s * q, r, r);
+  c = fmaf(c, q, 1.0f);
+  const int k = __double2loint(n + 6755399441055744.0) & 3;
+  const float x = (k & 1) ? s : c, y = (k & 1) ? c : s;
+  return make_float2((k == 1 || k == 2) ? -x : x, (k & 2) ? -y : y);
+}
+
 struct StoreArgs {
   const __nv_bfloat16* qkv;
   int64_t ld;
@@ -208,150 +235,206 @@ struct StoreArgs {
   __nv_bfloat16* q;             // [tokens][hq][D]
   uint8_t *k, *ks, *v, *vs;
   int tokens, hq, hkv;
+  int per_block;                // tokens of a block
   int64_t cache_rows;
   int* status;
 };
 
-// Block x takes tokens [kStoreTok x, + kStoreTok) with all their heads, 256 lanes at a time; the rotations of its tokens
-// are formed once, while the first loads are in flight.
-template <int D>
-__global__ void __launch_bounds__(kStoreThreads)
+// The E4M3 scale of a block from its largest magnitude in fp32, relative error below 2^-18; `sure` is false near a
+// midpoint of E4M3 and among its subnormals.
+__device__ __forceinline__ uint32_t block_scale(float amax, float inv_scale, bool& sure) {
+  const float want = fminf(amax * (inv_scale * (1.0f / 6.0f)), 448.0f);
+  const int from_mid = static_cast<int>(__float_as_uint(want) & 0xfffffu) - 0x80000;
+  sure = want >= 0.015625f && (from_mid < -64 || from_mid > 64);
+  return __nv_cvt_float_to_fp8(want, __NV_SATFINITE, __NV_E4M3);
+}
+
+// A key head's 8 channels of this lane in 64 bits, start to end; the whole warp takes part (two or four heads).
+template <int D, bool ROPE>
+__device__ __noinline__ uint32_t key_codes_f64(const uint4 raw, double position, const float* inv_freq, double scale,
+                                               uint32_t& s8) {
+  constexpr int LPH = D / 8;
+  const int sub = threadIdx.x % LPH;
+  const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+  double z[8], ss = 0.0, top = 0.0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    z[i] = bf16_bits_to_f64((w[i / 2] >> (16 * (i & 1))) & 0xffffu);
+    ss = fma(z[i], z[i], ss);
+  }
+#pragma unroll
+  for (int o = LPH / 2; o > 0; o >>= 1) ss += shfl_xor_f64(0xffffffffu, ss, o);
+  const double r = 1.0 / sqrt(ss / D + 1e-5);
+#pragma unroll
+  for (int i = 0; i < 8; i += 2) {
+    double e = z[i] * r, o = z[i + 1] * r;
+    if (ROPE) {
+      const double2 cs = cos_sin_f64(position * static_cast<double>(inv_freq[sub * 4 + i / 2]));
+      const double e2 = e * cs.x - o * cs.y;
+      o = e * cs.y + o * cs.x;
+      e = e2;
+    }
+    z[i] = e;
+    z[i + 1] = o;
+    top = fmax(top, fmax(fabs(e), fabs(o)));
+  }
+  top = fmax(top, shfl_xor_f64(0xffffffffu, top, 1));
+  s8 = e4m3_of_f64(fmin(top / (6.0 * scale), 448.0));
+  const double c = static_cast<double>(e4m3_to_f32(s8)) * scale;
+  uint32_t packed = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const double m = fabs(z[i]);
+    uint32_t code = (m > 0.25 * c) + (m >= 0.75 * c) + (m > 1.25 * c) + (m >= 1.75 * c) + (m > 2.5 * c) +
+                    (m >= 3.5 * c) + (m > 5.0 * c);
+    if (z[i] < 0.0) code |= 8u;
+    packed |= code << (4 * i);
+  }
+  return s8 == 0 ? 0u : packed;                             // a block below half the smallest scale
+}
+
+// A block takes p.per_block tokens with all their heads: their rotations first (a thread an angle), then the lanes of
+// their queries, keys and values in units of 32, dealt out to the warps in turn; a unit's heads have one role.
+template <int D, bool ROPE>
+__global__ void __launch_bounds__(kStoreThreads, 4)
 qk_rope_store_kv4_kernel(StoreArgs p) {
   constexpr int LPH = D / 8;
   // (cos, sin) of position * inv_freq[4 lane + i] at [i][lane]: a warp's reads are contiguous
-  __shared__ double2 rot[kStoreTok][4][LPH];
-  __shared__ float2 rot32[kStoreTok][4][LPH];
-  const int lanes = (p.hq + 2 * p.hkv) * LPH;
-  const int t0 = blockIdx.x * kStoreTok, nt = min(kStoreTok, p.tokens - t0);
-  const int sub = threadIdx.x % LPH;
-  const uint32_t mask = (0xffffffffu >> (32 - LPH)) << (threadIdx.x & 31 & ~(LPH - 1));   // the lanes of this head
-  uint4 raw[kStoreTok];
-  const auto fetch = [&](int idx) {
-#pragma unroll
-    for (int tt = 0; tt < kStoreTok; ++tt)
-      raw[tt] = idx < lanes && tt < nt ? *reinterpret_cast<const uint4*>(p.qkv + (t0 + tt) * p.ld + idx * 8)
-                                       : make_uint4(0, 0, 0, 0);
+  __shared__ float2 rot[kStoreTok][4][LPH];
+  const int t0 = blockIdx.x * p.per_block, nt = min(p.per_block, p.tokens - t0);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, sub = threadIdx.x % LPH;
+  const __nv_bfloat16* src = p.qkv + t0 * p.ld;
+  const int q_lanes = p.hq * LPH, kv_lanes = p.hkv * LPH;
+  const int q_units = (q_lanes + 31) / 32, kv_units = (kv_lanes + 31) / 32, units = q_units + 2 * kv_units;
+  // unit u: its first lane, and the first lane and the end of its role among the token's lanes
+  const auto role_of = [&](int u, int& at, int& first, int& count) {
+    const int kv = u - q_units;
+    first = kv < 0 ? 0 : kv < kv_units ? q_lanes : q_lanes + kv_lanes;
+    count = kv < 0 ? q_lanes : kv_lanes;
+    at = 32 * (kv < 0 ? u : kv < kv_units ? kv : kv - kv_units) + lane;
+    return kv;
   };
-  fetch(threadIdx.x);
-  if (p.inv_freq != nullptr) {
-    for (int x = threadIdx.x; x < kStoreTok * (D / 2); x += kStoreThreads) {
-      const int tt = x / (D / 2), j = x % (D / 2);
-      if (tt < nt) {
-        const double2 cs = cos_sin_f64(static_cast<double>(p.positions[t0 + tt]) * static_cast<double>(p.inv_freq[j]));
-        rot[tt][j % 4][j / 4] = cs;
-        rot32[tt][j % 4][j / 4] = make_float2(static_cast<float>(cs.x), static_cast<float>(cs.y));
-      }
+  const auto load = [&](int tt, int u) {                    // lanes past the role's end go through the motions
+    int at, first, count;
+    role_of(u, at, first, count);
+    return at < count ? *reinterpret_cast<const uint4*>(src + tt * p.ld + (first + at) * 8) : make_uint4(0, 0, 0, 0);
+  };
+  int u = warp, tt = 0;
+  const auto settle = [&]() {                               // on to the token that unit u falls into
+    while (u >= units) { u -= units; ++tt; }
+  };
+  settle();
+  uint4 next = tt < nt ? load(tt, u) : make_uint4(0, 0, 0, 0);
+  if (ROPE) {
+    for (int x = threadIdx.x; x < nt * (D / 2); x += kStoreThreads) {
+      const int t = x / (D / 2), j = x % (D / 2);
+      rot[t][j % 4][j / 4] = cos_sin_f32(static_cast<double>(p.positions[t0 + t]) * static_cast<double>(p.inv_freq[j]));
     }
     __syncthreads();
   }
-  for (int idx = threadIdx.x; idx < lanes; idx += kStoreThreads) {   // a head's lanes stay together
-    uint4 now[kStoreTok];
+  const float k_scale = *p.k_scale, v_scale = *p.v_scale, inv_k = 1.0f / k_scale, inv_v = 1.0f / v_scale;
+  while (tt < nt) {
+    const int now = tt, unit = u;
+    const uint4 raw = next;
+    u += kStoreWarps;
+    settle();
+    if (tt < nt) next = load(tt, u);
+    int at, first, count;
+    const int kv = role_of(unit, at, first, count);
+    const bool in = at < count;
+    uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+    if (kv < kv_units) {
+      // ---- a query or a key: norm and rotation
+      float v[8], ss = 0.f;
 #pragma unroll
-    for (int tt = 0; tt < kStoreTok; ++tt) now[tt] = raw[tt];
-    fetch(idx + kStoreThreads);
-    const int h = idx / LPH;
+      for (int i = 0; i < 8; ++i) {
+        v[i] = __uint_as_float(i & 1 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16);
+        ss = fmaf(v[i], v[i], ss);
+      }
 #pragma unroll
-    for (int tt = 0; tt < kStoreTok; ++tt) {
-      if (tt >= nt) break;
-      const int64_t t = t0 + tt;
-      const uint32_t w[4] = {now[tt].x, now[tt].y, now[tt].z, now[tt].w};
-      float v[8];
+      for (int o = LPH / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+      const float r = rsqrtf(ss * (1.0f / D) + 1e-5f);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = bf16_bits_to_f32((w[i / 2] >> (16 * (i & 1))) & 0xffffu);
-      if (h < p.hq) {
-        float ss = 0.f;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) ss += v[i] * v[i];
-#pragma unroll
-        for (int o = LPH / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(mask, ss, o);
-        const float r = rsqrtf(ss * (1.0f / D) + 1e-5f);
-        uint32_t out[4];
-#pragma unroll
-        for (int i = 0; i < 8; i += 2) {
-          float e = v[i] * r, o = v[i + 1] * r;
-          if (p.inv_freq != nullptr) {
-            const float2 cs = rot32[tt][i / 2][sub];
-            const float e2 = e * cs.x - o * cs.y;
-            o = e * cs.y + o * cs.x;
-            e = e2;
-          }
-          out[i / 2] = pack_bf16x2(e, o);
+      for (int i = 0; i < 4; ++i) {
+        float e = v[2 * i] * r, o = v[2 * i + 1] * r;
+        if (ROPE) {
+          const float2 cs = rot[now][i][sub];
+          const float e2 = e * cs.x - o * cs.y;
+          o = e * cs.y + o * cs.x;
+          e = e2;
         }
-        *reinterpret_cast<uint4*>(p.q + (t * p.hq + h) * D + sub * 8) = make_uint4(out[0], out[1], out[2], out[3]);
+        v[2 * i] = e;
+        v[2 * i + 1] = o;
+      }
+      if (kv < 0) {
+        if (in)
+          *reinterpret_cast<uint4*>(p.q + static_cast<int64_t>(t0 + now) * p.hq * D + at * 8) =
+              make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]),
+                         pack_bf16x2(v[6], v[7]));
         continue;
       }
-      const bool is_v = h >= p.hq + p.hkv;
-      double z[8];                                          // keys only: values are exact in v
-      if (!is_v) {
-        double ss = 0.0;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          z[i] = bf16_bits_to_f64((w[i / 2] >> (16 * (i & 1))) & 0xffffu);
-          ss += z[i] * z[i];
-        }
-#pragma unroll
-        for (int o = LPH / 2; o > 0; o >>= 1) ss += shfl_xor_f64(mask, ss, o);
-        const double r = 1.0 / sqrt(ss / D + 1e-5);
-#pragma unroll
-        for (int i = 0; i < 8; i += 2) {
-          double e = z[i] * r, o = z[i + 1] * r;
-          if (p.inv_freq != nullptr) {
-            const double2 cs = rot[tt][i / 2][sub];
-            const double e2 = e * cs.x - o * cs.y;
-            o = e * cs.y + o * cs.x;
-            e = e2;
-          }
-          z[i] = e;
-          z[i + 1] = o;
-        }
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = static_cast<float>(z[i]);
-      } else {
-        // no code for infinities and NaN: the largest finite magnitude, with the sign they have
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = copysignf(fminf(fabsf(v[i]), 3.402823466e38f), v[i]);
-      }
-      const auto exact = [&](int i) { return is_v ? static_cast<double>(v[i]) : z[i]; };
+      // fp32 errors, in half steps of 2^-24: 10 in r, 1 in e, 3 in cosine and sine, 2 in the rotation, so 16 (|e| + |o|)
+      // <= 32 largest magnitudes of the block: 2^-19 of it, 1.3e-5 of a code's unit; the nudge is 3e-5
       float amax = 0.f;
 #pragma unroll
       for (int i = 0; i < 8; ++i) amax = fmaxf(amax, fabsf(v[i]));
-      amax = fmaxf(amax, __shfl_xor_sync(mask, amax, 1));
-      const float scale = is_v ? *p.v_scale : *p.k_scale;
-      // the block scale; within 2^-20 of a midpoint of E4M3 (or among its subnormals) it is decided in 64 bits
-      const float want = fminf(amax / (6.0f * scale), 448.0f);
-      uint32_t s8 = __nv_cvt_float_to_fp8(want, __NV_SATFINITE, __NV_E4M3);
-      const int from_mid = static_cast<int>(__float_as_uint(want) & 0xfffffu) - 0x80000;
-      if (want < 0.015625f || (from_mid >= -8 && from_mid <= 8)) {   // the same for both lanes of a block
-        double top = 0.0;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) top = fmax(top, fabs(exact(i)));
-        top = fmax(top, shfl_xor_f64(3u << (threadIdx.x & 30), top, 1));
-        s8 = e4m3_of_f64(fmin(top / (6.0 * static_cast<double>(scale)), 448.0));
+      amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+      bool sure;
+      uint32_t s8 = block_scale(amax, inv_k, sure);
+      const float inv = __fdividef(inv_k, e4m3_to_f32(s8));
+      uint32_t packed = e2m1_of_8(v, inv, 3.0517578125e-5f);
+      sure &= packed == e2m1_of_8(v, inv, -3.0517578125e-5f) && ss < 1e38f;
+      if (__any_sync(0xffffffffu, in && !sure))
+        packed = key_codes_f64<D, ROPE>(raw, static_cast<double>(p.positions[t0 + now]), p.inv_freq, k_scale, s8);
+      const int64_t row = p.cache_loc[t0 + now];
+      if (row >= p.cache_rows) report_error(p.status, MSL_ERR_CAPACITY);
+      if (in && row >= 0 && row < p.cache_rows) {           // negative: a padding token
+        const int64_t to = row * kv_lanes + at;             // 4 bytes of codes and half a scale a lane
+        *reinterpret_cast<uint32_t*>(p.k + to * 4) = packed;
+        if ((lane & 1) == 0) p.ks[to >> 1] = static_cast<uint8_t>(s8);
       }
-      const float s = e4m3_to_f32(s8);
-      const float inv = 1.0f / (s * scale);
-      uint32_t packed = e2m1_of_8(v, inv * (1.0f + 9.5367431640625e-7f));
-      uint32_t unsure = (packed ^ e2m1_of_8(v, inv * (1.0f - 9.5367431640625e-7f)));
-      if (s8 == 0) { packed = 0; unsure = 0; }              // a block below half the smallest scale
-      if (unsure) {
-        const double c = static_cast<double>(s) * static_cast<double>(scale);
+      continue;
+    }
+    // ---- a value: exact in fp32; infinities and NaN, which have no code, count as the largest finite magnitude
+    uint32_t top = 0;
+    float v[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          if ((unsure >> (4 * i)) & 15u) {
-            // packed has the upper code; 4 x the border below it: 1 3 5 7 10 14 20
-            const uint32_t up = (packed >> (4 * i)) & 7u;
-            const uint32_t border4 = static_cast<uint32_t>(0x140e0a0705030100ull >> (8 * up)) & 255u;
-            const double d = fma(-0.25 * border4, c, fabs(exact(i)));
-            if (d < 0.0 || (d == 0.0 && (up & 1u))) packed -= 1u << (4 * i);   // a tie goes to the even code
-          }
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t mag = __vminu2(w[i] & 0x7fff7fffu, 0x7f7f7f7fu);
+      top = __vmaxu2(top, mag);
+      w[i] = mag | (w[i] & 0x80008000u);
+      v[2 * i] = __uint_as_float(w[i] << 16);
+      v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    }
+    top = max(top & 0xffffu, top >> 16);
+    top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    bool sure;
+    uint32_t s8 = block_scale(bf16_bits_to_f32(top), inv_v, sure);
+    if (!sure)
+      s8 = e4m3_of_f64(fmin(static_cast<double>(bf16_bits_to_f32(top)) / (6.0 * static_cast<double>(v_scale)), 448.0));
+    const float s = e4m3_to_f32(s8), inv = __fdividef(inv_v, s);   // good to 2^-21 or better, the nudge is 2^-20
+    uint32_t packed = e2m1_of_8(v, inv * (1.0f + 9.5367431640625e-7f));
+    uint32_t unsure = packed ^ e2m1_of_8(v, inv * (1.0f - 9.5367431640625e-7f));
+    if (s8 == 0) { packed = 0; unsure = 0; }                // a block below half the smallest scale
+    if (unsure) {
+      const double c = static_cast<double>(s) * static_cast<double>(v_scale);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        if ((unsure >> (4 * i)) & 15u) {
+          // packed has the upper code; 4 x the border below it: 1 3 5 7 10 14 20
+          const uint32_t up = (packed >> (4 * i)) & 7u;
+          const uint32_t border4 = static_cast<uint32_t>(0x140e0a0705030100ull >> (8 * up)) & 255u;
+          const double d = fma(-0.25 * border4, c, static_cast<double>(fabsf(v[i])));
+          if (d < 0.0 || (d == 0.0 && (up & 1u))) packed -= 1u << (4 * i);   // a tie goes to the even code
         }
       }
-      const int64_t row = p.cache_loc[t];
-      if (row < 0) continue;                                // a padding token
-      if (row >= p.cache_rows) { report_error(p.status, MSL_ERR_CAPACITY); continue; }
-      const int64_t at = row * p.hkv + (is_v ? h - p.hq - p.hkv : h - p.hq);
-      *reinterpret_cast<uint32_t*>((is_v ? p.v : p.k) + at * (D / 2) + sub * 4) = packed;
-      if ((sub & 1) == 0) (is_v ? p.vs : p.ks)[at * (D / 16) + sub / 2] = static_cast<uint8_t>(s8);
+    }
+    const int64_t row = p.cache_loc[t0 + now];
+    if (row >= p.cache_rows) report_error(p.status, MSL_ERR_CAPACITY);
+    if (in && row >= 0 && row < p.cache_rows) {
+      const int64_t to = row * kv_lanes + at;
+      *reinterpret_cast<uint32_t*>(p.v + to * 4) = packed;
+      if ((lane & 1) == 0) p.vs[to >> 1] = static_cast<uint8_t>(s8);
     }
   }
 }
@@ -447,13 +530,21 @@ extern "C" int msl_qk_rope_store_kv4(const void* qkv, int64_t ld, const int64_t*
   if (ld < static_cast<int64_t>(hq + 2 * hkv) * head_dim) return MSL_ERR_ARG;
   if (misaligned(qkv, 16) || misaligned(q, 16) || (ld & 7) || misaligned(k_cache, 16) || misaligned(v_cache, 16))
     return MSL_ERR_ALIGN;
+  // four tokens a block once that still fills the GPU, one before: their heads are then spread over more SMs
+  const int per_block = tokens >= 4 * kStoreTok * sm_count() ? kStoreTok : 1;
   const StoreArgs a{static_cast<const __nv_bfloat16*>(qkv), ld, positions, cache_loc, inv_freq, k_scale, v_scale,
                     static_cast<__nv_bfloat16*>(q), static_cast<uint8_t*>(k_cache), static_cast<uint8_t*>(k_sf),
-                    static_cast<uint8_t*>(v_cache), static_cast<uint8_t*>(v_sf), tokens, hq, hkv, cache_rows, status};
-  const int grid = (tokens + kStoreTok - 1) / kStoreTok;
+                    static_cast<uint8_t*>(v_cache), static_cast<uint8_t*>(v_sf), tokens, hq, hkv, per_block, cache_rows,
+                    status};
+  const int grid = (tokens + per_block - 1) / per_block;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (head_dim == 128) qk_rope_store_kv4_kernel<128><<<grid, kStoreThreads, 0, st>>>(a);
-  else qk_rope_store_kv4_kernel<64><<<grid, kStoreThreads, 0, st>>>(a);
+  if (head_dim == 128) {
+    if (inv_freq) qk_rope_store_kv4_kernel<128, true><<<grid, kStoreThreads, 0, st>>>(a);
+    else qk_rope_store_kv4_kernel<128, false><<<grid, kStoreThreads, 0, st>>>(a);
+  } else {
+    if (inv_freq) qk_rope_store_kv4_kernel<64, true><<<grid, kStoreThreads, 0, st>>>(a);
+    else qk_rope_store_kv4_kernel<64, false><<<grid, kStoreThreads, 0, st>>>(a);
+  }
   return cudaGetLastError() == cudaSuccess ? MSL_OK : MSL_ERR_CUDA;
 }
 
