@@ -128,8 +128,7 @@ __global__ void __launch_bounds__(kPlanThreads) page_plan_kernel(PlanArgs p) {
 }
 
 // ============================================================================ store
-// Lanes own 8 consecutive channels of a head, D / 8 lanes a head; two neighbouring lanes share a block of 16.  Queries
-// are rounded to bf16 once, so fp32 serves them.  Keys and values end on a coarse grid, where an error of one fp32 ulp
+// A lane owns a block of 16 consecutive channels, D / 16 lanes a head.  Queries are rounded to bf16 once, so fp32 serves them.  Keys and values end on a coarse grid, where an error of one fp32 ulp
 // next to a border moves a value by a whole step.  So fp32 only proposes: scale and codes are formed from the value
 // nudged up and down by more than the fp32 error (below), and where the two disagree 64 bits decide: a value against
 // border * (s * scale), 3 + 4 + 24 bits and exact, so that ties are seen as ties; a key (its norm and rotation are not
@@ -161,9 +160,8 @@ __device__ __forceinline__ float e4m3_to_f32(uint32_t b) {
   return __half2float(__half(__nv_cvt_fp8_to_halfraw(static_cast<__nv_fp8_storage_t>(b), __NV_E4M3)));
 }
 
-// Nearest E2M1 codes (saturating) of u[i] * f, its magnitude moved by `nudge`; element i in nibble i.  Without a nudge,
-// + 0 keeps a zero's code 0 whatever its sign.
-__device__ __forceinline__ uint32_t e2m1_pack(const float (&v)[8]) {
+// Nearest E2M1 codes (saturating) of eight values, element i in nibble i.
+__device__ __forceinline__ uint32_t e2m1_pack(const float* v) {
   uint32_t w;
   asm("{.reg .b8 a, b, c, d;\n\t"
       "cvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\n\tcvt.rn.satfinite.e2m1x2.f32 b, %4, %3;\n\t"
@@ -173,18 +171,39 @@ __device__ __forceinline__ uint32_t e2m1_pack(const float (&v)[8]) {
       : "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]));
   return w;
 }
-__device__ __forceinline__ uint32_t e2m1_of_8(const float (&u)[8], float f) {
-  float v[8];
+// Codes of u[i] * f; + 0 keeps a zero's code 0 whatever its sign.
+__device__ __forceinline__ uint2 e2m1_of_16(const float (&u)[16], float f) {
+  float v[16];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = fmaf(u[i], f, 0.0f);
-  return e2m1_pack(v);
+  for (int i = 0; i < 16; ++i) v[i] = fmaf(u[i], f, 0.0f);
+  return make_uint2(e2m1_pack(v), e2m1_pack(v + 8));
 }
-__device__ __forceinline__ uint32_t e2m1_of_8(const float (&u)[8], float f, float nudge) {
-  float v[8];
+// ... with the magnitude moved up or down by `nudge` (a zero keeps code 0 when it is moved up).
+template <bool UP>
+__device__ __forceinline__ uint2 e2m1_of_16(const float (&u)[16], float f, float nudge) {
+  float v[16];
 #pragma unroll
-  for (int i = 0; i < 8; ++i)   // copysign takes the magnitude alone: a downward nudge gets the other sign
-    v[i] = fmaf(u[i], f, nudge > 0.f ? copysignf(nudge, u[i]) : -copysignf(nudge, u[i]));
-  return e2m1_pack(v);
+  for (int i = 0; i < 16; ++i) v[i] = UP ? fmaf(u[i], f, copysignf(nudge, u[i])) : fmaf(u[i], f, -copysignf(nudge, u[i]));
+  return make_uint2(e2m1_pack(v), e2m1_pack(v + 8));
+}
+// 32 bytes at once where the rows allow it (`wide`: base and pitch multiples of 32), else as two halves.
+__device__ __forceinline__ void load_32(uint32_t (&w)[8], const void* src, bool wide) {
+  if (wide) {
+    asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7])
+                 : "l"(src));
+  } else {
+    const uint4 a = reinterpret_cast<const uint4*>(src)[0], b = reinterpret_cast<const uint4*>(src)[1];
+    w[0] = a.x; w[1] = a.y; w[2] = a.z; w[3] = a.w; w[4] = b.x; w[5] = b.y; w[6] = b.z; w[7] = b.w;
+  }
+}
+__device__ __forceinline__ void store_32(void* dst, const uint32_t (&w)[8], bool wide) {
+  if (wide) {
+    st_global_v8(dst, w);
+  } else {
+    reinterpret_cast<uint4*>(dst)[0] = make_uint4(w[0], w[1], w[2], w[3]);
+    reinterpret_cast<uint4*>(dst)[1] = make_uint4(w[4], w[5], w[6], w[7]);
+  }
 }
 
 // (cos, sin) of an angle of any size: quarter turns are taken off in 64 bits (pi / 2 as a sum of two doubles), what is
@@ -236,6 +255,7 @@ struct StoreArgs {
   uint8_t *k, *ks, *v, *vs;
   int tokens, hq, hkv;
   int per_block;                // tokens of a block
+  bool wide_in, wide_out;       // rows of qkv / q start on 32 bytes
   int64_t cache_rows;
   int* status;
 };
@@ -249,27 +269,26 @@ __device__ __forceinline__ uint32_t block_scale(float amax, float inv_scale, boo
   return __nv_cvt_float_to_fp8(want, __NV_SATFINITE, __NV_E4M3);
 }
 
-// A key head's 8 channels of this lane in 64 bits, start to end; the whole warp takes part (two or four heads).
+// A key head's 16 channels of this lane in 64 bits, start to end; the whole warp takes part.
 template <int D, bool ROPE>
-__device__ __noinline__ uint32_t key_codes_f64(const uint4 raw, double position, const float* inv_freq, double scale,
-                                               uint32_t& s8) {
-  constexpr int LPH = D / 8;
+__device__ __noinline__ uint2 key_codes_f64(const __nv_bfloat16* src, bool in, double position, const float* inv_freq,
+                                            double scale, uint32_t& s8) {
+  constexpr int LPH = D / 16;
   const int sub = threadIdx.x % LPH;
-  const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
-  double z[8], ss = 0.0, top = 0.0;
+  double z[16], ss = 0.0, top = 0.0;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    z[i] = bf16_bits_to_f64((w[i / 2] >> (16 * (i & 1))) & 0xffffu);
+  for (int i = 0; i < 16; ++i) {
+    z[i] = in ? bf16_bits_to_f64(reinterpret_cast<const uint16_t*>(src)[i]) : 0.0;
     ss = fma(z[i], z[i], ss);
   }
 #pragma unroll
   for (int o = LPH / 2; o > 0; o >>= 1) ss += shfl_xor_f64(0xffffffffu, ss, o);
   const double r = 1.0 / sqrt(ss / D + 1e-5);
 #pragma unroll
-  for (int i = 0; i < 8; i += 2) {
+  for (int i = 0; i < 16; i += 2) {
     double e = z[i] * r, o = z[i + 1] * r;
     if (ROPE) {
-      const double2 cs = cos_sin_f64(position * static_cast<double>(inv_freq[sub * 4 + i / 2]));
+      const double2 cs = cos_sin_f64(position * static_cast<double>(inv_freq[sub * 8 + i / 2]));
       const double e2 = e * cs.x - o * cs.y;
       o = e * cs.y + o * cs.x;
       e = e2;
@@ -278,19 +297,19 @@ __device__ __noinline__ uint32_t key_codes_f64(const uint4 raw, double position,
     z[i + 1] = o;
     top = fmax(top, fmax(fabs(e), fabs(o)));
   }
-  top = fmax(top, shfl_xor_f64(0xffffffffu, top, 1));
   s8 = e4m3_of_f64(fmin(top / (6.0 * scale), 448.0));
   const double c = static_cast<double>(e4m3_to_f32(s8)) * scale;
-  uint32_t packed = 0;
+  uint32_t packed[2] = {0, 0};
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
+  for (int i = 0; i < 16; ++i) {
     const double m = fabs(z[i]);
     uint32_t code = (m > 0.25 * c) + (m >= 0.75 * c) + (m > 1.25 * c) + (m >= 1.75 * c) + (m > 2.5 * c) +
                     (m >= 3.5 * c) + (m > 5.0 * c);
     if (z[i] < 0.0) code |= 8u;
-    packed |= code << (4 * i);
+    packed[i / 8] |= code << (4 * (i % 8));
   }
-  return s8 == 0 ? 0u : packed;                             // a block below half the smallest scale
+  // a block below half the smallest scale has zero codes
+  return s8 == 0 ? make_uint2(0, 0) : make_uint2(packed[0], packed[1]);
 }
 
 // A block takes p.per_block tokens with all their heads: their rotations first (a thread an angle), then the lanes of
@@ -298,15 +317,15 @@ __device__ __noinline__ uint32_t key_codes_f64(const uint4 raw, double position,
 template <int D, bool ROPE>
 __global__ void __launch_bounds__(kStoreThreads, 4)
 qk_rope_store_kv4_kernel(StoreArgs p) {
-  constexpr int LPH = D / 8;
-  // (cos, sin) of position * inv_freq[4 lane + i] at [i][lane]: a warp's reads are contiguous
-  __shared__ float2 rot[kStoreTok][4][LPH];
+  constexpr int LPH = D / 16;
+  // (cos, sin) of position * inv_freq[8 lane + i] at [i][lane]: a warp's reads are contiguous
+  __shared__ float2 rot[kStoreTok][8][LPH];
   const int t0 = blockIdx.x * p.per_block, nt = min(p.per_block, p.tokens - t0);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, sub = threadIdx.x % LPH;
   const __nv_bfloat16* src = p.qkv + t0 * p.ld;
   const int q_lanes = p.hq * LPH, kv_lanes = p.hkv * LPH;
   const int q_units = (q_lanes + 31) / 32, kv_units = (kv_lanes + 31) / 32, units = q_units + 2 * kv_units;
-  // unit u: its first lane, and the first lane and the end of its role among the token's lanes
+  // unit u: this lane's place in its role, the role's first lane among the token's lanes, its number of lanes
   const auto role_of = [&](int u, int& at, int& first, int& count) {
     const int kv = u - q_units;
     first = kv < 0 ? 0 : kv < kv_units ? q_lanes : q_lanes + kv_lanes;
@@ -314,40 +333,45 @@ qk_rope_store_kv4_kernel(StoreArgs p) {
     at = 32 * (kv < 0 ? u : kv < kv_units ? kv : kv - kv_units) + lane;
     return kv;
   };
-  const auto load = [&](int tt, int u) {                    // lanes past the role's end go through the motions
+  uint32_t next[8];
+  const auto fetch = [&](int tt, int u) {                   // lanes past the role's end go through the motions
     int at, first, count;
     role_of(u, at, first, count);
-    return at < count ? *reinterpret_cast<const uint4*>(src + tt * p.ld + (first + at) * 8) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) next[i] = 0;
+    if (at < count) load_32(next, src + tt * p.ld + (first + at) * 16, p.wide_in);
   };
   int u = warp, tt = 0;
   const auto settle = [&]() {                               // on to the token that unit u falls into
     while (u >= units) { u -= units; ++tt; }
   };
   settle();
-  uint4 next = tt < nt ? load(tt, u) : make_uint4(0, 0, 0, 0);
+  if (tt < nt) fetch(tt, u);
   if (ROPE) {
     for (int x = threadIdx.x; x < nt * (D / 2); x += kStoreThreads) {
       const int t = x / (D / 2), j = x % (D / 2);
-      rot[t][j % 4][j / 4] = cos_sin_f32(static_cast<double>(p.positions[t0 + t]) * static_cast<double>(p.inv_freq[j]));
+      rot[t][j % 8][j / 8] = cos_sin_f32(static_cast<double>(p.positions[t0 + t]) * static_cast<double>(p.inv_freq[j]));
     }
     __syncthreads();
   }
   const float k_scale = *p.k_scale, v_scale = *p.v_scale, inv_k = 1.0f / k_scale, inv_v = 1.0f / v_scale;
   while (tt < nt) {
     const int now = tt, unit = u;
-    const uint4 raw = next;
+    uint32_t w[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) w[i] = next[i];
     u += kStoreWarps;
     settle();
-    if (tt < nt) next = load(tt, u);
+    if (tt < nt) fetch(tt, u);
     int at, first, count;
     const int kv = role_of(unit, at, first, count);
     const bool in = at < count;
-    uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+    float v[16];
     if (kv < kv_units) {
       // ---- a query or a key: norm and rotation
-      float v[8], ss = 0.f;
+      float ss = 0.f;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
+      for (int i = 0; i < 16; ++i) {
         v[i] = __uint_as_float(i & 1 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16);
         ss = fmaf(v[i], v[i], ss);
       }
@@ -355,7 +379,7 @@ qk_rope_store_kv4_kernel(StoreArgs p) {
       for (int o = LPH / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
       const float r = rsqrtf(ss * (1.0f / D) + 1e-5f);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
+      for (int i = 0; i < 8; ++i) {
         float e = v[2 * i] * r, o = v[2 * i + 1] * r;
         if (ROPE) {
           const float2 cs = rot[now][i][sub];
@@ -367,65 +391,69 @@ qk_rope_store_kv4_kernel(StoreArgs p) {
         v[2 * i + 1] = o;
       }
       if (kv < 0) {
-        if (in)
-          *reinterpret_cast<uint4*>(p.q + static_cast<int64_t>(t0 + now) * p.hq * D + at * 8) =
-              make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]),
-                         pack_bf16x2(v[6], v[7]));
+#pragma unroll
+        for (int i = 0; i < 8; ++i) w[i] = pack_bf16x2(v[2 * i], v[2 * i + 1]);
+        if (in) store_32(p.q + static_cast<int64_t>(t0 + now) * p.hq * D + at * 16, w, p.wide_out);
         continue;
       }
-      // fp32 errors, in half steps of 2^-24: 10 in r, 1 in e, 3 in cosine and sine, 2 in the rotation, so 16 (|e| + |o|)
-      // <= 32 largest magnitudes of the block: 2^-19 of it, 1.3e-5 of a code's unit; the nudge is 3e-5
+      // fp32 errors, in half steps of 2^-24: 14 in r (16 products and 3 sums of shuffles, halved by the root; the root
+      // 4), 1 in e, 3 in cosine and sine, 2 in the rotation, so 20 (|e| + |o|) <= 40 largest magnitudes of the block:
+      // 2^-18.6 of it, 1.6e-5 of a code's unit; the nudge is 3e-5
       float amax = 0.f;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) amax = fmaxf(amax, fabsf(v[i]));
-      amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+      for (int i = 0; i < 16; ++i) amax = fmaxf(amax, fabsf(v[i]));
       bool sure;
       uint32_t s8 = block_scale(amax, inv_k, sure);
       const float inv = __fdividef(inv_k, e4m3_to_f32(s8));
-      uint32_t packed = e2m1_of_8(v, inv, 3.0517578125e-5f);
-      sure &= packed == e2m1_of_8(v, inv, -3.0517578125e-5f) && ss < 1e38f;
+      uint2 packed = e2m1_of_16<true>(v, inv, 3.0517578125e-5f);
+      const uint2 below = e2m1_of_16<false>(v, inv, 3.0517578125e-5f);
+      sure &= packed.x == below.x && packed.y == below.y && ss < 1e38f;
       if (__any_sync(0xffffffffu, in && !sure))
-        packed = key_codes_f64<D, ROPE>(raw, static_cast<double>(p.positions[t0 + now]), p.inv_freq, k_scale, s8);
+        packed = key_codes_f64<D, ROPE>(src + now * p.ld + (first + at) * 16, in,
+                                        static_cast<double>(p.positions[t0 + now]), p.inv_freq, k_scale, s8);
       const int64_t row = p.cache_loc[t0 + now];
       if (row >= p.cache_rows) report_error(p.status, MSL_ERR_CAPACITY);
       if (in && row >= 0 && row < p.cache_rows) {           // negative: a padding token
-        const int64_t to = row * kv_lanes + at;             // 4 bytes of codes and half a scale a lane
-        *reinterpret_cast<uint32_t*>(p.k + to * 4) = packed;
-        if ((lane & 1) == 0) p.ks[to >> 1] = static_cast<uint8_t>(s8);
+        const int64_t to = row * kv_lanes + at;             // 8 bytes of codes and a scale a lane
+        *reinterpret_cast<uint2*>(p.k + to * 8) = packed;
+        p.ks[to] = static_cast<uint8_t>(s8);
       }
       continue;
     }
     // ---- a value: exact in fp32; infinities and NaN, which have no code, count as the largest finite magnitude
     uint32_t top = 0;
-    float v[8];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < 8; ++i) {
       const uint32_t mag = __vminu2(w[i] & 0x7fff7fffu, 0x7f7f7f7fu);
       top = __vmaxu2(top, mag);
       w[i] = mag | (w[i] & 0x80008000u);
       v[2 * i] = __uint_as_float(w[i] << 16);
       v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
     }
-    top = max(top & 0xffffu, top >> 16);
-    top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    const float amax = bf16_bits_to_f32(max(top & 0xffffu, top >> 16));
     bool sure;
-    uint32_t s8 = block_scale(bf16_bits_to_f32(top), inv_v, sure);
-    if (!sure)
-      s8 = e4m3_of_f64(fmin(static_cast<double>(bf16_bits_to_f32(top)) / (6.0 * static_cast<double>(v_scale)), 448.0));
+    uint32_t s8 = block_scale(amax, inv_v, sure);
+    if (!sure) s8 = e4m3_of_f64(fmin(static_cast<double>(amax) / (6.0 * static_cast<double>(v_scale)), 448.0));
     const float s = e4m3_to_f32(s8), inv = __fdividef(inv_v, s);   // good to 2^-21 or better, the nudge is 2^-20
-    uint32_t packed = e2m1_of_8(v, inv * (1.0f + 9.5367431640625e-7f));
-    uint32_t unsure = packed ^ e2m1_of_8(v, inv * (1.0f - 9.5367431640625e-7f));
-    if (s8 == 0) { packed = 0; unsure = 0; }                // a block below half the smallest scale
-    if (unsure) {
+    uint2 packed = e2m1_of_16(v, inv * (1.0f + 9.5367431640625e-7f));
+    const uint2 below = e2m1_of_16(v, inv * (1.0f - 9.5367431640625e-7f));
+    if (s8 == 0) {                                          // a block below half the smallest scale
+      packed = make_uint2(0, 0);
+    } else if (packed.x != below.x || packed.y != below.y) {
       const double c = static_cast<double>(s) * static_cast<double>(v_scale);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        if ((unsure >> (4 * i)) & 15u) {
-          // packed has the upper code; 4 x the border below it: 1 3 5 7 10 14 20
-          const uint32_t up = (packed >> (4 * i)) & 7u;
-          const uint32_t border4 = static_cast<uint32_t>(0x140e0a0705030100ull >> (8 * up)) & 255u;
-          const double d = fma(-0.25 * border4, c, static_cast<double>(fabsf(v[i])));
-          if (d < 0.0 || (d == 0.0 && (up & 1u))) packed -= 1u << (4 * i);   // a tie goes to the even code
+      for (int half = 0; half < 2; ++half) {
+        uint32_t& mine = half ? packed.y : packed.x;
+        const uint32_t unsure = mine ^ (half ? below.y : below.x);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          if ((unsure >> (4 * i)) & 15u) {
+            // `mine` has the upper code; 4 x the border below it: 1 3 5 7 10 14 20
+            const uint32_t up = (mine >> (4 * i)) & 7u;
+            const uint32_t border4 = static_cast<uint32_t>(0x140e0a0705030100ull >> (8 * up)) & 255u;
+            const double d = fma(-0.25 * border4, c, static_cast<double>(fabsf(v[8 * half + i])));
+            if (d < 0.0 || (d == 0.0 && (up & 1u))) mine -= 1u << (4 * i);   // a tie goes to the even code
+          }
         }
       }
     }
@@ -433,8 +461,8 @@ qk_rope_store_kv4_kernel(StoreArgs p) {
     if (row >= p.cache_rows) report_error(p.status, MSL_ERR_CAPACITY);
     if (in && row >= 0 && row < p.cache_rows) {
       const int64_t to = row * kv_lanes + at;
-      *reinterpret_cast<uint32_t*>(p.v + to * 4) = packed;
-      if ((lane & 1) == 0) p.vs[to >> 1] = static_cast<uint8_t>(s8);
+      *reinterpret_cast<uint2*>(p.v + to * 8) = packed;
+      p.vs[to] = static_cast<uint8_t>(s8);
     }
   }
 }
@@ -534,8 +562,8 @@ extern "C" int msl_qk_rope_store_kv4(const void* qkv, int64_t ld, const int64_t*
   const int per_block = tokens >= 4 * kStoreTok * sm_count() ? kStoreTok : 1;
   const StoreArgs a{static_cast<const __nv_bfloat16*>(qkv), ld, positions, cache_loc, inv_freq, k_scale, v_scale,
                     static_cast<__nv_bfloat16*>(q), static_cast<uint8_t*>(k_cache), static_cast<uint8_t*>(k_sf),
-                    static_cast<uint8_t*>(v_cache), static_cast<uint8_t*>(v_sf), tokens, hq, hkv, per_block, cache_rows,
-                    status};
+                    static_cast<uint8_t*>(v_cache), static_cast<uint8_t*>(v_sf), tokens, hq, hkv, per_block,
+                    !misaligned(qkv, 32) && (ld & 15) == 0, !misaligned(q, 32), cache_rows, status};
   const int grid = (tokens + per_block - 1) / per_block;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (head_dim == 128) {
