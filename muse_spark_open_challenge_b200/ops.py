@@ -343,6 +343,9 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
     (lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+
+
 def _device(index, tensors, names):
     """All of `tensors` (None: absent) must be on CUDA device `index`."""
     for i, t in enumerate(tensors):
@@ -403,9 +406,11 @@ def page_plan(new_lens, seq_lens, page_table, free_pages, free_head, page_size, 
     i32 [1]); entries behind the last new token get position 0 and cache_loc -1.  Too few free pages, too short a
     table row or more new tokens than `tokens` are reported in `status`; slots without a page are -1."""
     index = new_lens.get_device()
-    _device(index, (new_lens, seq_lens, page_table, free_pages, free_head, status),
-            "new_lens seq_lens page_table free_pages free_head status")
-    if index != torch.cuda.current_device():
+    if not (0 <= index == seq_lens.get_device() == page_table.get_device() == free_pages.get_device()
+            == free_head.get_device()) or (status is not None and status.get_device() != index):
+        _device(index, (new_lens, seq_lens, page_table, free_pages, free_head, status),
+                "new_lens seq_lens page_table free_pages free_head status")
+    if index != _current_device():
         with torch.cuda.device(index):
             return page_plan(new_lens, seq_lens, page_table, free_pages, free_head, page_size, tokens, status)
     batch, i32 = new_lens.numel(), torch.int32
@@ -415,11 +420,10 @@ def page_plan(new_lens, seq_lens, page_table, free_pages, free_head, page_size, 
     _is(new_lens, i32, (batch,), "new_lens"), _is(seq_lens, i32, (batch,), "seq_lens")
     _is(page_table, i32, (batch, max_pages), "page_table"), _is(free_pages, i32, (n_free,), "free_pages")
     _is(free_head, i32, (1,), "free_head"), _status(status)
-    dev = new_lens.device
-    cu = torch.empty(batch + 1, dtype=i32, device=dev)
-    head = torch.empty(1, dtype=i32, device=dev)
-    positions = torch.empty(tokens, dtype=torch.int64, device=dev)
-    cache_loc = torch.empty(tokens, dtype=torch.int64, device=dev)
+    cu = new_lens.new_empty(batch + 1)
+    head = new_lens.new_empty(1)
+    positions = new_lens.new_empty(tokens, dtype=torch.int64)
+    cache_loc = torch.empty_like(positions)
     check(_lib.lib().msl_page_plan(new_lens.data_ptr(), seq_lens.data_ptr(), page_table.data_ptr(), max_pages,
                                    free_pages.data_ptr(), n_free, free_head.data_ptr(), head.data_ptr(), batch,
                                    page_size, tokens, cu.data_ptr(), positions.data_ptr(), cache_loc.data_ptr(),
@@ -433,9 +437,13 @@ def qk_rope_store_kv4(qkv, positions, cache_loc, inv_freq, k_scale, v_scale, k_c
     (u8 [..., hkv, head_dim / 2]) and block scales (e4m3 [..., hkv, head_dim / 16]).  A negative cache_loc marks a padding
     token, which is not stored."""
     index = qkv.get_device()
-    _device(index, (qkv, positions, cache_loc, inv_freq, k_scale, v_scale, k_cache, k_sf, v_cache, v_sf, status),
-            "qkv positions cache_loc inv_freq k_scale v_scale k_cache k_sf v_cache v_sf status")
-    if index != torch.cuda.current_device():
+    if not (0 <= index == positions.get_device() == cache_loc.get_device() == k_scale.get_device() ==
+            v_scale.get_device() == k_cache.get_device() == k_sf.get_device() == v_cache.get_device() ==
+            v_sf.get_device()) or (inv_freq is not None and inv_freq.get_device() != index) or \
+            (status is not None and status.get_device() != index):
+        _device(index, (qkv, positions, cache_loc, inv_freq, k_scale, v_scale, k_cache, k_sf, v_cache, v_sf, status),
+                "qkv positions cache_loc inv_freq k_scale v_scale k_cache k_sf v_cache v_sf status")
+    if index != _current_device():
         with torch.cuda.device(index):
             return qk_rope_store_kv4(qkv, positions, cache_loc, inv_freq, k_scale, v_scale, k_cache, k_sf, v_cache, v_sf,
                                      hq, hkv, head_dim, status)
@@ -450,7 +458,7 @@ def qk_rope_store_kv4(qkv, positions, cache_loc, inv_freq, k_scale, v_scale, k_c
     rows = _kv4_cache(k_cache, k_sf, hkv, head_dim, "k_cache")
     if _kv4_cache(v_cache, v_sf, hkv, head_dim, "v_cache") != rows:
         raise MslError("the key and value caches have different numbers of rows")
-    q = torch.empty((t, hq, head_dim), dtype=torch.bfloat16, device=qkv.device)
+    q = qkv.new_empty((t, hq, head_dim))
     check(_lib.lib().msl_qk_rope_store_kv4(qkv.data_ptr(), ld, positions.data_ptr(), cache_loc.data_ptr(),
                                            _ptr(inv_freq), k_scale.data_ptr(), v_scale.data_ptr(), q.data_ptr(),
                                            k_cache.data_ptr(), k_sf.data_ptr(), v_cache.data_ptr(), v_sf.data_ptr(), t,
@@ -463,8 +471,10 @@ def kv4_rows(codes, scales, scale, rows, dtype=torch.bfloat16, status=None):
     """The values that cache rows `rows` (i64 [n]) of a 4-bit cache stand for: bf16 or fp32 [n, hkv, head_dim].
     A negative row gives zeros."""
     index = codes.get_device()
-    _device(index, (codes, scales, scale, rows, status), "codes scales scale rows status")
-    if index != torch.cuda.current_device():
+    if not (0 <= index == scales.get_device() == scale.get_device() == rows.get_device()) or \
+            (status is not None and status.get_device() != index):
+        _device(index, (codes, scales, scale, rows, status), "codes scales scale rows status")
+    if index != _current_device():
         with torch.cuda.device(index):
             return kv4_rows(codes, scales, scale, rows, dtype, status)
     if codes.dim() < 3 or (dtype is not torch.bfloat16 and dtype is not torch.float32):
@@ -472,7 +482,7 @@ def kv4_rows(codes, scales, scale, rows, dtype=torch.bfloat16, status=None):
     hkv, head_dim, n = codes.shape[-2], 2 * codes.shape[-1], rows.numel()
     have = _kv4_cache(codes, scales, hkv, head_dim, "kv4_rows")
     _is(rows, torch.int64, (n,), "rows"), _scalars(scale), _status(status)
-    out = torch.empty((n, hkv, head_dim), dtype=dtype, device=codes.device)
+    out = codes.new_empty((n, hkv, head_dim), dtype=dtype)
     check(_lib.lib().msl_kv4_rows(codes.data_ptr(), scales.data_ptr(), scale.data_ptr(), rows.data_ptr(), n,
                                   hkv * head_dim, have, OUT_F32 if dtype is torch.float32 else OUT_BF16, out.data_ptr(),
                                   _ptr(status), _raw_stream(index)), "msl_kv4_rows")
@@ -491,10 +501,13 @@ def attention_kv4(q, k_cache, k_sf, v_cache, v_sf, page_table, seq_lens, cu_seql
     contiguous), result bf16 [T, hq * head_dim].  Rows behind the last request are left as they are (undefined when
     `out` is not given); a row that sees no key is zero."""
     index = q.get_device()
-    _device(index, (q, k_cache, k_sf, v_cache, v_sf, page_table, seq_lens, cu_seqlens_q, k_scale, v_scale, gate, out,
-                    status),
-            "q k_cache k_sf v_cache v_sf page_table seq_lens cu_seqlens_q k_scale v_scale gate out status")
-    if index != torch.cuda.current_device():
+    if not (0 <= index == k_cache.get_device() == k_sf.get_device() == v_cache.get_device() == v_sf.get_device() ==
+            page_table.get_device() == seq_lens.get_device() == cu_seqlens_q.get_device() == k_scale.get_device() ==
+            v_scale.get_device()) or any(x is not None and x.get_device() != index for x in (gate, out, status)):
+        _device(index, (q, k_cache, k_sf, v_cache, v_sf, page_table, seq_lens, cu_seqlens_q, k_scale, v_scale, gate, out,
+                        status),
+                "q k_cache k_sf v_cache v_sf page_table seq_lens cu_seqlens_q k_scale v_scale gate out status")
+    if index != _current_device():
         with torch.cuda.device(index):
             return attention_kv4(q, k_cache, k_sf, v_cache, v_sf, page_table, seq_lens, cu_seqlens_q, k_scale, v_scale,
                                  softmax_scale, batch, max_q_len, hq, hkv, head_dim, page_size, window, gate, out, status)
@@ -513,11 +526,11 @@ def attention_kv4(q, k_cache, k_sf, v_cache, v_sf, page_table, seq_lens, cu_seql
     if _kv4_cache(v_cache, v_sf, hkv, head_dim, "v_cache") != rows:
         raise MslError("the key and value caches have different numbers of rows")
     if out is None:
-        out = torch.empty((t, cols), dtype=torch.bfloat16, device=q.device)
+        out = q.new_empty((t, cols))
     ld_out = _pitch(out, t, cols, "out")
     ld_gate = 0 if gate is None else _pitch(gate, t, cols, "gate")
     size = _attention_kv4_workspace(index, batch, max_q_len, t, hq, hkv, head_dim, max_pages, page_size, window)
-    work = torch.empty(size, dtype=torch.uint8, device=q.device) if size else None
+    work = k_cache.new_empty(size) if size else None            # bytes
     check(_lib.lib().msl_attention_kv4(q.data_ptr(), q.stride(0) if t > 1 else cols, k_cache.data_ptr(), k_sf.data_ptr(),
                                        v_cache.data_ptr(), v_sf.data_ptr(), page_table.data_ptr(), max_pages,
                                        seq_lens.data_ptr(), cu_seqlens_q.data_ptr(), k_scale.data_ptr(),
