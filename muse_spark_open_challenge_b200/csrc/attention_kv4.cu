@@ -19,8 +19,6 @@
 // from the accumulator's layout to the operand's by one 8 x 8 transpose in registers.  Queries (bf16) are scaled by
 // a power of two per row so that the largest magnitude lies in [2^14, 2^15) and held in f16: exact for every
 // element within 2^28 of the row's largest.  P is f16 (2^-12 relative), statistics and O are fp32.
-#include <climits>
-
 #include "kv4_common.cuh"
 
 namespace msl {
@@ -177,26 +175,6 @@ __device__ __forceinline__ void kv4_issue(const Kv4Source& src, uint8_t* stage, 
     cp_async_small<S::kSfBytes>(base + S::kVs + lane * S::kSfBytes, src.vs + from * src.sf_pitch, bytes);
   }
   if (lane == 0) *reinterpret_cast<uint32_t*>(stage + S::kHeld) = mask;
-}
-
-// A key's page table entry, loaded a step before its row is needed.
-struct Kv4Page {
-  int page, off;                            // page INT_MIN: the key is hidden from every row
-};
-__device__ __forceinline__ Kv4Page kv4_page(const Kv4Args& p, const int* table, int key, int lo, int hi) {
-  Kv4Page x{INT_MIN, 0};
-  if (key >= lo && key < hi) {
-    const int idx = p.page_shift >= 0 ? key >> p.page_shift : key / p.page_size;
-    x.off = key - idx * p.page_size;
-    x.page = idx < p.max_pages ? table[idx] : -1;
-  }
-  return x;
-}
-__device__ __forceinline__ int kv4_row_of(const Kv4Args& p, const Kv4Page& x) {
-  const int64_t row = static_cast<int64_t>(x.page) * p.page_size + x.off;
-  if (x.page >= 0 && row < p.cache_rows) return static_cast<int>(row);
-  if (x.page != INT_MIN) report_error(p.status, MSL_ERR_CAPACITY);
-  return -1;
 }
 
 // Shared-memory layout of a warp's O [R][D]: channel d of the lane group D/8 at pitch D/8 + 2, so that the float2
@@ -726,16 +704,16 @@ static int kv4_row_blocks(int64_t rows) { return rows <= 8 ? 1 : 2; }
 
 // Up to this many query rows per KV head the mma.sync kernel above streams the keys once per 16 rows; beyond it the
 // tcgen05 kernel takes them 256 at a time.
-constexpr int kKvFewRows = 64;
+constexpr int kKvFewRows = 16;
 
 struct Kv4Plan {
   bool few;
-  int splits;
+  int splits, alternate;
   int64_t bytes;
 };
 static Kv4Plan kv4_plan(int batch, int max_q_len, int tokens, int hq, int hkv, int head_dim, int max_pages, int page_size,
                         int window) {
-  Kv4Plan plan{true, 1, 0};
+  Kv4Plan plan{true, 1, 0, 0};
   const int64_t rows = static_cast<int64_t>(max_q_len) * (hq / hkv);
   plan.few = rows <= kKvFewRows;
   if (plan.few) {
@@ -744,7 +722,8 @@ static Kv4Plan kv4_plan(int batch, int max_q_len, int tokens, int hq, int hkv, i
                                  : (one ? kv4_few_workspace<64, 1>(hkv) : kv4_few_workspace<64, 2>(hkv));
   } else {
     plan.splits = msl_attention_split_plan(batch, max_q_len, hq, hkv, max_pages, page_size, window);
-    plan.bytes = kv4_tc_workspace(plan.splits, tokens, hq, head_dim);
+    plan.alternate = rows <= 128;
+    plan.bytes = kv4_tc_workspace(plan.splits * (plan.alternate ? 2 : 1), tokens, hq, head_dim);
   }
   return plan;
 }
@@ -797,7 +776,7 @@ extern "C" int msl_attention_kv4(const void* q, int64_t ld_q, const void* k_cach
                   page_table, max_pages, seq_lens, cu_seqlens_q, k_scale, v_scale, softmax_scale, batch, max_q_len,
                   tokens, hq, hkv, page_size, window, cache_rows, static_cast<__nv_bfloat16*>(out), ld_out,
                   static_cast<const __nv_bfloat16*>(gate), ld_gate, static_cast<float*>(workspace),
-                  0, 0, 0, plan.splits, page_shift, status};
+                  0, 0, 0, plan.splits, plan.alternate, page_shift, status};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (!plan.few) return launch_kv4_tc(a, head_dim, st);
   if (kv4_row_blocks(static_cast<int64_t>(max_q_len) * G) == 1)

@@ -12,7 +12,7 @@
 //                   ahead, become f16 (e2m1 conversion times the block scale: exact) and are stored as K-major (K) and
 //                   N-major (V) swizzled operand tiles of a ring
 //   warps 9-11      idle: they round the warpgroup up whose registers the others use
-// Registers are split 176 (softmax) / 56 / 104 (producers): 128 x (176 + 176 + 56 + 104) = 65536, the launch's total.
+// Registers are split 184 (softmax) / 56 / 88 (producers): 128 x (184 + 184 + 56 + 88) = 65536, the launch's total.
 // P is f16 (2^-12 relative) times 2^6, which with a lag of the running maximum of at most 2^8 stays below 2^15.
 // A key whose page is missing is hidden: producers leave one bit per key, and the mask pass takes it with the causal
 // limits.  Every wait is bounded.
@@ -34,8 +34,8 @@ struct TcSmem {
   static constexpr int kRing = 2 * kTile;
   static constexpr int kHeld = kRing + kStages * kTile;    // 8 x 4 words: the keys of a tile that have a page
   static constexpr int kBar = kHeld + 8 * 16;
-  // q_full, full[stages], empty[stages], s_full[2], p_lo[2], p_hi[2], pv_done[2]
-  static constexpr int kNumBars = 1 + 2 * kStages + 8;
+  // q_full[2], full[stages], empty[stages], s_full[2], p_lo[2], p_hi[2], pv_done[2]
+  static constexpr int kNumBars = 2 + 2 * kStages + 8;
   static constexpr int kTotal = kBar + kNumBars * 8 + 16;
 };
 
@@ -159,9 +159,63 @@ __device__ __forceinline__ void tc_store_row(const TcRow<D>& x, uint8_t* tile, i
   }
 }
 
+// A block of work: up to 2 TQ query tokens of one request and KV head, and a slice of their key tiles.  Every role of a
+// CTA walks the same list, block i, i + gridDim.x, ...; longest key ranges first (later query blocks see more keys).
+struct TcItem {
+  int b, kvh, split, q_begin, q_len, seq, kt_begin, key_lo, last_qpos, n_tiles;
+  int first_tok[2], rows_valid[2], max_qpos[2], n_sub[2];  // per sub-tile: rows, last position, number of key tiles
+};
+__device__ __forceinline__ bool tc_item(const Kv4Args& p, int i, TcItem& it) {
+  const int G = p.hq / p.hkv, TQ = kTM / G;
+  it.split = i % p.kv_splits;
+  i /= p.kv_splits;
+  it.kvh = i % p.hkv;
+  i /= p.hkv;
+  it.b = i % p.batch;
+  const int rank = i / p.batch;
+  it.q_begin = max(0, min(p.cu_seqlens_q[it.b], p.tokens));
+  it.q_len = min(max(0, min(p.cu_seqlens_q[it.b + 1], p.tokens) - it.q_begin), p.max_q_len);
+  const int qblk = (it.q_len + 2 * TQ - 1) / (2 * TQ) - 1 - rank;
+  if (qblk < 0) return false;
+  const int q0 = qblk * 2 * TQ;
+  it.seq = p.seq_lens[it.b];
+  const int64_t table_keys = static_cast<int64_t>(p.max_pages) * p.page_size;
+  it.key_lo = p.window ? max(0, it.seq + q0 - p.window + 1) : 0;
+  it.kt_begin = it.key_lo / kTN;
+#pragma unroll
+  for (int s = 0; s < 2; ++s) {
+    it.first_tok[s] = q0 + (p.alternate ? 0 : s * TQ);     // alternate: both sub-tiles hold the same rows
+    const int cnt = max(0, min(TQ, it.q_len - it.first_tok[s]));
+    it.rows_valid[s] = cnt * G;
+    it.max_qpos[s] = it.seq + it.first_tok[s] + cnt - 1;
+    const int last_key = static_cast<int>(min(static_cast<int64_t>(it.max_qpos[s]), table_keys - 1));
+    // one tile at least: a row that sees nothing is still written
+    it.n_sub[s] = cnt > 0 ? max(1, last_key / kTN + 1 - it.kt_begin) : 0;
+  }
+  it.last_qpos = max(it.rows_valid[0] ? it.max_qpos[0] : -1, it.rows_valid[1] ? it.max_qpos[1] : -1);
+  it.n_tiles = max(it.n_sub[0], it.n_sub[1]);
+  if (p.kv_splits > 1) {                                    // a slice may be empty for one or both sub-tiles
+    const int chunk = (it.n_tiles + p.kv_splits - 1) / p.kv_splits;
+    const int lo = it.split * chunk, hi = min(it.n_tiles, lo + chunk);
+#pragma unroll
+    for (int s = 0; s < 2; ++s) it.n_sub[s] = max(0, min(it.n_sub[s], hi) - lo);
+    it.kt_begin += lo;
+    it.n_tiles = max(it.n_sub[0], it.n_sub[1]);
+  }
+  if (p.alternate) {
+    it.n_sub[0] = (it.n_tiles + 1) / 2;
+    it.n_sub[1] = it.n_tiles / 2;
+  }
+  return true;
+}
+// Place of the tiles of an item with n tiles in the order in which the ring carries them: `lag` K tiles first, then V(j)
+// and K(j + lag) in turn.
+__device__ __forceinline__ int tc_place_k(int j, int lag) { return j < lag ? j : 2 * j - lag + 1; }
+__device__ __forceinline__ int tc_place_v(int j, int n, int lag) { return min(lag, n) + j + min(j, max(n - lag, 0)); }
+
 template <int D>
 __global__ void __launch_bounds__(kTcThreads, 1)
-attention_kv4_tc_kernel(Kv4Args p) {
+attention_kv4_tc_kernel(Kv4Args p, int n_items) {
   using S = TcSmem<D>;
   constexpr int kSt = S::kStages;
   constexpr int kSlab = kTN * 128;                         // 128 rows x 64 f16 channels
@@ -169,7 +223,7 @@ attention_kv4_tc_kernel(Kv4Args p) {
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + S::kBar);
   uint64_t* q_full = bars;
-  uint64_t* full = bars + 1;
+  uint64_t* full = bars + 2;
   uint64_t* empty = full + kSt;
   uint64_t* s_full = empty + kSt;
   uint64_t* p_lo = s_full + 2;
@@ -180,63 +234,11 @@ attention_kv4_tc_kernel(Kv4Args p) {
   uint32_t* held = reinterpret_cast<uint32_t*>(smem + S::kHeld);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int G = p.hq / p.hkv;
-  const int TQ = kTM / G;                                  // query tokens per sub-tile
-  const int b = blockIdx.z, kvh = blockIdx.y;
-  const int q_begin = max(0, min(p.cu_seqlens_q[b], p.tokens));
-  const int q_len = min(max(0, min(p.cu_seqlens_q[b + 1], p.tokens) - q_begin), p.max_q_len);
-  // Longest key ranges first: later query blocks attend to more keys.
-  const int n_qblk = (q_len + 2 * TQ - 1) / (2 * TQ);
-  const int split = static_cast<int>(blockIdx.x) % p.kv_splits;
-  const int qblk = n_qblk - 1 - static_cast<int>(blockIdx.x) / p.kv_splits;
-  if (qblk < 0) return;                                    // uniform for the CTA, before any barrier
-  const int q0 = qblk * 2 * TQ;
-  const int seq = p.seq_lens[b];
-  const int64_t table_keys = static_cast<int64_t>(p.max_pages) * p.page_size;
-  int kt_begin = p.window ? max(0, seq + q0 - p.window + 1) / kTN : 0;
-  const int key_lo = p.window ? max(0, seq + q0 - p.window + 1) : 0;
-  // per sub-tile: valid rows, last query position, number of key tiles (one at least: a row that sees nothing is
-  // still written)
-  int rows_valid[2], max_qpos[2], n_sub[2];
-#pragma unroll
-  for (int s = 0; s < 2; ++s) {
-    const int first = q0 + s * TQ;
-    const int cnt = max(0, min(TQ, q_len - first));
-    rows_valid[s] = cnt * G;
-    max_qpos[s] = seq + first + cnt - 1;
-    const int last_key = static_cast<int>(min(static_cast<int64_t>(max_qpos[s]), table_keys - 1));
-    n_sub[s] = cnt > 0 ? max(1, last_key / kTN + 1 - kt_begin) : 0;
-  }
-  const int last_qpos = max(rows_valid[0] ? max_qpos[0] : -1, rows_valid[1] ? max_qpos[1] : -1);
-  if (threadIdx.x == 0 && last_qpos >= table_keys) report_error(p.status, MSL_ERR_CAPACITY);
-  if (p.kv_splits > 1) {
-    // this CTA's slice of the key tiles; a slice may be empty for one or both sub-tiles
-    const int n_full = max(n_sub[0], n_sub[1]);
-    const int chunk = (n_full + p.kv_splits - 1) / p.kv_splits;
-    const int lo = split * chunk, hi = min(n_full, lo + chunk);
-#pragma unroll
-    for (int s = 0; s < 2; ++s) n_sub[s] = max(0, min(n_sub[s], hi) - lo);
-    kt_begin += lo;
-  }
-  float* part_ml = p.part + static_cast<int64_t>(p.kv_splits) * p.tokens * p.hq * D;
-  const int n_tiles = max(n_sub[0], n_sub[1]);
-  if (n_tiles == 0) {                                      // an empty slice; uniform for the CTA, before any barrier
-    for (int i = threadIdx.x; i < 2 * kTM; i += blockDim.x) {
-      const int s = i / kTM, r = i % kTM;
-      if (r < rows_valid[s]) {
-        const int64_t idx = (static_cast<int64_t>(split) * p.tokens + q_begin + q0 + s * TQ + r / G) * p.hq +
-                            kvh * G + r % G;
-        part_ml[2 * idx] = -INFINITY;
-        part_ml[2 * idx + 1] = 0.f;
-      }
-    }
-    return;
-  }
-
+  const int lag = p.alternate ? 2 : 1;
   if (threadIdx.x == 0) {
-    mbar_init(q_full, 8);
     for (int i = 0; i < kSt; ++i) { mbar_init(&full[i], 4); mbar_init(&empty[i], 1); }
     for (int i = 0; i < 2; ++i) {
+      mbar_init(&q_full[i], 4);
       mbar_init(&s_full[i], 1);
       mbar_init(&p_lo[i], 4);
       mbar_init(&p_hi[i], 4);
@@ -253,37 +255,56 @@ attention_kv4_tc_kernel(Kv4Args p) {
 
   if (warp >= 12) {
     // ------------------------------------------------------------------ producers: thread = key of the tile
-    reg_dealloc<104>();
+    reg_dealloc<88>();
     const int r = (warp - 12) * 32 + lane;
-    const int* table = p.page_table + static_cast<int64_t>(b) * p.max_pages;
-    const int first_key = kt_begin * kTN + r;
-    int row = kv4_row(p, table, first_key, key_lo, last_qpos + 1);
-    int row_next = n_tiles > 1 ? kv4_row(p, table, first_key + kTN, key_lo, last_qpos + 1) : -1;
-    TcRow<D> k, v;
-    tc_load_row<D>(k, p.k, p.ks, row, p.hkv, kvh);
-    tc_load_row<D>(v, p.v, p.vs, row, p.hkv, kvh);
     bool ok = true;
-    for (int j = 0; j < n_tiles; ++j) {
-      const uint32_t mask = __ballot_sync(0xffffffffu, row >= 0);
-      int row_after = -1;
-      if (j + 2 < n_tiles) row_after = kv4_row(p, table, first_key + (j + 2) * kTN, key_lo, last_qpos + 1);
-      const int i0 = 2 * j, st0 = i0 % kSt;
-      if (*abort_flag || !mbar_wait(&empty[st0], ((i0 / kSt) & 1) ^ 1, true)) { ok = false; break; }
-      tc_store_row<D>(k, smem + S::kRing + st0 * S::kTile, r);
-      if (lane == 0) held[(j & 7) * 4 + warp - 12] = mask;
-      fence_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&full[st0]);
-      if (j + 1 < n_tiles) tc_load_row<D>(k, p.k, p.ks, row_next, p.hkv, kvh);
-      const int i1 = i0 + 1, st1 = i1 % kSt;
-      if (*abort_flag || !mbar_wait(&empty[st1], ((i1 / kSt) & 1) ^ 1, true)) { ok = false; break; }
-      tc_store_row<D>(v, smem + S::kRing + st1 * S::kTile, r);
-      fence_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&full[st1]);
-      if (j + 1 < n_tiles) tc_load_row<D>(v, p.v, p.vs, row_next, p.hkv, kvh);
-      row = row_next;
-      row_next = row_after;
+    int pos = 0, tiles = 0;                                 // ring places and tiles of the items before
+    for (int i = blockIdx.x; i < n_items && ok; i += gridDim.x) {
+      TcItem it;
+      if (!tc_item(p, i, it) || it.n_tiles == 0) continue;
+      const int n = it.n_tiles;
+      const int* table = p.page_table + static_cast<int64_t>(it.b) * p.max_pages;
+      const int first_key = it.kt_begin * kTN + r, hi = it.last_qpos + 1;
+      if (r == 0 && hi > static_cast<int64_t>(p.max_pages) * p.page_size) report_error(p.status, MSL_ERR_CAPACITY);
+      const auto page_of = [&](int j) {
+        return j < n ? kv4_page(p, table, first_key + j * kTN, it.key_lo, hi) : Kv4Page{INT_MIN, 0};
+      };
+      // this thread's key in tiles j .. j + 3: its cache rows, and the table entry of the next, on its way
+      Kv4Page ahead = page_of(0), ahead1 = page_of(1), ahead2 = page_of(2), ahead3 = page_of(3);
+      int row0 = kv4_row_of(p, ahead), row1 = kv4_row_of(p, ahead1), row2 = kv4_row_of(p, ahead2),
+          row3 = kv4_row_of(p, ahead3);
+      ahead = page_of(4);
+      TcRow<D> k, v;
+      tc_load_row<D>(k, p.k, p.ks, row0, p.hkv, it.kvh);
+      tc_load_row<D>(v, p.v, p.vs, row0, p.hkv, it.kvh);
+      const auto put = [&](const TcRow<D>& x, int place) {  // into the ring; false: the wait ran out
+        const int st = (pos + place) % kSt;
+        if (*abort_flag || !mbar_wait(&empty[st], (((pos + place) / kSt) & 1) ^ 1, true)) return false;
+        tc_store_row<D>(x, smem + S::kRing + st * S::kTile, r);
+        fence_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&full[st]);
+        return true;
+      };
+      const auto put_k = [&](int j, int row, int row_next) {
+        const uint32_t mask = __ballot_sync(0xffffffffu, row >= 0);
+        if (lane == 0) held[((tiles + j) & 7) * 4 + warp - 12] = mask;
+        if (!put(k, tc_place_k(j, lag))) return false;
+        if (j + 1 < n) tc_load_row<D>(k, p.k, p.ks, row_next, p.hkv, it.kvh);
+        return true;
+      };
+      ok = put_k(0, row0, row1);
+      if (ok && lag == 2 && n > 1) ok = put_k(1, row1, row2);
+      for (int j = 0; j < n && ok; ++j) {
+        const int row4 = kv4_row_of(p, ahead);
+        ahead = page_of(j + 5);
+        if (!put(v, tc_place_v(j, n, lag))) { ok = false; break; }
+        if (j + 1 < n) tc_load_row<D>(v, p.v, p.vs, row1, p.hkv, it.kvh);
+        if (j + lag < n) ok = put_k(j + lag, lag == 2 ? row2 : row1, lag == 2 ? row3 : row2);
+        row0 = row1; row1 = row2; row2 = row3; row3 = row4;
+      }
+      pos += 2 * n;
+      tiles += n;
     }
     if (!ok && lane == 0) { *abort_flag = 1; report_error(p.status, MSL_ERR_DEVICE_TIMEOUT); }
   } else if (warp >= 8) {
@@ -294,7 +315,7 @@ attention_kv4_tc_kernel(Kv4Args p) {
       constexpr uint32_t idesc_qk = make_idesc(0, 0, kTM, kTN);
       constexpr uint32_t idesc_pv = make_idesc(0, 0, kTM, D, 0, 1);     // A = P from TMEM (K-major), B = V, N-major
       const uint32_t sq = smem_u32(smem + S::kQ), ring = smem_u32(smem + S::kRing);
-      auto issue_qk = [&](int s, uint32_t sk) {
+      const auto issue_qk = [&](int s, uint32_t sk) {
 #pragma unroll
         for (int k = 0; k < D / 16; ++k) {                 // 32 bytes of a slab's 128-byte rows each
           const uint32_t off = (k / 4) * kSlab + (k % 4) * 32;
@@ -304,248 +325,323 @@ attention_kv4_tc_kernel(Kv4Args p) {
         tc_commit_if(on, &s_full[s]);
       };
       // keys [64 half, 64 half + 64) of the tile: P columns [32 half, +32) of the sub-tile's S, 8 per MMA
-      auto issue_pv_half = [&](int s, uint32_t sv, int half, bool first) {
+      const auto issue_pv_half = [&](int s, uint32_t sv, int half, bool first) {
 #pragma unroll
         for (int k = 4 * half; k < 4 * half + 4; ++k)
           tc_mma_f16_ts_if(on, tmem_base + 2 * kTN + s * kTN, tmem_base + s * kTN + k * 8,
                            make_sdesc(sv + k * 16 * 128, kSlab, 1024, 2), idesc_pv, !(first && k == 0));
       };
-      bool ok = mbar_wait(q_full, 0) && mbar_wait(&full[0], 0);
-      if (ok) {
-        tc_fence_after();
-        if (n_sub[0] > 0) issue_qk(0, ring);
-        if (n_sub[1] > 0) issue_qk(1, ring);
-        tc_commit_if(on, &empty[0]);
-      }
-      for (int j = 0; j < n_tiles && ok; ++j) {
-        const uint32_t ph = j & 1;
-        const int iv = 2 * j + 1, sv_st = iv % kSt, ik = 2 * j + 2, sk_st = ik % kSt;
-        const uint32_t sv = ring + sv_st * S::kTile, sk = ring + sk_st * S::kTile;
-        bool v_ready = false, k_ready = false;
+      bool ok = true;
+      int pos = 0, taken0 = 0, taken1 = 0;                  // ring places of, and items with tiles for, the sub-tiles before
+      int done0 = 0, done1 = 0;                             // their tiles
+      for (int i = blockIdx.x; i < n_items && ok; i += gridDim.x) {
+        TcItem it;
+        if (!tc_item(p, i, it) || it.n_tiles == 0) continue;
+        const int n = it.n_tiles;
+        const auto wait_full = [&](int place) {
+          const bool got = !*abort_flag && mbar_wait(&full[place % kSt], (place / kSt) & 1);
+          tc_fence_after();
+          return got;
+        };
+        // a sub-tile's queries, where it has any tiles (the groups may be items apart where it has none)
+        if (it.n_sub[0] > 0) ok = !*abort_flag && mbar_wait(&q_full[0], taken0++ & 1);
+        if (it.n_sub[1] > 0) ok = ok && !*abort_flag && mbar_wait(&q_full[1], taken1++ & 1);
+        for (int j = 0; j < min(lag, n) && ok; ++j) {
+          const int place = pos + tc_place_k(j, lag);
+          ok = wait_full(place);
+          if (!ok) break;
+          const uint32_t sk = ring + (place % kSt) * S::kTile;
+          if (p.alternate) {
+            issue_qk(j, sk);
+          } else {
+            if (it.n_sub[0] > 0) issue_qk(0, sk);
+            if (it.n_sub[1] > 0) issue_qk(1, sk);
+          }
+          tc_commit_if(on, &empty[place % kSt]);
+        }
+        for (int j = 0; j < n && ok; ++j) {
+          const int pv = pos + tc_place_v(j, n, lag), pk = pos + tc_place_k(j + lag, lag);
+          const uint32_t sv = ring + (pv % kSt) * S::kTile, sk = ring + (pk % kSt) * S::kTile;
+          const int local = p.alternate ? j >> 1 : j;       // this tile's number among the sub-tile's own
+          bool v_ready = false, k_ready = false;
 #pragma unroll
-        for (int s = 0; s < 2; ++s) {
-          if (j < n_sub[s]) {
-            if (!v_ready) {
-              if (*abort_flag || !mbar_wait(&full[sv_st], (iv / kSt) & 1)) { ok = false; break; }
-              v_ready = true;
-            }
-            if (*abort_flag || !mbar_wait(&p_lo[s], ph)) { ok = false; break; }
-            tc_fence_after();
-            issue_pv_half(s, sv, 0, j == 0);
-            if (*abort_flag || !mbar_wait(&p_hi[s], ph)) { ok = false; break; }
-            tc_fence_after();
-            issue_pv_half(s, sv, 1, false);
-            if (j == n_sub[s] - 1) tc_commit_if(on, &pv_done[s]);
-            if (j + 1 < n_sub[s]) {
-              if (!k_ready) {
-                if (*abort_flag || !mbar_wait(&full[sk_st], (ik / kSt) & 1)) { ok = false; break; }
-                tc_fence_after();
-                k_ready = true;
+          for (int s = 0; s < 2; ++s) {
+            if (p.alternate ? (j & 1) == s : j < it.n_sub[s]) {
+              const uint32_t ph = ((s ? done1 : done0) + local) & 1;
+              if (!v_ready) {
+                if (!wait_full(pv)) { ok = false; break; }
+                v_ready = true;
               }
-              issue_qk(s, sk);
+              if (*abort_flag || !mbar_wait(&p_lo[s], ph)) { ok = false; break; }
+              tc_fence_after();
+              issue_pv_half(s, sv, 0, local == 0);
+              if (*abort_flag || !mbar_wait(&p_hi[s], ph)) { ok = false; break; }
+              tc_fence_after();
+              issue_pv_half(s, sv, 1, false);
+              if (local == it.n_sub[s] - 1) tc_commit_if(on, &pv_done[s]);
+              if (local + 1 < it.n_sub[s]) {
+                if (!k_ready) {
+                  if (!wait_full(pk)) { ok = false; break; }
+                  k_ready = true;
+                }
+                issue_qk(s, sk);
+              }
             }
           }
+          if (!ok) break;
+          tc_commit_if(on, &empty[pv % kSt]);
+          if (k_ready) tc_commit_if(on, &empty[pk % kSt]);
         }
-        if (!ok) break;
-        tc_commit_if(on, &empty[sv_st]);
-        if (k_ready) tc_commit_if(on, &empty[sk_st]);
+        pos += 2 * n;
+        done0 += it.n_sub[0];
+        done1 += it.n_sub[1];
       }
       if (!ok && lane == 0) { *abort_flag = 1; report_error(p.status, MSL_ERR_DEVICE_TIMEOUT); }
     }
   } else {
     // ------------------------------------------------------------------ softmax / correction / epilogue
-    reg_alloc<176>();
+    reg_alloc<184>();
+    const int G = p.hq / p.hkv;
     const int sub = warp >> 2;                             // query sub-tile of this group
     const int r = (warp & 3) * 32 + lane;                  // row = TMEM lane
-    const int n_mine = n_sub[sub];
     const int tq = r / G, g = r - tq * G;
-    const bool row_valid = r < rows_valid[sub];
-    const int first_tok = q0 + sub * TQ;
-    const int qpos = seq + min(first_tok + tq, max(q_len - 1, 0));
-    const int sub_min_qpos = seq + first_tok;
-    float scale_log2 = p.softmax_scale * (*p.k_scale) * 1.4426950408889634f;
-    {
-      // this thread's query row, f16 with the largest magnitude in [2^14, 2^15)
-      const uint4* src = reinterpret_cast<const uint4*>(
-          p.q + (static_cast<int64_t>(q_begin) + first_tok + tq) * p.ld_q + (kvh * G + g) * D);
-      uint8_t* dst = smem + S::kQ + sub * S::kTile;
-      uint32_t w[D / 2];
-#pragma unroll
-      for (int i = 0; i < D / 8; ++i) {
-        uint4 x = make_uint4(0, 0, 0, 0);
-        if (row_valid) x = src[i];
-        w[4 * i] = x.x; w[4 * i + 1] = x.y; w[4 * i + 2] = x.z; w[4 * i + 3] = x.w;
-      }
-      uint32_t mx = 0;
-#pragma unroll
-      for (int i = 0; i < D / 2; ++i) mx = max(mx, max(w[i] & 0x7fffu, (w[i] >> 16) & 0x7fffu));
-      const int e = min(max(static_cast<int>(mx >> 7), 16), 254);
-      const float up = __uint_as_float(static_cast<uint32_t>(127 + 141 - e) << 23);
-      scale_log2 = scale_log2 / up;
-#pragma unroll
-      for (int i = 0; i < D / 8; ++i) {
-        uint32_t h[4];
-#pragma unroll
-        for (int x = 0; x < 4; ++x)
-          h[x] = h2_bits(__floats2half2_rn(bf16_bits_to_f32(w[4 * i + x] & 0xffffu) * up,
-                                           bf16_bits_to_f32(w[4 * i + x] >> 16) * up));
-        *reinterpret_cast<uint4*>(dst + (i / 8) * kSlab + swz128(r, i % 8)) = make_uint4(h[0], h[1], h[2], h[3]);
-      }
-      fence_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(q_full);
-    }
+    const float scale0 = p.softmax_scale * (*p.k_scale) * 1.4426950408889634f;
     const uint32_t lane_sel = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t tmem_s = tmem_base + sub * kTN + lane_sel;
     const uint32_t tmem_o = tmem_base + 2 * kTN + sub * kTN + lane_sel;
-    float m_run = -INFINITY, l_run = 0.f;                  // l accumulates 2^kTcShift * sum of exponentials
-    bool ok = true;
-    for (int j = 0; j < n_mine && ok; ++j) {
-      const uint32_t ph = j & 1;
-      const int key0 = (kt_begin + j) * kTN;
-      if (*abort_flag || !mbar_wait(&s_full[sub], ph)) { ok = false; break; }
-      tc_fence_after();
-      const uint4 hm = *reinterpret_cast<const uint4*>(held + (j & 7) * 4);
-      const bool full_tile = (key0 + kTN - 1 <= sub_min_qpos) && (!p.window || key0 > max_qpos[sub] - p.window) &&
-                             (hm.x & hm.y & hm.z & hm.w) == 0xffffffffu;
-      const int lim_hi = qpos - key0;                       // visible columns: lim_lo < col <= lim_hi
-      const int lim_lo = p.window ? qpos - p.window - key0 : -1;
-      uint32_t sa[32], sb[32], sc[32], sd[32];
-      tmem_ld32(tmem_s, sa);
-      tmem_ld32(tmem_s + 32, sb);
-      tmem_ld32(tmem_s + 64, sc);
-      tmem_ld32(tmem_s + 96, sd);
-      tmem_ld_wait();
-      if (!full_tile) {
-        tc_mask(sa, 0, lim_hi, lim_lo, hm.x);
-        tc_mask(sb, 32, lim_hi, lim_lo, hm.y);
-        tc_mask(sc, 64, lim_hi, lim_lo, hm.z);
-        tc_mask(sd, 96, lim_hi, lim_lo, hm.w);
-      }
-      const float m_cand = tc_row_max(sc, sd, tc_row_max(sa, sb, -INFINITY)) * scale_log2;
-      // A row's reference maximum moves when the row exceeds it by more than tau, or finds its first visible key.  Each
-      // row decides for itself, so that its bits do not depend on its neighbours; the warp rescales together.
-      const bool move = m_cand > m_run + kTcTau || (m_run == -INFINITY && m_cand > -INFINITY);
-      float corr = 1.0f;
-      if (__any_sync(0xffffffffu, move)) {
-        if (move) {
-          corr = kv_ex2(m_run - m_cand);                    // 0 when m_run = -inf
-          m_run = m_cand;
+    const int slots = p.kv_splits * (p.alternate ? 2 : 1);  // partial results per row; one: the row is written at once
+    float* part_ml = p.part + static_cast<int64_t>(slots) * p.tokens * p.hq * D;
+    // What the main loop needs of an item; the rest is formed again for the results.
+    struct Mine {
+      int n_tiles, n, kt_begin, qpos, min_qpos, max_qpos;
+      float scale_log2;
+    };
+    // The next item with tiles from i on; where this sub-tile has some, its query rows go to shared memory (every
+    // Q K^T of the sub-tile before has finished: its last S has been waited for).  Empty slices are dealt with here.
+    const auto take = [&](int& i, Mine& m) {
+      for (; i < n_items; i += gridDim.x) {
+        TcItem it;
+        if (!tc_item(p, i, it)) continue;
+        const int first_tok = sub ? it.first_tok[1] : it.first_tok[0];
+        const bool valid = r < (sub ? it.rows_valid[1] : it.rows_valid[0]);
+        const int64_t token = static_cast<int64_t>(it.q_begin) + first_tok + tq;
+        if (it.n_tiles == 0) {
+          if (valid) {
+            const int slot = p.alternate ? 2 * it.split + sub : it.split;
+            const int64_t idx = (static_cast<int64_t>(slot) * p.tokens + token) * p.hq + it.kvh * G + g;
+            part_ml[2 * idx] = -INFINITY;
+            part_ml[2 * idx + 1] = 0.f;
+          }
+          continue;
         }
-        if (j > 0) {
-          // O moves to the new maximum before any of this tile's P is used.  S(j) was ready only after P V(j-1) had
-          // finished (the tensor pipe ran it first), so O is quiet.  Small pieces: the scores hold the registers.
-#pragma unroll 1
-          for (int c = 0; c < D; c += 16) {
-            uint32_t oa[16];
-            tmem_ld16(tmem_o + c, oa);
-            tmem_ld_wait();
+        m.n_tiles = it.n_tiles;
+        m.n = sub ? it.n_sub[1] : it.n_sub[0];
+        m.kt_begin = it.kt_begin;
+        m.qpos = it.seq + min(first_tok + tq, max(it.q_len - 1, 0));
+        m.min_qpos = it.seq + first_tok;
+        m.max_qpos = sub ? it.max_qpos[1] : it.max_qpos[0];
+        if (m.n == 0) return true;
+        // f16 with the largest magnitude in [2^14, 2^15)
+        const uint4* src = reinterpret_cast<const uint4*>(p.q + token * p.ld_q + (it.kvh * G + g) * D);
+        uint8_t* dst = smem + S::kQ + sub * S::kTile;
+        uint32_t w[D / 2];
 #pragma unroll
-            for (int i = 0; i < 16; ++i) oa[i] = __float_as_uint(__uint_as_float(oa[i]) * corr);
-            tmem_st16(tmem_o + c, oa);
+        for (int x = 0; x < D / 8; ++x) {
+          uint4 u = make_uint4(0, 0, 0, 0);
+          if (valid) u = src[x];
+          w[4 * x] = u.x; w[4 * x + 1] = u.y; w[4 * x + 2] = u.z; w[4 * x + 3] = u.w;
+        }
+        uint32_t mx = 0;
+#pragma unroll
+        for (int x = 0; x < D / 2; ++x) mx = max(mx, max(w[x] & 0x7fffu, (w[x] >> 16) & 0x7fffu));
+        const int e = min(max(static_cast<int>(mx >> 7), 16), 254);
+        const float up = __uint_as_float(static_cast<uint32_t>(127 + 141 - e) << 23);
+        m.scale_log2 = scale0 / up;
+#pragma unroll
+        for (int x = 0; x < D / 8; ++x) {
+          uint32_t h[4];
+#pragma unroll
+          for (int y = 0; y < 4; ++y)
+            h[y] = h2_bits(__floats2half2_rn(bf16_bits_to_f32(w[4 * x + y] & 0xffffu) * up,
+                                             bf16_bits_to_f32(w[4 * x + y] >> 16) * up));
+          *reinterpret_cast<uint4*>(dst + (x / 8) * kSlab + swz128(r, x % 8)) = make_uint4(h[0], h[1], h[2], h[3]);
+        }
+        fence_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&q_full[sub]);
+        return true;
+      }
+      return false;
+    };
+
+    bool ok = true;
+    int done = 0, tiles = 0, outs = 0;                      // of this sub-tile, of the CTA, results: items before
+    int i = blockIdx.x;
+    Mine next;
+    next.scale_log2 = 0.f;
+    bool more = take(i, next);
+    while (more && ok) {
+      const Mine m = next;
+      const int at = i;
+      const float scale_log2 = m.scale_log2;
+      float m_run = -INFINITY, l_run = 0.f;                // l accumulates 2^kTcShift * sum of exponentials
+      for (int j = 0; j < m.n && ok; ++j) {
+        const int tile = p.alternate ? 2 * j + sub : j;
+        const int key0 = (m.kt_begin + tile) * kTN;
+        if (*abort_flag || !mbar_wait(&s_full[sub], (done + j) & 1)) { ok = false; break; }
+        tc_fence_after();
+        const uint4 hm = *reinterpret_cast<const uint4*>(held + ((tiles + tile) & 7) * 4);
+        const bool full_tile = (key0 + kTN - 1 <= m.min_qpos) && (!p.window || key0 > m.max_qpos - p.window) &&
+                               (hm.x & hm.y & hm.z & hm.w) == 0xffffffffu;
+        const int lim_hi = m.qpos - key0;                   // visible columns: lim_lo < col <= lim_hi
+        const int lim_lo = p.window ? m.qpos - p.window - key0 : -1;
+        uint32_t sa[32], sb[32], sc[32], sd[32];
+        tmem_ld32(tmem_s, sa);
+        tmem_ld32(tmem_s + 32, sb);
+        tmem_ld32(tmem_s + 64, sc);
+        tmem_ld32(tmem_s + 96, sd);
+        tmem_ld_wait();
+        if (!full_tile) {
+          tc_mask(sa, 0, lim_hi, lim_lo, hm.x);
+          tc_mask(sb, 32, lim_hi, lim_lo, hm.y);
+          tc_mask(sc, 64, lim_hi, lim_lo, hm.z);
+          tc_mask(sd, 96, lim_hi, lim_lo, hm.w);
+        }
+        const float m_cand = tc_row_max(sc, sd, tc_row_max(sa, sb, -INFINITY)) * scale_log2;
+        // A row's reference maximum moves when the row exceeds it by more than tau, or finds its first visible key.
+        // Each row decides for itself, so that its bits do not depend on its neighbours; the warp rescales together.
+        const bool move = m_cand > m_run + kTcTau || (m_run == -INFINITY && m_cand > -INFINITY);
+        float corr = 1.0f;
+        if (__any_sync(0xffffffffu, move)) {
+          if (move) {
+            corr = kv_ex2(m_run - m_cand);                  // 0 when m_run = -inf
+            m_run = m_cand;
+          }
+          if (j > 0) {
+            // O moves to the new maximum before any of this tile's P is used.  S was ready only after the P V before
+            // had finished (the tensor pipe ran it first), so O is quiet.  Small pieces: the scores hold the registers.
+#pragma unroll 1
+            for (int c = 0; c < D; c += 16) {
+              uint32_t oa[16];
+              tmem_ld16(tmem_o + c, oa);
+              tmem_ld_wait();
+#pragma unroll
+              for (int x = 0; x < 16; ++x) oa[x] = __float_as_uint(__uint_as_float(oa[x]) * corr);
+              tmem_st16(tmem_o + c, oa);
+            }
           }
         }
-      }
-      const float m_use = (m_run == -INFINITY) ? 0.f : m_run;
-      const uint64_t scale2 = f32x2(scale_log2, scale_log2), neg_m2 = f32x2(kTcShift - m_use, kTcShift - m_use);
-      uint64_t sum[2] = {0, 0};                             // two pairs of +0
-      {
+        const float m_use = (m_run == -INFINITY) ? 0.f : m_run;
+        const uint64_t scale2 = f32x2(scale_log2, scale_log2), neg_m2 = f32x2(kTcShift - m_use, kTcShift - m_use);
+        uint64_t sum[2] = {0, 0};                           // two pairs of +0
+        {
+          uint32_t pk[32];
+          tc_exp32(sa, scale2, neg_m2, sum, pk);
+          tc_exp32(sb, scale2, neg_m2, sum, pk + 16);
+          tc_st32(tmem_s, pk);
+        }
         uint32_t pk[32];
-        tc_exp32(sa, scale2, neg_m2, sum, pk);
-        tc_exp32(sb, scale2, neg_m2, sum, pk + 16);
-        tc_st32(tmem_s, pk);
+        tc_exp32(sc, scale2, neg_m2, sum, pk);              // the first half's stores land meanwhile
+        tmem_st_wait();                                     // P's first half and a rescaled O
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_lo[sub]);
+        tc_exp32(sd, scale2, neg_m2, sum, pk + 16);
+        tc_st32(tmem_s + 32, pk);
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_hi[sub]);
+        const float2 total = unpack_f32x2(add_f32x2(sum[0], sum[1]));
+        l_run = l_run * corr + (total.x + total.y);
       }
-      uint32_t pk[32];
-      tc_exp32(sc, scale2, neg_m2, sum, pk);                // the first half's stores land meanwhile
-      tmem_st_wait();                                       // P's first half and a rescaled O
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&p_lo[sub]);
-      tc_exp32(sd, scale2, neg_m2, sum, pk + 16);
-      tc_st32(tmem_s + 32, pk);
-      tmem_st_wait();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&p_hi[sub]);
-      const float2 total = unpack_f32x2(add_f32x2(sum[0], sum[1]));
-      const float l_tile = total.x + total.y;
-      l_run = l_run * corr + l_tile;
-    }
-    // ---------------------------------------------------------------- epilogue
-    if (ok && n_mine > 0) {
-      if (*abort_flag || !mbar_wait(&pv_done[sub], 0)) ok = false;     // committed once, behind the last P V
-    }
-    if (p.kv_splits > 1) {
-      // partial result of this key slice: O as it stands in TMEM, with the maximum and sum it refers to
-      const bool have = ok && n_mine > 0;
-      if (have) tc_fence_after();
-      const int64_t idx = (static_cast<int64_t>(split) * p.tokens + q_begin + first_tok + tq) * p.hq + kvh * G + g;
-      if (row_valid) {
-        part_ml[2 * idx] = have ? m_run : -INFINITY;
-        part_ml[2 * idx + 1] = have ? l_run : 0.f;
+      if (!ok) break;
+      done += m.n;
+      tiles += m.n_tiles;
+      // The next item's queries before this one's results: its first Q K^T runs behind the last P V.
+      i += gridDim.x;
+      more = take(i, next);
+
+      // -------------------------------------------------------------- epilogue
+      TcItem it;
+      tc_item(p, at, it);
+      const int n_mine = m.n;
+      const bool row_valid = r < (sub ? it.rows_valid[1] : it.rows_valid[0]);
+      const int64_t token = static_cast<int64_t>(it.q_begin) + (sub ? it.first_tok[1] : it.first_tok[0]) + tq;
+      const int head = it.kvh * G + g;
+      if (n_mine > 0) {
+        if (*abort_flag || !mbar_wait(&pv_done[sub], outs & 1)) { ok = false; break; }   // behind the last P V
+        ++outs;
+        tc_fence_after();
       }
-      if (have) {
+      if (slots > 1) {
+        // partial result of this key slice: O as it stands in TMEM, with the maximum and sum it refers to
+        const int slot = p.alternate ? 2 * it.split + sub : it.split;
+        const int64_t idx = (static_cast<int64_t>(slot) * p.tokens + token) * p.hq + head;
+        if (row_valid) {
+          part_ml[2 * idx] = m_run;
+          part_ml[2 * idx + 1] = l_run;
+        }
+        if (n_mine > 0) {
+#pragma unroll 1
+          for (int c = 0; c < D; c += 32) {
+            uint32_t o[32];
+            tmem_ld32(tmem_o + c, o);
+            tmem_ld_wait();
+            if (row_valid) {
+              float4* dst = reinterpret_cast<float4*>(p.part + idx * D + c);
+#pragma unroll
+              for (int x = 0; x < 8; ++x)
+                dst[x] = make_float4(__uint_as_float(o[4 * x]), __uint_as_float(o[4 * x + 1]),
+                                     __uint_as_float(o[4 * x + 2]), __uint_as_float(o[4 * x + 3]));
+            }
+          }
+        }
+      } else if (n_mine > 0) {
+        // l carries the same power of two as P; a row that sees nothing is zero, a NaN sum (a NaN query) stays visible
+        const float c_out = l_run > 0.f ? (*p.v_scale) / l_run : (l_run != l_run ? l_run : 0.f);
+        float r_norm = 1.0f;
+        if (p.gate != nullptr) {
+          float ss = 0.f;
+#pragma unroll 1
+          for (int c = 0; c < D; c += 32) {
+            uint32_t o[32];
+            tmem_ld32(tmem_o + c, o);
+            tmem_ld_wait();
+#pragma unroll
+            for (int x = 0; x < 32; ++x) { const float y = __uint_as_float(o[x]) * c_out; ss += y * y; }
+          }
+          r_norm = 1.0f / sqrtf(ss / D + 1e-5f);
+        }
+        __nv_bfloat16* orow = p.out + token * p.ld_out + head * D;
+        const __nv_bfloat16* grow = p.gate ? p.gate + token * p.ld_gate + head * D : nullptr;
 #pragma unroll 1
         for (int c = 0; c < D; c += 32) {
           uint32_t o[32];
           tmem_ld32(tmem_o + c, o);
           tmem_ld_wait();
           if (row_valid) {
-            float4* dst = reinterpret_cast<float4*>(p.part + idx * D + c);
+            float v[32];
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-              dst[i] = make_float4(__uint_as_float(o[4 * i]), __uint_as_float(o[4 * i + 1]),
-                                   __uint_as_float(o[4 * i + 2]), __uint_as_float(o[4 * i + 3]));
-          }
-        }
-      }
-    } else if (ok && n_mine > 0) {
-      tc_fence_after();
-      // l carries the same power of two as P; a row that sees nothing is zero, a NaN sum (a NaN query) stays visible
-      const float c_out = l_run > 0.f ? (*p.v_scale) / l_run : (l_run != l_run ? l_run : 0.f);
-      float r_norm = 1.0f;
-      if (p.gate != nullptr) {
-        float ss = 0.f;
-#pragma unroll 1
-        for (int c = 0; c < D; c += 32) {
-          uint32_t o[32];
-          tmem_ld32(tmem_o + c, o);
-          tmem_ld_wait();
+            for (int x = 0; x < 32; ++x) v[x] = __uint_as_float(o[x]) * c_out * r_norm;
+            if (grow != nullptr) {
 #pragma unroll
-          for (int i = 0; i < 32; ++i) { const float x = __uint_as_float(o[i]) * c_out; ss += x * x; }
-        }
-        r_norm = 1.0f / sqrtf(ss / D + 1e-5f);
-      }
-      const int64_t token = static_cast<int64_t>(q_begin) + first_tok + tq;
-      const int head = kvh * G + g;
-      __nv_bfloat16* orow = p.out + token * p.ld_out + head * D;
-      const __nv_bfloat16* grow = p.gate ? p.gate + token * p.ld_gate + head * D : nullptr;
-#pragma unroll 1
-      for (int c = 0; c < D; c += 32) {
-        uint32_t o[32];
-        tmem_ld32(tmem_o + c, o);
-        tmem_ld_wait();
-        if (row_valid) {
-          float v[32];
+              for (int x = 0; x < 32; x += 8) {
+                const uint4 gq = *reinterpret_cast<const uint4*>(grow + c + x);
+                const uint32_t gw[4] = {gq.x, gq.y, gq.z, gq.w};
 #pragma unroll
-          for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(o[i]) * c_out * r_norm;
-          if (grow != nullptr) {
-#pragma unroll
-            for (int i = 0; i < 32; i += 8) {
-              const uint4 gq = *reinterpret_cast<const uint4*>(grow + c + i);
-              const uint32_t gw[4] = {gq.x, gq.y, gq.z, gq.w};
-#pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                v[i + 2 * e] *= 1.0f / (1.0f + __expf(-bf16_bits_to_f32(gw[e] & 0xffffu)));
-                v[i + 2 * e + 1] *= 1.0f / (1.0f + __expf(-bf16_bits_to_f32(gw[e] >> 16)));
+                for (int e = 0; e < 4; ++e) {
+                  v[x + 2 * e] *= 1.0f / (1.0f + __expf(-bf16_bits_to_f32(gw[e] & 0xffffu)));
+                  v[x + 2 * e + 1] *= 1.0f / (1.0f + __expf(-bf16_bits_to_f32(gw[e] >> 16)));
+                }
               }
             }
-          }
 #pragma unroll
-          for (int i = 0; i < 32; i += 8)
-            *reinterpret_cast<uint4*>(orow + c + i) =
-                make_uint4(pack_bf16x2(v[i], v[i + 1]), pack_bf16x2(v[i + 2], v[i + 3]),
-                           pack_bf16x2(v[i + 4], v[i + 5]), pack_bf16x2(v[i + 6], v[i + 7]));
+            for (int x = 0; x < 32; x += 8)
+              *reinterpret_cast<uint4*>(orow + c + x) =
+                  make_uint4(pack_bf16x2(v[x], v[x + 1]), pack_bf16x2(v[x + 2], v[x + 3]),
+                             pack_bf16x2(v[x + 4], v[x + 5]), pack_bf16x2(v[x + 6], v[x + 7]));
+          }
         }
       }
     }
@@ -574,14 +670,15 @@ kv4_tc_merge_kernel(Kv4Args p) {
   if (item >= static_cast<int64_t>(q_len) * p.hq) return;
   const int64_t token = q_begin + item / p.hq;
   const int head = static_cast<int>(item % p.hq);
-  const float* part_ml = p.part + static_cast<int64_t>(p.kv_splits) * p.tokens * p.hq * D;
+  const int slots = p.kv_splits * (p.alternate ? 2 : 1);
+  const float* part_ml = p.part + static_cast<int64_t>(slots) * p.tokens * p.hq * D;
   const int64_t stride = static_cast<int64_t>(p.tokens) * p.hq, base = token * p.hq + head;
   float mx = -INFINITY;
-  for (int s = 0; s < p.kv_splits; ++s) mx = fmaxf(mx, part_ml[2 * (s * stride + base)]);
+  for (int s = 0; s < slots; ++s) mx = fmaxf(mx, part_ml[2 * (s * stride + base)]);
   float acc[PER], sum = 0.f;
 #pragma unroll
   for (int i = 0; i < PER; ++i) acc[i] = 0.f;
-  for (int s = 0; s < p.kv_splits; ++s) {
+  for (int s = 0; s < slots; ++s) {
     const int64_t at = s * stride + base;
     const float l = part_ml[2 * at + 1];
     if (l == 0.f) continue;                                 // an empty slice wrote no O
@@ -600,11 +697,13 @@ static int launch_tc(const Kv4Args& a, cudaStream_t st) {
   static SmemConfig config;
   if (int rc = config.ensure(attention_kv4_tc_kernel<D>, smem)) return rc;
   const int tq2 = 2 * (kTM / (a.hq / a.hkv));
-  const dim3 grid(((a.max_q_len + tq2 - 1) / tq2) * a.kv_splits, a.hkv, a.batch);
-  attention_kv4_tc_kernel<D><<<grid, kTcThreads, smem, st>>>(a);
-  if (a.kv_splits > 1) {
-    const int64_t items = static_cast<int64_t>(a.max_q_len) * a.hq;
-    kv4_tc_merge_kernel<D><<<dim3(static_cast<unsigned>((items + 7) / 8), a.batch), 256, 0, st>>>(a);
+  const int64_t items = static_cast<int64_t>((a.max_q_len + tq2 - 1) / tq2) * a.kv_splits * a.hkv * a.batch;
+  if (items > 0x7fffffff) return MSL_ERR_UNSUPPORTED;
+  attention_kv4_tc_kernel<D><<<static_cast<int>(std::min<int64_t>(items, sm_count())), kTcThreads, smem, st>>>(
+      a, static_cast<int>(items));
+  if (a.kv_splits > 1 || a.alternate) {
+    const int64_t rows = static_cast<int64_t>(a.max_q_len) * a.hq;
+    kv4_tc_merge_kernel<D><<<dim3(static_cast<unsigned>((rows + 7) / 8), a.batch), 256, 0, st>>>(a);
   }
   return cudaGetLastError() == cudaSuccess ? MSL_OK : MSL_ERR_CUDA;
 }
@@ -613,8 +712,8 @@ int launch_kv4_tc(const Kv4Args& a, int head_dim, cudaStream_t st) {
   return head_dim == 128 ? launch_tc<128>(a, st) : launch_tc<64>(a, st);
 }
 
-int64_t kv4_tc_workspace(int kv_splits, int tokens, int hq, int head_dim) {
-  return kv_splits <= 1 ? 0 : static_cast<int64_t>(kv_splits) * tokens * hq * (head_dim + 2) * 4;
+int64_t kv4_tc_workspace(int slots, int tokens, int hq, int head_dim) {
+  return slots <= 1 ? 0 : static_cast<int64_t>(slots) * tokens * hq * (head_dim + 2) * 4;
 }
 
 }  // namespace msl

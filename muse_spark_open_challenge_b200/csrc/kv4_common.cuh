@@ -3,6 +3,8 @@
 #pragma once
 #include <cuda_fp16.h>
 
+#include <climits>
+
 #include "msl_common.cuh"
 #include "msl_host.h"
 
@@ -30,6 +32,7 @@ struct Kv4Args {
   int heads;                    //   KV heads a CTA takes at once,
   int tile_shift;               //   log2 of a tile's keys
   int kv_splits;                // many rows: slices of a query block's keys
+  int alternate;                //   one block of up to 128 rows: the two sub-tiles take its key tiles in turn
   int page_shift;               // log2 of the page size, -1: not a power of two
   int* status;
 };
@@ -61,17 +64,24 @@ __device__ __forceinline__ __half2 scales_h2(uint32_t two) {
 __device__ __forceinline__ void pdl_launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
-// The cache row of key `key` (-1: hidden from every row of the block, or no valid page).
-__device__ __forceinline__ int kv4_row(const Kv4Args& p, const int* table, int key, int lo, int hi) {
-  if (key < lo || key >= hi) return -1;
-  const int idx = p.page_shift >= 0 ? key >> p.page_shift : key / p.page_size;
-  const int page = idx < p.max_pages ? table[idx] : -1;
-  const int64_t row = static_cast<int64_t>(page) * p.page_size + (key - idx * p.page_size);
-  if (page < 0 || row >= p.cache_rows) {
-    report_error(p.status, MSL_ERR_CAPACITY);
-    return -1;
+// A key's page table entry, loaded a step before its row is needed.
+struct Kv4Page {
+  int page, off;                // page INT_MIN: the key is hidden from every row
+};
+__device__ __forceinline__ Kv4Page kv4_page(const Kv4Args& p, const int* table, int key, int lo, int hi) {
+  Kv4Page x{INT_MIN, 0};
+  if (key >= lo && key < hi) {
+    const int idx = p.page_shift >= 0 ? key >> p.page_shift : key / p.page_size;
+    x.off = key - idx * p.page_size;
+    x.page = idx < p.max_pages ? table[idx] : -1;
   }
-  return static_cast<int>(row);
+  return x;
+}
+__device__ __forceinline__ int kv4_row_of(const Kv4Args& p, const Kv4Page& x) {
+  const int64_t row = static_cast<int64_t>(x.page) * p.page_size + x.off;
+  if (x.page >= 0 && row < p.cache_rows) return static_cast<int>(row);
+  if (x.page != INT_MIN) report_error(p.status, MSL_ERR_CAPACITY);
+  return -1;
 }
 
 // Rows of a finished block: O / l, v_scale, optional per-head RMS norm * sigmoid(gate), bf16.  One warp per row,
@@ -99,6 +109,6 @@ __device__ __forceinline__ void kv4_write_row(const Kv4Args& p, float (&o)[D / 3
 
 // Many query rows per KV head (prefill, chunks): csrc/attention_kv4_tc.cu.
 int launch_kv4_tc(const Kv4Args& a, int head_dim, cudaStream_t st);
-int64_t kv4_tc_workspace(int kv_splits, int tokens, int hq, int head_dim);
+int64_t kv4_tc_workspace(int slots, int tokens, int hq, int head_dim);
 
 }  // namespace msl
