@@ -67,13 +67,15 @@ __device__ __forceinline__ float tc_row_max(const uint32_t (&s0)[32], const uint
   for (int i = 0; i < 32; ++i) acc[i & 3] = tc_max3(acc[i & 3], __uint_as_float(s0[i]), __uint_as_float(s1[i]));
   return fmaxf(fmaxf(acc[0], acc[1]), fmaxf(acc[2], acc[3]));
 }
-// Scores of keys that this row does not see become -inf: lim_lo < column <= lim_hi and a page are needed.
+// Scores of keys that this row does not see become -inf: of the 32 columns from col0 on, lim_lo < column <= lim_hi and a
+// cache row are needed.
 __device__ __forceinline__ void tc_mask(uint32_t (&s)[32], int col0, int lim_hi, int lim_lo, uint32_t held) {
+  const int hi = lim_hi - col0, lo = lim_lo - col0;         // columns in (lo, hi]
+  uint32_t seen = held & (hi >= 31 ? 0xffffffffu : hi < 0 ? 0u : (2u << hi) - 1u);
+  seen &= lo >= 31 ? 0u : lo < 0 ? 0xffffffffu : ~((2u << lo) - 1u);
 #pragma unroll
-  for (int i = 0; i < 32; ++i) {
-    const int col = col0 + i;
-    if (!(col <= lim_hi && col > lim_lo && ((held >> i) & 1u))) s[i] = 0xff800000u;
-  }
+  for (int i = 0; i < 32; ++i)
+    if (!(seen & (1u << i))) s[i] = 0xff800000u;
 }
 // Two fp32 values an instruction: the FMA pipe takes half the issue slots.
 __device__ __forceinline__ uint64_t f32x2(float a, float b) {
@@ -106,6 +108,37 @@ __device__ __forceinline__ void tc_exp32(const uint32_t (&s)[32], uint64_t scale
     sum[(i / 2) & 1] = add_f32x2(sum[(i / 2) & 1], f32x2(a, b));
     packed[i / 2] = h2_bits(__floats2half2_rn(a, b));
   }
+}
+
+// Four K = 16 steps of S += Q K^T: both operands advance 32 bytes within a 128-byte swizzled row (descriptors count 16
+// bytes).  One asm block, so that the issuing warp's loop stays small: it is fetched over and over between the softmax
+// warps' (the issue of each instruction by itself, unrolled over the sub-tiles: 711 against 665 us for 4 x 4096).
+__device__ __forceinline__ void tc_mma4_qk(uint32_t on, uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p, q, t;\n\t.reg .b64 a1, a2, a3, b1, b2, b3;\n\t"
+      "setp.ne.b32 q, %5, 0;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.eq.b32 t, 0, 0;\n\t"
+      "add.u64 a1, %1, 2;\n\tadd.u64 a2, %1, 4;\n\tadd.u64 a3, %1, 6;\n\t"
+      "add.u64 b1, %2, 2;\n\tadd.u64 b2, %2, 4;\n\tadd.u64 b3, %2, 6;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], a1, b1, %3, t;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], a2, b2, %3, t;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], a3, b3, %3, t;\n\t}"
+      ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc), "r"(on)
+      : "memory");
+}
+// Four K = 16 steps of O += P V: P advances 8 TMEM columns, V 16 rows of 128 bytes.
+__device__ __forceinline__ void tc_mma4_pv(uint32_t on, uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p, q, t;\n\t.reg .b64 b1, b2, b3;\n\t.reg .b32 a1, a2, a3;\n\t"
+      "setp.ne.b32 q, %5, 0;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.eq.b32 t, 0, 0;\n\t"
+      "add.u32 a1, %1, 8;\n\tadd.u32 a2, %1, 16;\n\tadd.u32 a3, %1, 24;\n\t"
+      "add.u64 b1, %2, 128;\n\tadd.u64 b2, %2, 256;\n\tadd.u64 b3, %2, 384;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [a1], b1, %3, t;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [a2], b2, %3, t;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [a3], b3, %3, t;\n\t}"
+      ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(acc), "r"(on)
+      : "memory");
 }
 
 // A key row's codes and scales as loaded.
@@ -316,20 +349,16 @@ attention_kv4_tc_kernel(Kv4Args p, int n_items) {
       constexpr uint32_t idesc_pv = make_idesc(0, 0, kTM, D, 0, 1);     // A = P from TMEM (K-major), B = V, N-major
       const uint32_t sq = smem_u32(smem + S::kQ), ring = smem_u32(smem + S::kRing);
       const auto issue_qk = [&](int s, uint32_t sk) {
+        const uint64_t a = make_sdesc(sq + s * S::kTile, 16, 1024, 2), b = make_sdesc(sk, 16, 1024, 2);
 #pragma unroll
-        for (int k = 0; k < D / 16; ++k) {                 // 32 bytes of a slab's 128-byte rows each
-          const uint32_t off = (k / 4) * kSlab + (k % 4) * 32;
-          tc_mma_f16_if(on, tmem_base + s * kTN, make_sdesc(sq + s * S::kTile + off, 16, 1024, 2),
-                        make_sdesc(sk + off, 16, 1024, 2), idesc_qk, k != 0);
-        }
+        for (int k = 0; k < D / 64; ++k)                   // a slab of 64 channels each
+          tc_mma4_qk(on, tmem_base + s * kTN, a + k * (kSlab >> 4), b + k * (kSlab >> 4), idesc_qk, k != 0);
         tc_commit_if(on, &s_full[s]);
       };
-      // keys [64 half, 64 half + 64) of the tile: P columns [32 half, +32) of the sub-tile's S, 8 per MMA
+      // keys [64 half, 64 half + 64) of the tile: P columns [32 half, +32) of the sub-tile's S
       const auto issue_pv_half = [&](int s, uint32_t sv, int half, bool first) {
-#pragma unroll
-        for (int k = 4 * half; k < 4 * half + 4; ++k)
-          tc_mma_f16_ts_if(on, tmem_base + 2 * kTN + s * kTN, tmem_base + s * kTN + k * 8,
-                           make_sdesc(sv + k * 16 * 128, kSlab, 1024, 2), idesc_pv, !(first && k == 0));
+        tc_mma4_pv(on, tmem_base + 2 * kTN + s * kTN, tmem_base + s * kTN + 32 * half,
+                   make_sdesc(sv + half * 64 * 128, kSlab, 1024, 2), idesc_pv, !(first && half == 0));
       };
       bool ok = true;
       int pos = 0, taken0 = 0, taken1 = 0;                  // ring places of, and items with tiles for, the sub-tiles before
@@ -351,12 +380,9 @@ attention_kv4_tc_kernel(Kv4Args p, int n_items) {
           ok = wait_full(place);
           if (!ok) break;
           const uint32_t sk = ring + (place % kSt) * S::kTile;
-          if (p.alternate) {
-            issue_qk(j, sk);
-          } else {
-            if (it.n_sub[0] > 0) issue_qk(0, sk);
-            if (it.n_sub[1] > 0) issue_qk(1, sk);
-          }
+#pragma unroll 1
+          for (int s = 0; s < 2; ++s)
+            if (p.alternate ? s == j : (s ? it.n_sub[1] : it.n_sub[0]) > 0) issue_qk(s, sk);
           tc_commit_if(on, &empty[place % kSt]);
         }
         for (int j = 0; j < n && ok; ++j) {
@@ -364,28 +390,28 @@ attention_kv4_tc_kernel(Kv4Args p, int n_items) {
           const uint32_t sv = ring + (pv % kSt) * S::kTile, sk = ring + (pk % kSt) * S::kTile;
           const int local = p.alternate ? j >> 1 : j;       // this tile's number among the sub-tile's own
           bool v_ready = false, k_ready = false;
-#pragma unroll
+#pragma unroll 1
           for (int s = 0; s < 2; ++s) {
-            if (p.alternate ? (j & 1) == s : j < it.n_sub[s]) {
-              const uint32_t ph = ((s ? done1 : done0) + local) & 1;
-              if (!v_ready) {
-                if (!wait_full(pv)) { ok = false; break; }
-                v_ready = true;
+            const int mine = s ? it.n_sub[1] : it.n_sub[0];
+            if (!(p.alternate ? (j & 1) == s : j < mine)) continue;
+            const uint32_t ph = ((s ? done1 : done0) + local) & 1;
+            if (!v_ready) {
+              if (!wait_full(pv)) { ok = false; break; }
+              v_ready = true;
+            }
+            if (*abort_flag || !mbar_wait(&p_lo[s], ph)) { ok = false; break; }
+            tc_fence_after();
+            issue_pv_half(s, sv, 0, local == 0);
+            if (*abort_flag || !mbar_wait(&p_hi[s], ph)) { ok = false; break; }
+            tc_fence_after();
+            issue_pv_half(s, sv, 1, false);
+            if (local == mine - 1) tc_commit_if(on, &pv_done[s]);
+            if (local + 1 < mine) {
+              if (!k_ready) {
+                if (!wait_full(pk)) { ok = false; break; }
+                k_ready = true;
               }
-              if (*abort_flag || !mbar_wait(&p_lo[s], ph)) { ok = false; break; }
-              tc_fence_after();
-              issue_pv_half(s, sv, 0, local == 0);
-              if (*abort_flag || !mbar_wait(&p_hi[s], ph)) { ok = false; break; }
-              tc_fence_after();
-              issue_pv_half(s, sv, 1, false);
-              if (local == it.n_sub[s] - 1) tc_commit_if(on, &pv_done[s]);
-              if (local + 1 < it.n_sub[s]) {
-                if (!k_ready) {
-                  if (!wait_full(pk)) { ok = false; break; }
-                  k_ready = true;
-                }
-                issue_qk(s, sk);
-              }
+              issue_qk(s, sk);
             }
           }
           if (!ok) break;
@@ -413,7 +439,7 @@ attention_kv4_tc_kernel(Kv4Args p, int n_items) {
     float* part_ml = p.part + static_cast<int64_t>(slots) * p.tokens * p.hq * D;
     // What the main loop needs of an item; the rest is formed again for the results.
     struct Mine {
-      int n_tiles, n, kt_begin, qpos, min_qpos, max_qpos;
+      int n_tiles, n, kt_begin, qpos, min_qpos, max_qpos, rows;
       float scale_log2;
     };
     // The next item with tiles from i on; where this sub-tile has some, its query rows go to shared memory (every
@@ -440,6 +466,7 @@ attention_kv4_tc_kernel(Kv4Args p, int n_items) {
         m.qpos = it.seq + min(first_tok + tq, max(it.q_len - 1, 0));
         m.min_qpos = it.seq + first_tok;
         m.max_qpos = sub ? it.max_qpos[1] : it.max_qpos[0];
+        m.rows = sub ? it.rows_valid[1] : it.rows_valid[0];
         if (m.n == 0) return true;
         // f16 with the largest magnitude in [2^14, 2^15)
         const uint4* src = reinterpret_cast<const uint4*>(p.q + token * p.ld_q + (it.kvh * G + g) * D);
@@ -484,11 +511,18 @@ attention_kv4_tc_kernel(Kv4Args p, int n_items) {
       const Mine m = next;
       const int at = i;
       const float scale_log2 = m.scale_log2;
+      const bool any_row = (warp & 3) * 32 < m.rows;
       float m_run = -INFINITY, l_run = 0.f;                // l accumulates 2^kTcShift * sum of exponentials
       for (int j = 0; j < m.n && ok; ++j) {
         const int tile = p.alternate ? 2 * j + sub : j;
         const int key0 = (m.kt_begin + tile) * kTN;
         if (*abort_flag || !mbar_wait(&s_full[sub], (done + j) & 1)) { ok = false; break; }
+        if (!any_row) {                                     // no row of this warp is valid: P may be anything
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) { mbar_arrive(&p_lo[sub]); mbar_arrive(&p_hi[sub]); }
+          continue;
+        }
         tc_fence_after();
         const uint4 hm = *reinterpret_cast<const uint4*>(held + ((tiles + tile) & 7) * 4);
         const bool full_tile = (key0 + kTN - 1 <= m.min_qpos) && (!p.window || key0 > m.max_qpos - p.window) &&

@@ -226,17 +226,6 @@ __device__ __forceinline__ void tc_mma_f8_ts_if(uint32_t on, uint32_t d_tmem, ui
       ::"r"(d_tmem), "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(on)
       : "memory");
 }
-// f16 / bf16 operands with A in tensor memory: two 16-bit elements per 32-bit column in K order (8 columns per K = 16
-// instruction).
-__device__ __forceinline__ void tc_mma_f16_ts_if(uint32_t on, uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc,
-                                                 uint32_t idesc, uint32_t accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
-      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
-      ::"r"(d_tmem), "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(on)
-      : "memory");
-}
-
 // 4 x 4 transpose of 32-byte units among the four lanes of a quad (lanes 4k .. 4k + 3).  Lane q gives the
 // four units u[8 j .. 8 j + 7] (j = 0..3) of ITS row and ends with unit q of the quad's four rows in
 // f[8 j .. 8 j + 7] (row j of the quad).  With a lane per row, four lanes can then write 128 contiguous bytes
