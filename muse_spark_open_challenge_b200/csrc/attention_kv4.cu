@@ -1,15 +1,15 @@
-// Causal varlen attention over the paged 4-bit K/V cache (format: csrc/kv4.cu), few query rows per KV head:
-// decode steps, verify blocks.
+// Causal varlen attention over the paged 4-bit K/V cache (format: csrc/kv4.cu), up to 16 query rows per KV head: decode
+// steps.  More rows: csrc/attention_kv4_tc.cu.
 //
-// A worker (one CTA of four warps) owns an equal share of all key tiles of the batch: the tiles of every
-// (request, block of R query rows, KV head) are laid end to end and cut into `workers` equal ranges, so ragged
-// lengths cost nothing.  A range that covers all tiles of a work item writes its rows; the others leave
-// (O, maximum, sum) in the workspace and kv4_merge_kernel joins them.  The ranges follow from the lengths, which
-// live on the device: both kernels form the same sums, no host knows them.
+// A worker (one CTA) owns an equal share of all key tiles of the batch: the tiles of every request and group of KV heads
+// are laid end to end and cut into equal ranges, so ragged lengths cost nothing.  A range that covers all tiles of a
+// work item writes its rows; the others leave (O, maximum, sum) in the workspace and kv4_merge_kernel joins them.
+// The ranges follow from the lengths, which live on the device: both kernels form the same sums, no host knows them.
 //
-// Each warp takes 32 of a tile's 128 keys straight from global memory into registers, in the layout of the
-// MMA operands.  The contraction index of Q K^T and the row index of O^T may be permuted freely, and the
-// permutation is chosen so that a lane's share is contiguous in memory:
+// A warp takes 32 keys of one KV head at a time, from a ring of cp.async stages in shared memory into registers, in
+// the layout of the MMA operands (mma.sync: the operands change hands in registers, and a decode step has far too few
+// rows for the 128 of a tcgen05 tile).  The contraction index of Q K^T and the row index of O^T may be permuted
+// freely, and the permutation is chosen so that a lane's share is contiguous in memory:
 //   S^T[key][q] = K Q^T   lane (g, t) holds channels [D/4 t, D/4 (t+1)) of keys g and g + 8: one 16-byte load
 //                         (8 at head_dim 64), whose elements lie in at most two scale blocks
 //   O^T[d][q]  += V^T P^T lane (g, t) holds channels [D/8 g, D/8 (g+1)) of keys 2t, 2t+1, 2t+8, 2t+9: one
@@ -18,7 +18,12 @@
 // Codes become f16 by the e2m1 conversion, times their block scale: exact (2 + 4 significant bits).  P^T moves
 // from the accumulator's layout to the operand's by one 8 x 8 transpose in registers.  Queries (bf16) are scaled by
 // a power of two per row so that the largest magnitude lies in [2^14, 2^15) and held in f16: exact for every
-// element within 2^28 of the row's largest.  P is f16 (2^-12 relative), statistics and O are fp32.
+// element within 2^28 of the row's largest.  P is f16 (half a step 2^-11), statistics and O are fp32.
+//
+// What bounds it: issue slots.  64 requests x 8192 keys, 8 heads x 128 (604 MB): 174 us = 3.5 TB/s of the measured 6.55
+// with DRAM traffic equal to the bytes needed; 720 warp instructions per 32 keys (640 of them converting and scaling
+// 8192 elements), 0.6 issued per cycle and scheduler, ALU half busy.  On the way: codes straight from global memory into
+// registers 330 us (one ragged batch), the ring 263 us, the heads of a cache row fetched together 171 us.
 #include "kv4_common.cuh"
 
 namespace msl {
@@ -37,33 +42,25 @@ __device__ __forceinline__ Kv4Req kv4_request(const Kv4Args& p, int b) {
   r.seq = p.seq_lens[b];
   return r;
 }
-// Key tiles [first, last) that rows [R i, R (i + 1)) of a request's len * G rows can see.
+// Key tiles [first, last) that a request's rows can see, 2^tile_shift keys a tile.
 struct Kv4Span {
   int first, last;
 };
-template <int R>
-__device__ __forceinline__ Kv4Span kv4_span(const Kv4Args& p, const Kv4Req& r, int G, int i, int tile_shift) {
-  const int last_tok = min(r.len - 1, (R * i + R - 1) / G);
-  const int low_tok = R * i / G;
+__device__ __forceinline__ Kv4Span kv4_span(const Kv4Args& p, const Kv4Req& r, int tile_shift) {
   // keys past the table's row have no page: they are not walked (the kernel reports them)
-  const int hi = static_cast<int>(min(static_cast<int64_t>(r.seq) + last_tok + 1,
+  const int hi = static_cast<int>(min(static_cast<int64_t>(r.seq) + r.len,
                                       static_cast<int64_t>(p.max_pages) * p.page_size));
-  const int lo = p.window ? max(0, r.seq + low_tok - p.window + 1) : 0;
+  const int lo = p.window ? max(0, r.seq - p.window + 1) : 0;
   Kv4Span s;
   s.first = lo >> tile_shift;
   s.last = max(s.first + 1, (hi + (1 << tile_shift) - 1) >> tile_shift);   // with nothing to see: zeros are written
   return s;
 }
-// Tiles of a request (all row blocks and KV heads) when a CTA takes `heads` KV heads at once, 2^tile_shift keys a tile.
-template <int R>
-__device__ __forceinline__ int64_t kv4_tiles(const Kv4Args& p, const Kv4Req& r, int G, int heads, int tile_shift) {
-  const int blocks = (r.len * G + R - 1) / R;
-  int64_t sum = 0;
-  for (int i = 0; i < blocks; ++i) {
-    const Kv4Span s = kv4_span<R>(p, r, G, i, tile_shift);
-    sum += s.last - s.first;
-  }
-  return sum * (p.hkv / heads);
+// Tiles of a request, all its KV heads, when a CTA takes `heads` of them at once.
+__device__ __forceinline__ int64_t kv4_tiles(const Kv4Args& p, const Kv4Req& r, int heads, int tile_shift) {
+  if (r.len <= 0) return 0;
+  const Kv4Span s = kv4_span(p, r, tile_shift);
+  return static_cast<int64_t>(s.last - s.first) * (p.hkv / heads);
 }
 // A CTA takes p.heads KV heads of 32 W / p.heads keys at once where every worker has at least kKvLong tiles (below), and
 // one head of 32 W keys otherwise: the heads of a cache row lie side by side, so taking them together fetches whole rows
@@ -220,8 +217,8 @@ attention_kv4_kernel(Kv4Args p) {
   int64_t mine_all = 0, mine = 0;                           // tiles with p.heads heads a CTA, and with one
   for (int b = b0; b < b1; ++b) {
     const Kv4Req r = kv4_request(p, b);
-    mine_all += kv4_tiles<R>(p, r, G, p.heads, p.tile_shift);
-    mine += kv4_tiles<R>(p, r, G, 1, kWide);
+    mine_all += kv4_tiles(p, r, p.heads, p.tile_shift);
+    mine += kv4_tiles(p, r, 1, kWide);
   }
   const bool together = block_sum_i64<W>(mine_all, scratch) >= static_cast<int64_t>(kKvLong) * p.workers;
   const int heads = together ? p.heads : 1, tile_shift = together ? p.tile_shift : kWide;
@@ -247,7 +244,7 @@ attention_kv4_kernel(Kv4Args p) {
     int64_t base = inc - mine;
     int b = b0;
     for (; b < b1 - 1; ++b) {
-      const int64_t n = kv4_tiles<R>(p, kv4_request(p, b), G, heads, tile_shift);
+      const int64_t n = kv4_tiles(p, kv4_request(p, b), heads, tile_shift);
       if (at < base + n) break;
       base += n;
     }
@@ -263,306 +260,303 @@ attention_kv4_kernel(Kv4Args p) {
 
   for (; at < end && b < p.batch; ++b) {
     const Kv4Req r = kv4_request(p, b);
-    const int blocks = (r.len * G + R - 1) / R;
+    if (r.len <= 0) continue;
     const int* table = p.page_table + static_cast<int64_t>(b) * p.max_pages;
-    for (int i = 0; i < blocks && at < end; ++i) {
-      const Kv4Span span = kv4_span<R>(p, r, G, i, tile_shift);
-      const int n_span = span.last - span.first;
-      if (skip >= static_cast<int64_t>(n_span) * groups) { skip -= static_cast<int64_t>(n_span) * groups; continue; }
-      for (int group = static_cast<int>(skip / n_span); group < groups && at < end; ++group) {
-        const int kvh = group * heads + my_head;
-        const int off = static_cast<int>(skip % n_span);
-        skip = 0;
-        const int n = static_cast<int>(min(end - at, static_cast<int64_t>(n_span - off)));
-        // ---- rows of the block: row = token * G + head in group
-        const int rows = min(R, r.len * G - i * R);
-        const int last_tok = (i * R + rows - 1) / G;
-        const int hi = r.seq + last_tok + 1;                // keys [lo, hi) are visible to some row
-        const int lo = p.window ? max(0, r.seq + i * R / G - p.window + 1) : 0;
-        if (tid == 0 && hi > static_cast<int64_t>(p.max_pages) * p.page_size) report_error(p.status, MSL_ERR_CAPACITY);
-        const int all_lo = p.window ? max(0, r.seq + last_tok - p.window + 1) : 0;   // keys [all_lo, all_hi) to all
-        const int all_hi = r.seq + i * R / G + 1;
-        uint32_t qf[NB][KS][2];
-        float qs[NB][2];                                    // log2 scale of columns 2t, 2t + 1
-        int qpos[NB][2];
+    const Kv4Span span = kv4_span(p, r, tile_shift);
+    const int n_span = span.last - span.first;
+    for (int group = static_cast<int>(skip / n_span); group < groups && at < end; ++group) {
+      const int kvh = group * heads + my_head;
+      const int off = static_cast<int>(skip % n_span);
+      skip = 0;
+      const int n = static_cast<int>(min(end - at, static_cast<int64_t>(n_span - off)));
+      // ---- rows of the block: row = token * G + head in group
+      const int rows = min(R, r.len * G);                 // (the launch takes care that R is enough)
+      const int last_tok = r.len - 1;
+      const int hi = r.seq + last_tok + 1;                // keys [lo, hi) are visible to some row
+      const int lo = p.window ? max(0, r.seq - p.window + 1) : 0;
+      if (tid == 0 && hi > static_cast<int64_t>(p.max_pages) * p.page_size) report_error(p.status, MSL_ERR_CAPACITY);
+      const int all_lo = p.window ? max(0, r.seq + last_tok - p.window + 1) : 0;   // keys [all_lo, all_hi) to all
+      const int all_hi = r.seq + 1;
+      uint32_t qf[NB][KS][2];
+      float qs[NB][2];                                    // log2 scale of columns 2t, 2t + 1
+      int qpos[NB][2];
 #pragma unroll
-        for (int nb = 0; nb < NB; ++nb) {
-          const int row = nb * 8 + g;
-          uint32_t raw[KS * 2];
+      for (int nb = 0; nb < NB; ++nb) {
+        const int row = nb * 8 + g;
+        uint32_t raw[KS * 2];
 #pragma unroll
-          for (int w = 0; w < KS * 2; ++w) raw[w] = 0;
-          if (row < rows) {
-            const int tok = (i * R + row) / G, head = kvh * G + (i * R + row) % G;
-            const uint4* src = reinterpret_cast<const uint4*>(p.q + (static_cast<int64_t>(r.begin) + tok) * p.ld_q +
-                                                              head * D + t * (D / 4));
+        for (int w = 0; w < KS * 2; ++w) raw[w] = 0;
+        if (row < rows) {
+          const int tok = row / G, head = kvh * G + row % G;
+          const uint4* src = reinterpret_cast<const uint4*>(p.q + (static_cast<int64_t>(r.begin) + tok) * p.ld_q +
+                                                            head * D + t * (D / 4));
 #pragma unroll
-            for (int w = 0; w < KS / 2; ++w) {
-              const uint4 x = src[w];
-              raw[4 * w] = x.x; raw[4 * w + 1] = x.y; raw[4 * w + 2] = x.z; raw[4 * w + 3] = x.w;
+          for (int w = 0; w < KS / 2; ++w) {
+            const uint4 x = src[w];
+            raw[4 * w] = x.x; raw[4 * w + 1] = x.y; raw[4 * w + 2] = x.z; raw[4 * w + 3] = x.w;
+          }
+        }
+        uint32_t mx = 0;                                  // largest magnitude as bits (NaN and infinity on top)
+#pragma unroll
+        for (int w = 0; w < KS * 2; ++w) mx = max(mx, max(raw[w] & 0x7fffu, (raw[w] >> 16) & 0x7fffu));
+        mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+        mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+        // 2^(141 - e) takes the exponent e to 141 = 127 + 14; its inverse goes into the row's score scale
+        const int e = min(max(static_cast<int>(mx >> 7), 16), 254);
+        const float up = __uint_as_float(static_cast<uint32_t>(127 + 141 - e) << 23);
+        const float down = scale_log2 / up;
+#pragma unroll
+        for (int w = 0; w < KS * 2; ++w)
+          qf[nb][w / 2][w & 1] = h2_bits(__floats2half2_rn(bf16_bits_to_f32(raw[w] & 0xffffu) * up,
+                                                           bf16_bits_to_f32(raw[w] >> 16) * up));
+        qs[nb][0] = __shfl_sync(0xffffffffu, down, 8 * t);         // lane (g = 2t, 0) holds row 2t
+        qs[nb][1] = __shfl_sync(0xffffffffu, down, 8 * t + 4);
+#pragma unroll
+        for (int c = 0; c < 2; ++c) qpos[nb][c] = r.seq + (nb * 8 + 2 * t + c) / G;
+      }
+      float o[NB][KS][4], m[NB][2], l[NB][2];
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) {
+#pragma unroll
+        for (int c = 0; c < 2; ++c) { m[nb][c] = -INFINITY; l[nb][c] = 0.f; }
+#pragma unroll
+        for (int k = 0; k < KS; ++k)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) o[nb][k][c] = 0.f;
+      }
+      // ---- the keys, 32 a step
+      const int tile = 1 << tile_shift;
+      const int key_first = (span.first + off) * tile + (warp / heads) * 32;
+      const auto page_of = [&](int j) {
+        return j < n ? kv4_page(p, table, key_first + j * tile + lane, lo, hi) : Kv4Page{INT_MIN, 0};
+      };
+      const Kv4Source source = kv4_source<D>(p, kvh, lane);
+      Kv4Page ahead[S::kStages];
+#pragma unroll
+      for (int j = 0; j < S::kStages; ++j) ahead[j] = page_of(j);
+#pragma unroll
+      for (int j = 0; j < S::kStages - 1; ++j) {
+        if (j < n) kv4_issue<D>(source, ring + j * S::kStage, kv4_row_of(p, ahead[j]), lane);
+        cp_async_commit();
+      }
+      Kv4Page page_next = ahead[S::kStages - 1];          // of step j + kStages - 1
+      int slot = 0;
+      for (int j = 0; j < n; ++j) {
+        const int key0 = key_first + j * tile;
+        uint8_t* stage = ring + slot * S::kStage;
+        cp_async_wait<S::kStages - 2>();
+        __syncwarp();                                     // every lane's copies are in, and the last slot is free
+        if (j + S::kStages - 1 < n)
+          kv4_issue<D>(source, ring + (slot == 0 ? S::kStages - 1 : slot - 1) * S::kStage, kv4_row_of(p, page_next), lane);
+        cp_async_commit();
+        page_next = page_of(j + S::kStages);
+        slot = slot + 1 == S::kStages ? 0 : slot + 1;
+        const uint32_t held = *reinterpret_cast<const uint32_t*>(stage + S::kHeld);
+        const bool partial = held != 0xffffffffu || key0 < all_lo || key0 + 32 > all_hi;
+        float s[2][NB][4];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+#pragma unroll
+          for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) s[h][nb][c] = 0.f;
+          uint32_t k[2][D / 32];
+          __half2 sc[2];
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            const int row = 16 * h + 8 * x + g;
+            if constexpr (D == 128) {
+              const uint4 v = *reinterpret_cast<const uint4*>(stage + row * 64 + t * 16);
+              k[x][0] = v.x; k[x][1] = v.y; k[x][2] = v.z; k[x][3] = v.w;
+              sc[x] = scales_h2(*reinterpret_cast<const uint16_t*>(stage + S::kKs + row * 8 + t * 2));
+            } else {
+              const uint2 v = *reinterpret_cast<const uint2*>(stage + row * 32 + t * 8);
+              k[x][0] = v.x; k[x][1] = v.y;
+              sc[x] = scales_h2(stage[S::kKs + row * 4 + t]);
             }
           }
-          uint32_t mx = 0;                                  // largest magnitude as bits (NaN and infinity on top)
 #pragma unroll
-          for (int w = 0; w < KS * 2; ++w) mx = max(mx, max(raw[w] & 0x7fffu, (raw[w] >> 16) & 0x7fffu));
-          mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-          mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-          // 2^(141 - e) takes the exponent e to 141 = 127 + 14; its inverse goes into the row's score scale
-          const int e = min(max(static_cast<int>(mx >> 7), 16), 254);
-          const float up = __uint_as_float(static_cast<uint32_t>(127 + 141 - e) << 23);
-          const float down = scale_log2 / up;
+          for (int w = 0; w < D / 32; ++w) {              // one word = two MMA steps
+            __half2 a[4], c[4];
+            e2m1x8(k[0][w], a);
+            e2m1x8(k[1][w], c);
+            const bool second = D == 128 && w >= 2;       // which of the lane's two scale blocks
+            const __half2 s0 = second ? __high2half2(sc[0]) : __low2half2(sc[0]);
+            const __half2 s1 = second ? __high2half2(sc[1]) : __low2half2(sc[1]);
 #pragma unroll
-          for (int w = 0; w < KS * 2; ++w)
-            qf[nb][w / 2][w & 1] = h2_bits(__floats2half2_rn(bf16_bits_to_f32(raw[w] & 0xffffu) * up,
-                                                             bf16_bits_to_f32(raw[w] >> 16) * up));
-          qs[nb][0] = __shfl_sync(0xffffffffu, down, 8 * t);         // lane (g = 2t, 0) holds row 2t
-          qs[nb][1] = __shfl_sync(0xffffffffu, down, 8 * t + 4);
+            for (int x = 0; x < 4; ++x) { a[x] = __hmul2(a[x], s0); c[x] = __hmul2(c[x], s1); }
 #pragma unroll
-          for (int c = 0; c < 2; ++c) qpos[nb][c] = r.seq + (i * R + nb * 8 + 2 * t + c) / G;
+            for (int nb = 0; nb < NB; ++nb) {
+              mma_16816(s[h][nb], h2_bits(a[0]), h2_bits(c[0]), h2_bits(a[1]), h2_bits(c[1]), qf[nb][2 * w][0],
+                        qf[nb][2 * w][1]);
+              mma_16816(s[h][nb], h2_bits(a[2]), h2_bits(c[2]), h2_bits(a[3]), h2_bits(c[3]), qf[nb][2 * w + 1][0],
+                        qf[nb][2 * w + 1][1]);
+            }
+          }
         }
-        float o[NB][KS][4], m[NB][2], l[NB][2];
+        // ---- mask where some row does not see a key
+        if (partial) {
 #pragma unroll
-        for (int nb = 0; nb < NB; ++nb) {
-#pragma unroll
-          for (int c = 0; c < 2; ++c) { m[nb][c] = -INFINITY; l[nb][c] = 0.f; }
-#pragma unroll
-          for (int k = 0; k < KS; ++k)
-#pragma unroll
-            for (int c = 0; c < 4; ++c) o[nb][k][c] = 0.f;
-        }
-        // ---- the keys, 32 a step
-        const int tile = 1 << tile_shift;
-        const int key_first = (span.first + off) * tile + (warp / heads) * 32;
-        const auto page_of = [&](int j) {
-          return j < n ? kv4_page(p, table, key_first + j * tile + lane, lo, hi) : Kv4Page{INT_MIN, 0};
-        };
-        const Kv4Source source = kv4_source<D>(p, kvh, lane);
-        Kv4Page ahead[S::kStages];
-#pragma unroll
-        for (int j = 0; j < S::kStages; ++j) ahead[j] = page_of(j);
-#pragma unroll
-        for (int j = 0; j < S::kStages - 1; ++j) {
-          if (j < n) kv4_issue<D>(source, ring + j * S::kStage, kv4_row_of(p, ahead[j]), lane);
-          cp_async_commit();
-        }
-        Kv4Page page_next = ahead[S::kStages - 1];          // of step j + kStages - 1
-        int slot = 0;
-        for (int j = 0; j < n; ++j) {
-          const int key0 = key_first + j * tile;
-          uint8_t* stage = ring + slot * S::kStage;
-          cp_async_wait<S::kStages - 2>();
-          __syncwarp();                                     // every lane's copies are in, and the last slot is free
-          if (j + S::kStages - 1 < n)
-            kv4_issue<D>(source, ring + (slot == 0 ? S::kStages - 1 : slot - 1) * S::kStage, kv4_row_of(p, page_next), lane);
-          cp_async_commit();
-          page_next = page_of(j + S::kStages);
-          slot = slot + 1 == S::kStages ? 0 : slot + 1;
-          const uint32_t held = *reinterpret_cast<const uint32_t*>(stage + S::kHeld);
-          const bool partial = held != 0xffffffffu || key0 < all_lo || key0 + 32 > all_hi;
-          float s[2][NB][4];
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-#pragma unroll
-            for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-              for (int c = 0; c < 4; ++c) s[h][nb][c] = 0.f;
-            uint32_t k[2][D / 32];
-            __half2 sc[2];
+          for (int h = 0; h < 2; ++h)
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
-              const int row = 16 * h + 8 * x + g;
-              if constexpr (D == 128) {
-                const uint4 v = *reinterpret_cast<const uint4*>(stage + row * 64 + t * 16);
-                k[x][0] = v.x; k[x][1] = v.y; k[x][2] = v.z; k[x][3] = v.w;
-                sc[x] = scales_h2(*reinterpret_cast<const uint16_t*>(stage + S::kKs + row * 8 + t * 2));
-              } else {
-                const uint2 v = *reinterpret_cast<const uint2*>(stage + row * 32 + t * 8);
-                k[x][0] = v.x; k[x][1] = v.y;
-                sc[x] = scales_h2(stage[S::kKs + row * 4 + t]);
-              }
+              const int kk = 16 * h + g + 8 * x;
+#pragma unroll
+              for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                  const int key = key0 + kk;
+                  const bool seen = ((held >> kk) & 1u) && key <= qpos[nb][c] && (!p.window || key > qpos[nb][c] - p.window);
+                  if (!seen) s[h][nb][2 * x + c] = -INFINITY;
+                }
             }
+        }
+        // ---- running maximum: it moves when a row of the warp exceeds it by more than 2^tau
+        float top[NB][2];
+        bool move = false;
 #pragma unroll
-            for (int w = 0; w < D / 32; ++w) {              // one word = two MMA steps
-              __half2 a[4], c[4];
-              e2m1x8(k[0][w], a);
-              e2m1x8(k[1][w], c);
-              const bool second = D == 128 && w >= 2;       // which of the lane's two scale blocks
-              const __half2 s0 = second ? __high2half2(sc[0]) : __low2half2(sc[0]);
-              const __half2 s1 = second ? __high2half2(sc[1]) : __low2half2(sc[1]);
+        for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-              for (int x = 0; x < 4; ++x) { a[x] = __hmul2(a[x], s0); c[x] = __hmul2(c[x], s1); }
-#pragma unroll
-              for (int nb = 0; nb < NB; ++nb) {
-                mma_16816(s[h][nb], h2_bits(a[0]), h2_bits(c[0]), h2_bits(a[1]), h2_bits(c[1]), qf[nb][2 * w][0],
-                          qf[nb][2 * w][1]);
-                mma_16816(s[h][nb], h2_bits(a[2]), h2_bits(c[2]), h2_bits(a[3]), h2_bits(c[3]), qf[nb][2 * w + 1][0],
-                          qf[nb][2 * w + 1][1]);
-              }
-            }
+          for (int c = 0; c < 2; ++c) {
+            // in log2 units (the scale is positive)
+            const float x = fmaxf(fmaxf(s[0][nb][c], s[0][nb][2 + c]), fmaxf(s[1][nb][c], s[1][nb][2 + c])) * qs[nb][c];
+            top[nb][c] = x;
+            move |= x > m[nb][c] + kKvTau || (m[nb][c] == -INFINITY && x > -INFINITY);
           }
-          // ---- mask where some row does not see a key
-          if (partial) {
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
-#pragma unroll
-              for (int x = 0; x < 2; ++x) {
-                const int kk = 16 * h + g + 8 * x;
-#pragma unroll
-                for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-                  for (int c = 0; c < 2; ++c) {
-                    const int key = key0 + kk;
-                    const bool seen = ((held >> kk) & 1u) && key <= qpos[nb][c] && (!p.window || key > qpos[nb][c] - p.window);
-                    if (!seen) s[h][nb][2 * x + c] = -INFINITY;
-                  }
-              }
-          }
-          // ---- running maximum: it moves when a row of the warp exceeds it by more than 2^tau
-          float top[NB][2];
-          bool move = false;
+        if (__any_sync(0xffffffffu, move)) {
 #pragma unroll
           for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
-              // in log2 units (the scale is positive)
-              const float x = fmaxf(fmaxf(s[0][nb][c], s[0][nb][2 + c]), fmaxf(s[1][nb][c], s[1][nb][2 + c])) * qs[nb][c];
-              top[nb][c] = x;
-              move |= x > m[nb][c] + kKvTau || (m[nb][c] == -INFINITY && x > -INFINITY);
+              float x = top[nb][c];
+#pragma unroll
+              for (int d = 4; d < 32; d <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, d));
+              // each column (query row) decides for itself: its bits do not depend on its neighbours
+              const float new_m = (x > m[nb][c] + kKvTau || m[nb][c] == -INFINITY) ? x : m[nb][c];
+              const float corr = kv_ex2(m[nb][c] - (new_m == -INFINITY ? 0.f : new_m));
+              m[nb][c] = new_m;
+              l[nb][c] *= corr;
+#pragma unroll
+              for (int k = 0; k < KS; ++k) { o[nb][k][c] *= corr; o[nb][k][2 + c] *= corr; }
             }
-          if (__any_sync(0xffffffffu, move)) {
-#pragma unroll
-            for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-              for (int c = 0; c < 2; ++c) {
-                float x = top[nb][c];
-#pragma unroll
-                for (int d = 4; d < 32; d <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, d));
-                // each column (query row) decides for itself: its bits do not depend on its neighbours
-                const float new_m = (x > m[nb][c] + kKvTau || m[nb][c] == -INFINITY) ? x : m[nb][c];
-                const float corr = kv_ex2(m[nb][c] - (new_m == -INFINITY ? 0.f : new_m));
-                m[nb][c] = new_m;
-                l[nb][c] *= corr;
-#pragma unroll
-                for (int k = 0; k < KS; ++k) { o[nb][k][c] *= corr; o[nb][k][2 + c] *= corr; }
-              }
-          }
-          uint32_t pf[2][NB][2];
-#pragma unroll
-          for (int nb = 0; nb < NB; ++nb) {
-            const float n0 = m[nb][0] == -INFINITY ? 0.f : m[nb][0], n1 = m[nb][1] == -INFINITY ? 0.f : m[nb][1];
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
-#pragma unroll
-              for (int x = 0; x < 2; ++x) {
-                const float e0 = kv_ex2(fmaf(s[h][nb][2 * x], qs[nb][0], -n0));
-                const float e1 = kv_ex2(fmaf(s[h][nb][2 * x + 1], qs[nb][1], -n1));
-                l[nb][0] += e0;
-                l[nb][1] += e1;
-                pf[h][nb][x] = transpose8x8(h2_bits(__floats2half2_rn(e0, e1)));
-              }
-          }
-          // ---- O^T += V^T P^T
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            uint32_t v[4][D / 64];
-            uint32_t vs[4];
-#pragma unroll
-            for (int x = 0; x < 4; ++x) {
-              const int row = 16 * h + 2 * t + (x & 1) + 8 * (x >> 1);
-              const uint8_t* src = stage + S::kV + kv4_v_offset<D>(row, g * (D / 16));
-              if constexpr (D == 128) {
-                const uint2 u = *reinterpret_cast<const uint2*>(src);
-                v[x][0] = u.x; v[x][1] = u.y;
-                vs[x] = stage[S::kVs + row * 8 + g];
-              } else {
-                v[x][0] = *reinterpret_cast<const uint32_t*>(src);
-                vs[x] = stage[S::kVs + row * 4 + g / 2];
-              }
-            }
-            const __half2 s01 = scales_h2(vs[0] | (vs[1] << 8));
-            const __half2 s23 = scales_h2(vs[2] | (vs[3] << 8));
-#pragma unroll
-            for (int w = 0; w < D / 64; ++w) {              // one word a key = four 16-row tiles
-              // pairs along the keys: low nibbles (even channels, MMA rows g) and high ones (odd, g + 8)
-              const uint32_t lo01 = (v[0][w] & 0x0f0f0f0fu) | ((v[1][w] << 4) & 0xf0f0f0f0u);
-              const uint32_t hi01 = ((v[0][w] >> 4) & 0x0f0f0f0fu) | (v[1][w] & 0xf0f0f0f0u);
-              const uint32_t lo23 = (v[2][w] & 0x0f0f0f0fu) | ((v[3][w] << 4) & 0xf0f0f0f0u);
-              const uint32_t hi23 = ((v[2][w] >> 4) & 0x0f0f0f0fu) | (v[3][w] & 0xf0f0f0f0u);
-              __half2 a0[4], a1[4], a2[4], a3[4];
-              e2m1x8(lo01, a0);
-              e2m1x8(hi01, a1);
-              e2m1x8(lo23, a2);
-              e2m1x8(hi23, a3);
-#pragma unroll
-              for (int x = 0; x < 4; ++x) {
-                const uint32_t u0 = h2_bits(__hmul2(a0[x], s01)), u1 = h2_bits(__hmul2(a1[x], s01));
-                const uint32_t u2 = h2_bits(__hmul2(a2[x], s23)), u3 = h2_bits(__hmul2(a3[x], s23));
-#pragma unroll
-                for (int nb = 0; nb < NB; ++nb)
-                  mma_16816(o[nb][4 * w + x], u0, u1, u2, u3, pf[h][nb][0], pf[h][nb][1]);
-              }
-            }
-          }
         }
-        __syncwarp();                                       // the ring is read; O takes its place
-        // ---- join the warps of a head
+        uint32_t pf[2][NB][2];
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) {
+          const float n0 = m[nb][0] == -INFINITY ? 0.f : m[nb][0], n1 = m[nb][1] == -INFINITY ? 0.f : m[nb][1];
 #pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            float x = l[nb][c];
+          for (int h = 0; h < 2; ++h)
 #pragma unroll
-            for (int d = 4; d < 32; d <<= 1) x += __shfl_xor_sync(0xffffffffu, x, d);
-            const int row = nb * 8 + 2 * t + c;
-            if (g == 0) { sm_m[warp][row] = m[nb][c]; sm_l[warp][row] = x; }
-#pragma unroll
-            for (int k = 0; k < KS; ++k)
-              *reinterpret_cast<float2*>(sm_o(warp, row) + g * M::kGroup + 2 * k) =
-                  make_float2(o[nb][k][c], o[nb][k][2 + c]);
-          }
+            for (int x = 0; x < 2; ++x) {
+              const float e0 = kv_ex2(fmaf(s[h][nb][2 * x], qs[nb][0], -n0));
+              const float e1 = kv_ex2(fmaf(s[h][nb][2 * x + 1], qs[nb][1], -n1));
+              l[nb][0] += e0;
+              l[nb][1] += e1;
+              pf[h][nb][x] = transpose8x8(h2_bits(__floats2half2_rn(e0, e1)));
+            }
         }
-        __syncthreads();
-        const bool whole = n == n_span;
-        // a worker has at most two partial results: the rest of an item that an earlier worker began (slot 0) and
-        // the beginning of one that a later worker ends (slot 1)
-        float* part = p.part + (static_cast<int64_t>(blockIdx.x) * 2 + (off == 0 ? 1 : 0)) * p.heads * R * (D + 2);
-        for (int job = warp; job < heads * rows; job += W) {
-          const int h = job & (heads - 1), row = job / heads;
-          float mx = -INFINITY;
-          for (int x = 0; x < n_sub; ++x) mx = fmaxf(mx, sm_m[x * heads + h][row]);
-          float acc[D / 32], sum = 0.f;
+        // ---- O^T += V^T P^T
 #pragma unroll
-          for (int x = 0; x < D / 32; ++x) acc[x] = 0.f;
-          for (int y = 0; y < n_sub; ++y) {
-            const int w = y * heads + h;
-            const float c = kv_ex2(sm_m[w][row] - (mx == -INFINITY ? 0.f : mx));
-            sum += sm_l[w][row] * c;
+        for (int h = 0; h < 2; ++h) {
+          uint32_t v[4][D / 64];
+          uint32_t vs[4];
 #pragma unroll
-            for (int x = 0; x < D / 32; ++x) {
-              const int d = lane * (D / 32) + x;
-              acc[x] += sm_o(w, row)[(d / (D / 8)) * M::kGroup + d % (D / 8)] * c;
+          for (int x = 0; x < 4; ++x) {
+            const int row = 16 * h + 2 * t + (x & 1) + 8 * (x >> 1);
+            const uint8_t* src = stage + S::kV + kv4_v_offset<D>(row, g * (D / 16));
+            if constexpr (D == 128) {
+              const uint2 u = *reinterpret_cast<const uint2*>(src);
+              v[x][0] = u.x; v[x][1] = u.y;
+              vs[x] = stage[S::kVs + row * 8 + g];
+            } else {
+              v[x][0] = *reinterpret_cast<const uint32_t*>(src);
+              vs[x] = stage[S::kVs + row * 4 + g / 2];
             }
           }
-          if (whole) {
-            const int tok = (i * R + row) / G, head = (group * heads + h) * G + (i * R + row) % G;
-            kv4_write_row<D>(p, acc, sum, static_cast<int64_t>(r.begin) + tok, head, lane);
-          } else {
-            float* dst = part + (h * R + row) * (D + 2);
-            if (lane == 0) { dst[0] = mx; dst[1] = sum; }
+          const __half2 s01 = scales_h2(vs[0] | (vs[1] << 8));
+          const __half2 s23 = scales_h2(vs[2] | (vs[3] << 8));
 #pragma unroll
-            for (int x = 0; x < D / 32; x += 2)
-              *reinterpret_cast<float2*>(dst + 2 + lane * (D / 32) + x) = make_float2(acc[x], acc[x + 1]);
+          for (int w = 0; w < D / 64; ++w) {              // one word a key = four 16-row tiles
+            // pairs along the keys: low nibbles (even channels, MMA rows g) and high ones (odd, g + 8)
+            const uint32_t lo01 = (v[0][w] & 0x0f0f0f0fu) | ((v[1][w] << 4) & 0xf0f0f0f0u);
+            const uint32_t hi01 = ((v[0][w] >> 4) & 0x0f0f0f0fu) | (v[1][w] & 0xf0f0f0f0u);
+            const uint32_t lo23 = (v[2][w] & 0x0f0f0f0fu) | ((v[3][w] << 4) & 0xf0f0f0f0u);
+            const uint32_t hi23 = ((v[2][w] >> 4) & 0x0f0f0f0fu) | (v[3][w] & 0xf0f0f0f0u);
+            __half2 a0[4], a1[4], a2[4], a3[4];
+            e2m1x8(lo01, a0);
+            e2m1x8(hi01, a1);
+            e2m1x8(lo23, a2);
+            e2m1x8(hi23, a3);
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+              const uint32_t u0 = h2_bits(__hmul2(a0[x], s01)), u1 = h2_bits(__hmul2(a1[x], s01));
+              const uint32_t u2 = h2_bits(__hmul2(a2[x], s23)), u3 = h2_bits(__hmul2(a3[x], s23));
+#pragma unroll
+              for (int nb = 0; nb < NB; ++nb)
+                mma_16816(o[nb][4 * w + x], u0, u1, u2, u3, pf[h][nb][0], pf[h][nb][1]);
+            }
           }
         }
-        __syncthreads();
-        at += n;
       }
+      __syncwarp();                                       // the ring is read; O takes its place
+      // ---- join the warps of a head
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) {
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          float x = l[nb][c];
+#pragma unroll
+          for (int d = 4; d < 32; d <<= 1) x += __shfl_xor_sync(0xffffffffu, x, d);
+          const int row = nb * 8 + 2 * t + c;
+          if (g == 0) { sm_m[warp][row] = m[nb][c]; sm_l[warp][row] = x; }
+#pragma unroll
+          for (int k = 0; k < KS; ++k)
+            *reinterpret_cast<float2*>(sm_o(warp, row) + g * M::kGroup + 2 * k) =
+                make_float2(o[nb][k][c], o[nb][k][2 + c]);
+        }
+      }
+      __syncthreads();
+      const bool whole = n == n_span;
+      // a worker has at most two partial results: the rest of an item that an earlier worker began (slot 0) and
+      // the beginning of one that a later worker ends (slot 1)
+      float* part = p.part + (static_cast<int64_t>(blockIdx.x) * 2 + (off == 0 ? 1 : 0)) * p.heads * R * (D + 2);
+      for (int job = warp; job < heads * rows; job += W) {
+        const int h = job & (heads - 1), row = job / heads;
+        float mx = -INFINITY;
+        for (int x = 0; x < n_sub; ++x) mx = fmaxf(mx, sm_m[x * heads + h][row]);
+        float acc[D / 32], sum = 0.f;
+#pragma unroll
+        for (int x = 0; x < D / 32; ++x) acc[x] = 0.f;
+        for (int y = 0; y < n_sub; ++y) {
+          const int w = y * heads + h;
+          const float c = kv_ex2(sm_m[w][row] - (mx == -INFINITY ? 0.f : mx));
+          sum += sm_l[w][row] * c;
+#pragma unroll
+          for (int x = 0; x < D / 32; ++x) {
+            const int d = lane * (D / 32) + x;
+            acc[x] += sm_o(w, row)[(d / (D / 8)) * M::kGroup + d % (D / 8)] * c;
+          }
+        }
+        if (whole) {
+          const int tok = row / G, head = (group * heads + h) * G + row % G;
+          kv4_write_row<D>(p, acc, sum, static_cast<int64_t>(r.begin) + tok, head, lane);
+        } else {
+          float* dst = part + (h * R + row) * (D + 2);
+          if (lane == 0) { dst[0] = mx; dst[1] = sum; }
+#pragma unroll
+          for (int x = 0; x < D / 32; x += 2)
+            *reinterpret_cast<float2*>(dst + 2 + lane * (D / 32) + x) = make_float2(acc[x], acc[x + 1]);
+        }
+      }
+      __syncthreads();
+      at += n;
     }
     // `skip` is below request b's tiles when the range starts in it, and zero from then on
   }
 }
 
 // Joins the partial results of work items that several workers share; items that one worker covered are final already.
-// One CTA per (row block and KV head, request, and, where there are few of them, row).  Its warps share out the rows
+// One CTA per (KV head, request, and, where there are few of them, row).  Its warps share out the rows
 // and, with warps to spare, the partial results of a row.
 constexpr int kMergeWarps = 8;
 template <int D, int NB, int W>
@@ -573,12 +567,12 @@ kv4_merge_kernel(Kv4Args p) {
   __shared__ float sm_o[kMergeWarps][D], sm_l[kMergeWarps];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int G = p.hq / p.hkv;
-  const int b = blockIdx.y, i = blockIdx.x / p.hkv, kvh = blockIdx.x % p.hkv;
+  const int b = blockIdx.y, kvh = blockIdx.x;
   constexpr int kWide = W == 8 ? 8 : 7;
   int64_t before = 0, all = 0, before_all = 0, all_all = 0;
   for (int x = tid; x < p.batch; x += blockDim.x) {
     const Kv4Req r = kv4_request(p, x);
-    const int64_t n = kv4_tiles<R>(p, r, G, 1, kWide), m = kv4_tiles<R>(p, r, G, p.heads, p.tile_shift);
+    const int64_t n = kv4_tiles(p, r, 1, kWide), m = kv4_tiles(p, r, p.heads, p.tile_shift);
     all += n;
     all_all += m;
     if (x < b) { before += n; before_all += m; }
@@ -590,19 +584,15 @@ kv4_merge_kernel(Kv4Args p) {
   before = block_sum_i64<kMergeWarps>(together ? before_all : before, scratch);
   const Kv4Req r = kv4_request(p, b);
   pdl_wait();                               // in every block: this grid ends only after the one before it
-  if (i * R >= r.len * G) return;
-  for (int x = 0; x < i; ++x) {
-    const Kv4Span s = kv4_span<R>(p, r, G, x, tile_shift);
-    before += static_cast<int64_t>(s.last - s.first) * (p.hkv / heads);
-  }
-  const Kv4Span span = kv4_span<R>(p, r, G, i, tile_shift);
+  if (r.len <= 0) return;
+  const Kv4Span span = kv4_span(p, r, tile_shift);
   const int n_span = span.last - span.first;
   const int64_t t0 = before + static_cast<int64_t>(kvh / heads) * n_span, t1 = t0 + n_span;   // this item's tiles
   // tile t belongs to the largest w with floor(all * w / workers) <= t
   const int64_t workers = min(static_cast<int64_t>(p.workers), all);
   const int w0 = static_cast<int>(((t0 + 1) * workers - 1) / all), w1 = static_cast<int>((t1 * workers - 1) / all);
   if (w0 == w1) return;
-  const int rows = min(R, r.len * G - i * R);
+  const int rows = min(R, r.len * G);
   // rows_par rows at a time, `share` warps a row
   const int here = gridDim.z == 1 ? rows : 1;
   const int rows_par = here > 4 ? 8 : here > 2 ? 4 : here, share = kMergeWarps / rows_par;
@@ -650,7 +640,7 @@ kv4_merge_kernel(Kv4Args p) {
       __syncthreads();
     }
     if (live && mine == 0) {
-      const int tok = (i * R + row) / G, head = kvh * G + (i * R + row) % G;
+      const int tok = row / G, head = kvh * G + row % G;
       kv4_write_row<D>(p, acc, sum, static_cast<int64_t>(r.begin) + tok, head, lane);
     }
   }
@@ -682,16 +672,14 @@ static int launch_kv4(Kv4Args a, cudaStream_t st) {
   while ((1 << a.tile_shift) < 32 * (W / a.heads)) ++a.tile_shift;
   attention_kv4_kernel<D, NB, W><<<a.workers, 32 * W, smem, st>>>(a);
   if (cudaGetLastError() != cudaSuccess) return MSL_ERR_CUDA;
-  const int G = a.hq / a.hkv;
-  const int64_t blocks = (static_cast<int64_t>(a.max_q_len) * G + R - 1) / R;
   // The merge forms its schedule while the attention runs and waits for it on the device (programmatic launch).
   cudaLaunchAttribute attr;
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr.val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg = {};
   // few items: a CTA a row, whose warps share its many partial results
-  const int64_t items = blocks * a.hkv * a.batch;
-  cfg.gridDim = dim3(static_cast<unsigned>(blocks * a.hkv), a.batch, items <= sm_count() / 2 ? R : 1);
+  const int64_t items = static_cast<int64_t>(a.hkv) * a.batch;
+  cfg.gridDim = dim3(a.hkv, a.batch, items <= sm_count() / 2 ? R : 1);
   cfg.blockDim = dim3(32 * kMergeWarps);
   cfg.stream = st;
   cfg.attrs = &attr;

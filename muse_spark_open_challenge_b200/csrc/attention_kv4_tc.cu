@@ -439,7 +439,7 @@ attention_kv4_tc_kernel(Kv4Args p, int n_items) {
     float* part_ml = p.part + static_cast<int64_t>(slots) * p.tokens * p.hq * D;
     // What the main loop needs of an item; the rest is formed again for the results.
     struct Mine {
-      int n_tiles, n, kt_begin, qpos, min_qpos, max_qpos, rows;
+      int n_tiles, n, kt_begin, qpos, min_qpos, max_qpos;
       float scale_log2;
     };
     // The next item with tiles from i on; where this sub-tile has some, its query rows go to shared memory (every
@@ -466,7 +466,6 @@ attention_kv4_tc_kernel(Kv4Args p, int n_items) {
         m.qpos = it.seq + min(first_tok + tq, max(it.q_len - 1, 0));
         m.min_qpos = it.seq + first_tok;
         m.max_qpos = sub ? it.max_qpos[1] : it.max_qpos[0];
-        m.rows = sub ? it.rows_valid[1] : it.rows_valid[0];
         if (m.n == 0) return true;
         // f16 with the largest magnitude in [2^14, 2^15)
         const uint4* src = reinterpret_cast<const uint4*>(p.q + token * p.ld_q + (it.kvh * G + g) * D);
@@ -511,18 +510,11 @@ attention_kv4_tc_kernel(Kv4Args p, int n_items) {
       const Mine m = next;
       const int at = i;
       const float scale_log2 = m.scale_log2;
-      const bool any_row = (warp & 3) * 32 < m.rows;
       float m_run = -INFINITY, l_run = 0.f;                // l accumulates 2^kTcShift * sum of exponentials
       for (int j = 0; j < m.n && ok; ++j) {
         const int tile = p.alternate ? 2 * j + sub : j;
         const int key0 = (m.kt_begin + tile) * kTN;
         if (*abort_flag || !mbar_wait(&s_full[sub], (done + j) & 1)) { ok = false; break; }
-        if (!any_row) {                                     // no row of this warp is valid: P may be anything
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) { mbar_arrive(&p_lo[sub]); mbar_arrive(&p_hi[sub]); }
-          continue;
-        }
         tc_fence_after();
         const uint4 hm = *reinterpret_cast<const uint4*>(held + ((tiles + tile) & 7) * 4);
         const bool full_tile = (key0 + kTN - 1 <= m.min_qpos) && (!p.window || key0 > m.max_qpos - p.window) &&
