@@ -657,8 +657,8 @@ attention_kv4_tc_kernel(Kv4Args p, int n_items) {
                 const uint32_t gw[4] = {gq.x, gq.y, gq.z, gq.w};
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                  v[x + 2 * e] *= 1.0f / (1.0f + __expf(-bf16_bits_to_f32(gw[e] & 0xffffu)));
-                  v[x + 2 * e + 1] *= 1.0f / (1.0f + __expf(-bf16_bits_to_f32(gw[e] >> 16)));
+                  v[x + 2 * e] *= __fdividef(1.0f, 1.0f + __expf(-bf16_bits_to_f32(gw[e] & 0xffffu)));
+                  v[x + 2 * e + 1] *= __fdividef(1.0f, 1.0f + __expf(-bf16_bits_to_f32(gw[e] >> 16)));
                 }
               }
             }

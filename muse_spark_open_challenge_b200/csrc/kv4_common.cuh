@@ -100,7 +100,7 @@ __device__ __forceinline__ void kv4_write_row(const Kv4Args& p, float (&o)[D / 3
     const float r = 1.0f / sqrtf(warp_sum(ss) / D + 1e-5f);
     const __nv_bfloat16* grow = p.gate + token * p.ld_gate + head * D + lane * PER;
 #pragma unroll
-    for (int i = 0; i < PER; ++i) o[i] *= r / (1.0f + __expf(-__bfloat162float(grow[i])));
+    for (int i = 0; i < PER; ++i) o[i] *= __fdividef(r, 1.0f + __expf(-__bfloat162float(grow[i])));
   }
   __nv_bfloat16* orow = p.out + token * p.ld_out + head * D + lane * PER;
 #pragma unroll
