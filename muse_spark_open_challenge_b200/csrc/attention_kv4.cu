@@ -30,32 +30,6 @@ namespace msl {
 
 constexpr float kKvTau = 8.0f;             // the running maximum may lag by 2^8: P stays within f16
 
-// A request as the schedule sees it: q rows [begin, begin + len), `seq` cached tokens.
-struct Kv4Req {
-  int begin, len, seq;
-};
-__device__ __forceinline__ Kv4Req kv4_request(const Kv4Args& p, int b) {
-  Kv4Req r;
-  r.begin = max(0, min(p.cu_seqlens_q[b], p.tokens));
-  const int end = max(r.begin, min(p.cu_seqlens_q[b + 1], p.tokens));
-  r.len = min(end - r.begin, p.max_q_len);
-  r.seq = p.seq_lens[b];
-  return r;
-}
-// Key tiles [first, last) that a request's rows can see, 2^tile_shift keys a tile.
-struct Kv4Span {
-  int first, last;
-};
-__device__ __forceinline__ Kv4Span kv4_span(const Kv4Args& p, const Kv4Req& r, int tile_shift) {
-  // keys past the table's row have no page: they are not walked (the kernel reports them)
-  const int hi = static_cast<int>(min(static_cast<int64_t>(r.seq) + r.len,
-                                      static_cast<int64_t>(p.max_pages) * p.page_size));
-  const int lo = p.window ? max(0, r.seq - p.window + 1) : 0;
-  Kv4Span s;
-  s.first = lo >> tile_shift;
-  s.last = max(s.first + 1, (hi + (1 << tile_shift) - 1) >> tile_shift);   // with nothing to see: zeros are written
-  return s;
-}
 // Tiles of a request, all its KV heads, when a CTA takes `heads` of them at once.
 __device__ __forceinline__ int64_t kv4_tiles(const Kv4Args& p, const Kv4Req& r, int heads, int tile_shift) {
   if (r.len <= 0) return 0;
@@ -68,18 +42,6 @@ __device__ __forceinline__ int64_t kv4_tiles(const Kv4Args& p, const Kv4Req& r, 
 // results per item to join, which a short step cannot hide.  64 requests x 8192 keys, 8 heads: 291 -> 174 us with all
 // heads at once; 1 x 4096: 18 -> 40 us.
 constexpr int kKvLong = 8;
-
-template <int W>
-__device__ __forceinline__ int64_t block_sum_i64(int64_t v, int64_t* scratch) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = v;
-  __syncthreads();
-  int64_t s = 0;
-  for (int w = 0; w < W; ++w) s += scratch[w];
-  __syncthreads();
-  return s;
-}
 
 __device__ __forceinline__ void mma_16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
                                           uint32_t b0, uint32_t b1) {
@@ -711,7 +673,9 @@ static Kv4Plan kv4_plan(int batch, int max_q_len, int tokens, int hq, int hkv, i
   } else {
     plan.splits = msl_attention_split_plan(batch, max_q_len, hq, hkv, max_pages, page_size, window);
     plan.alternate = rows <= 128;
-    plan.bytes = kv4_tc_workspace(plan.splits * (plan.alternate ? 2 : 1), tokens, hq, head_dim);
+    if (plan.alternate) plan.splits = 1;
+    plan.bytes = plan.alternate ? kv4_tc_shared_workspace(static_cast<int>(rows), tokens, hq, head_dim)
+                                : kv4_tc_workspace(plan.splits, tokens, hq, head_dim);
   }
   return plan;
 }

@@ -13,7 +13,7 @@
 //                   N-major (V) swizzled operand tiles of a ring
 //   warps 9-11      idle: they round the warpgroup up whose registers the others use
 // Registers are split 184 (softmax) / 56 / 88 (producers): 128 x (184 + 184 + 56 + 88) = 65536, the launch's total.
-// P is f16 (2^-12 relative) times 2^6, which with a lag of the running maximum of at most 2^8 stays below 2^15.
+// P is f16 (half a step 2^-11) times 2^6, which with a lag of the running maximum of at most 2^8 stays below 2^15.
 // A key whose page is missing is hidden: producers leave one bit per key, and the mask pass takes it with the causal
 // limits.  Every wait is bounded.
 #include "kv4_common.cuh"
@@ -217,7 +217,7 @@ __device__ __forceinline__ bool tc_item(const Kv4Args& p, int i, TcItem& it) {
   it.kt_begin = it.key_lo / kTN;
 #pragma unroll
   for (int s = 0; s < 2; ++s) {
-    it.first_tok[s] = q0 + (p.alternate ? 0 : s * TQ);     // alternate: both sub-tiles hold the same rows
+    it.first_tok[s] = q0 + s * TQ;
     const int cnt = max(0, min(TQ, it.q_len - it.first_tok[s]));
     it.rows_valid[s] = cnt * G;
     it.max_qpos[s] = it.seq + it.first_tok[s] + cnt - 1;
@@ -235,18 +235,75 @@ __device__ __forceinline__ bool tc_item(const Kv4Args& p, int i, TcItem& it) {
     it.kt_begin += lo;
     it.n_tiles = max(it.n_sub[0], it.n_sub[1]);
   }
-  if (p.alternate) {
-    it.n_sub[0] = (it.n_tiles + 1) / 2;
-    it.n_sub[1] = it.n_tiles / 2;
-  }
   return true;
 }
+// What a CTA works on, item by item; every role of it makes the same walk.
+//   SHARED = false  block i, i + gridDim.x, ... of the list above
+//   SHARED = true   up to 128 rows a request (verify blocks): the key tiles of all requests and KV heads, laid end to
+//                   end, are cut into equal ranges, one a CTA, as in csrc/attention_kv4.cu; the two sub-tiles hold the same
+//                   rows and take the tiles of an item in turn.  16 requests x 8 tokens after 500 .. 8192: 94 us
+//                   against 125 with the requests' own slices.
+template <bool SHARED>
+struct TcWalk;
+template <>
+struct TcWalk<false> {
+  int i;                                                    // next block
+};
+template <>
+struct TcWalk<true> {
+  int b;                                                    // request
+  int64_t skip, at, end;                                    // its tiles before; the range that is left
+};
+__device__ __forceinline__ bool tc_next(const Kv4Args& p, int n_items, TcWalk<false>& w, TcItem& it) {
+  for (; w.i < n_items; w.i += gridDim.x)
+    if (tc_item(p, w.i, it)) return true;
+  return false;
+}
+__device__ __forceinline__ void tc_step(TcWalk<false>& w) { w.i += gridDim.x; }
+__device__ __forceinline__ void tc_step(TcWalk<true>&) {}
+__device__ __forceinline__ bool tc_next(const Kv4Args& p, int, TcWalk<true>& w, TcItem& it) {
+  while (w.at < w.end && w.b < p.batch) {
+    const Kv4Req r = kv4_request(p, w.b);
+    if (r.len <= 0) { ++w.b; continue; }
+    const Kv4Span span = kv4_span(p, r, 7);
+    const int n_span = span.last - span.first, off = static_cast<int>(w.skip % n_span);
+    it.b = w.b;
+    it.kvh = static_cast<int>(w.skip / n_span);
+    it.q_begin = r.begin;
+    it.q_len = r.len;
+    it.seq = r.seq;
+    it.key_lo = p.window ? max(0, r.seq - p.window + 1) : 0;
+    it.kt_begin = span.first + off;
+    it.last_qpos = r.seq + r.len - 1;
+    it.n_tiles = static_cast<int>(min(w.end - w.at, static_cast<int64_t>(n_span - off)));
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      it.first_tok[s] = 0;
+      it.rows_valid[s] = r.len * (p.hq / p.hkv);
+      it.max_qpos[s] = it.last_qpos;
+      it.n_sub[s] = (it.n_tiles + 1 - s) / 2;
+    }
+    // where its result goes: an item has one beginning (-1), a CTA at most one rest of an item that an earlier one began
+    it.split = off == 0 ? -1 : static_cast<int>(blockIdx.x);
+    w.at += it.n_tiles;
+    w.skip += it.n_tiles;
+    if (w.skip == static_cast<int64_t>(n_span) * p.hkv) { w.skip = 0; ++w.b; }
+    return true;
+  }
+  return false;
+}
+
 // Place of the tiles of an item with n tiles in the order in which the ring carries them: `lag` K tiles first, then V(j)
 // and K(j + lag) in turn.
 __device__ __forceinline__ int tc_place_k(int j, int lag) { return j < lag ? j : 2 * j - lag + 1; }
 __device__ __forceinline__ int tc_place_v(int j, int n, int lag) { return min(lag, n) + j + min(j, max(n - lag, 0)); }
 
-template <int D>
+// Rows of partial results of shared ranges: two sub-tiles' beginnings of each query row, and `ctas` CTAs' rests.
+__host__ __device__ __forceinline__ int64_t kv4_tc_shared_parts(int tokens, int hq, int ctas, int max_rows) {
+  return 2 * (static_cast<int64_t>(tokens) * hq + static_cast<int64_t>(ctas) * max_rows);
+}
+
+template <int D, bool SHARED>
 __global__ void __launch_bounds__(kTcThreads, 1)
 attention_kv4_tc_kernel(Kv4Args p, int n_items) {
   using S = TcSmem<D>;
@@ -267,7 +324,47 @@ attention_kv4_tc_kernel(Kv4Args p, int n_items) {
   uint32_t* held = reinterpret_cast<uint32_t*>(smem + S::kHeld);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int lag = p.alternate ? 2 : 1;
+  constexpr int lag = SHARED ? 2 : 1;
+  TcWalk<SHARED> walk0;
+  if constexpr (!SHARED) {
+    walk0.i = blockIdx.x;
+  } else {
+    pdl_launch_dependents();
+    __shared__ int64_t scratch[kTcThreads / 32];
+    __shared__ TcWalk<true> found;
+    const auto tiles_of = [&](int b) {
+      const Kv4Req r = kv4_request(p, b);
+      const Kv4Span span = kv4_span(p, r, 7);
+      return r.len > 0 ? static_cast<int64_t>(span.last - span.first) * p.hkv : 0;
+    };
+    const int per = (p.batch + kTcThreads - 1) / kTcThreads;
+    const int b0 = min(static_cast<int>(threadIdx.x) * per, p.batch), b1 = min(b0 + per, p.batch);
+    int64_t mine = 0, total = 0;
+    for (int b = b0; b < b1; ++b) mine += tiles_of(b);
+    int64_t inc = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t x = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc += x;
+    }
+    if (lane == 31) scratch[warp] = inc;
+    __syncthreads();
+    for (int w = 0; w < kTcThreads / 32; ++w) {
+      if (w < warp) inc += scratch[w];
+      total += scratch[w];
+    }
+    const int64_t workers = min(static_cast<int64_t>(gridDim.x), total);   // no empty range in between
+    if (blockIdx.x >= workers) return;                      // uniform, before any barrier of the roles
+    const int64_t at = total * blockIdx.x / workers;
+    if (inc - mine <= at && at < inc) {                     // one thread: walk its few requests
+      int64_t base = inc - mine;
+      int b = b0;
+      for (; b < b1 - 1 && at >= base + tiles_of(b); ++b) base += tiles_of(b);
+      found = TcWalk<true>{b, at - base, at, total * (blockIdx.x + 1) / workers};
+    }
+    __syncthreads();
+    walk0 = found;
+  }
   if (threadIdx.x == 0) {
     for (int i = 0; i < kSt; ++i) { mbar_init(&full[i], 4); mbar_init(&empty[i], 1); }
     for (int i = 0; i < 2; ++i) {
@@ -292,9 +389,10 @@ attention_kv4_tc_kernel(Kv4Args p, int n_items) {
     const int r = (warp - 12) * 32 + lane;
     bool ok = true;
     int pos = 0, tiles = 0;                                 // ring places and tiles of the items before
-    for (int i = blockIdx.x; i < n_items && ok; i += gridDim.x) {
-      TcItem it;
-      if (!tc_item(p, i, it) || it.n_tiles == 0) continue;
+    TcWalk<SHARED> walk = walk0;
+    TcItem it;
+    for (; ok && tc_next(p, n_items, walk, it); tc_step(walk)) {
+      if (it.n_tiles == 0) continue;
       const int n = it.n_tiles;
       const int* table = p.page_table + static_cast<int64_t>(it.b) * p.max_pages;
       const int first_key = it.kt_begin * kTN + r, hi = it.last_qpos + 1;
@@ -363,9 +461,10 @@ attention_kv4_tc_kernel(Kv4Args p, int n_items) {
       bool ok = true;
       int pos = 0, taken0 = 0, taken1 = 0;                  // ring places of, and items with tiles for, the sub-tiles before
       int done0 = 0, done1 = 0;                             // their tiles
-      for (int i = blockIdx.x; i < n_items && ok; i += gridDim.x) {
-        TcItem it;
-        if (!tc_item(p, i, it) || it.n_tiles == 0) continue;
+      TcWalk<SHARED> walk = walk0;
+      TcItem it;
+      for (; ok && tc_next(p, n_items, walk, it); tc_step(walk)) {
+        if (it.n_tiles == 0) continue;
         const int n = it.n_tiles;
         const auto wait_full = [&](int place) {
           const bool got = !*abort_flag && mbar_wait(&full[place % kSt], (place / kSt) & 1);
@@ -382,18 +481,18 @@ attention_kv4_tc_kernel(Kv4Args p, int n_items) {
           const uint32_t sk = ring + (place % kSt) * S::kTile;
 #pragma unroll 1
           for (int s = 0; s < 2; ++s)
-            if (p.alternate ? s == j : (s ? it.n_sub[1] : it.n_sub[0]) > 0) issue_qk(s, sk);
+            if (SHARED ? s == j : (s ? it.n_sub[1] : it.n_sub[0]) > 0) issue_qk(s, sk);
           tc_commit_if(on, &empty[place % kSt]);
         }
         for (int j = 0; j < n && ok; ++j) {
           const int pv = pos + tc_place_v(j, n, lag), pk = pos + tc_place_k(j + lag, lag);
           const uint32_t sv = ring + (pv % kSt) * S::kTile, sk = ring + (pk % kSt) * S::kTile;
-          const int local = p.alternate ? j >> 1 : j;       // this tile's number among the sub-tile's own
+          const int local = SHARED ? j >> 1 : j;       // this tile's number among the sub-tile's own
           bool v_ready = false, k_ready = false;
 #pragma unroll 1
           for (int s = 0; s < 2; ++s) {
             const int mine = s ? it.n_sub[1] : it.n_sub[0];
-            if (!(p.alternate ? (j & 1) == s : j < mine)) continue;
+            if (!(SHARED ? (j & 1) == s : j < mine)) continue;
             const uint32_t ph = ((s ? done1 : done0) + local) & 1;
             if (!v_ready) {
               if (!wait_full(pv)) { ok = false; break; }
@@ -435,8 +534,17 @@ attention_kv4_tc_kernel(Kv4Args p, int n_items) {
     const uint32_t lane_sel = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t tmem_s = tmem_base + sub * kTN + lane_sel;
     const uint32_t tmem_o = tmem_base + 2 * kTN + sub * kTN + lane_sel;
-    const int slots = p.kv_splits * (p.alternate ? 2 : 1);  // partial results per row; one: the row is written at once
-    float* part_ml = p.part + static_cast<int64_t>(slots) * p.tokens * p.hq * D;
+    // Partial results: slices of a query block's keys by (slice, token, head); of shared ranges the beginnings of items by
+    // (sub-tile, token, head), then the rests by (CTA, sub-tile, row).  Without any a row is written at once.
+    const bool partial = SHARED || p.kv_splits > 1;
+    const int max_rows = p.max_q_len * G;
+    float* part_ml = p.part + (SHARED ? kv4_tc_shared_parts(p.tokens, p.hq, gridDim.x, max_rows)
+                                      : static_cast<int64_t>(p.kv_splits) * p.tokens * p.hq) * D;
+    const auto part_index = [&](const TcItem& it, int64_t token) {
+      if (SHARED && it.split >= 0)
+        return kv4_tc_shared_parts(p.tokens, p.hq, it.split, max_rows) + static_cast<int64_t>(sub) * max_rows + r;
+      return (static_cast<int64_t>(SHARED ? sub : it.split) * p.tokens + token) * p.hq + it.kvh * G + g;
+    };
     // What the main loop needs of an item; the rest is formed again for the results.
     struct Mine {
       int n_tiles, n, kt_begin, qpos, min_qpos, max_qpos;
@@ -444,17 +552,17 @@ attention_kv4_tc_kernel(Kv4Args p, int n_items) {
     };
     // The next item with tiles from i on; where this sub-tile has some, its query rows go to shared memory (every
     // Q K^T of the sub-tile before has finished: its last S has been waited for).  Empty slices are dealt with here.
-    const auto take = [&](int& i, Mine& m) {
-      for (; i < n_items; i += gridDim.x) {
+    const auto take = [&](TcWalk<SHARED>& walk, TcWalk<SHARED>& before, Mine& m) {
+      for (;; tc_step(walk)) {
         TcItem it;
-        if (!tc_item(p, i, it)) continue;
+        if constexpr (SHARED) before = walk;
+        if (!tc_next(p, n_items, walk, it)) return false;
         const int first_tok = sub ? it.first_tok[1] : it.first_tok[0];
         const bool valid = r < (sub ? it.rows_valid[1] : it.rows_valid[0]);
         const int64_t token = static_cast<int64_t>(it.q_begin) + first_tok + tq;
         if (it.n_tiles == 0) {
           if (valid) {
-            const int slot = p.alternate ? 2 * it.split + sub : it.split;
-            const int64_t idx = (static_cast<int64_t>(slot) * p.tokens + token) * p.hq + it.kvh * G + g;
+            const int64_t idx = part_index(it, token);
             part_ml[2 * idx] = -INFINITY;
             part_ml[2 * idx + 1] = 0.f;
           }
@@ -497,22 +605,22 @@ attention_kv4_tc_kernel(Kv4Args p, int n_items) {
         if (lane == 0) mbar_arrive(&q_full[sub]);
         return true;
       }
-      return false;
     };
 
     bool ok = true;
     int done = 0, tiles = 0, outs = 0;                      // of this sub-tile, of the CTA, results: items before
-    int i = blockIdx.x;
+    TcWalk<SHARED> walk = walk0, before, at;
     Mine next;
     next.scale_log2 = 0.f;
-    bool more = take(i, next);
+    bool more = take(walk, before, next);
     while (more && ok) {
       const Mine m = next;
-      const int at = i;
+      if constexpr (SHARED) at = before;
+      else at = walk;
       const float scale_log2 = m.scale_log2;
       float m_run = -INFINITY, l_run = 0.f;                // l accumulates 2^kTcShift * sum of exponentials
       for (int j = 0; j < m.n && ok; ++j) {
-        const int tile = p.alternate ? 2 * j + sub : j;
+        const int tile = SHARED ? 2 * j + sub : j;
         const int key0 = (m.kt_begin + tile) * kTN;
         if (*abort_flag || !mbar_wait(&s_full[sub], (done + j) & 1)) { ok = false; break; }
         tc_fence_after();
@@ -585,12 +693,13 @@ attention_kv4_tc_kernel(Kv4Args p, int n_items) {
       done += m.n;
       tiles += m.n_tiles;
       // The next item's queries before this one's results: its first Q K^T runs behind the last P V.
-      i += gridDim.x;
-      more = take(i, next);
+      tc_step(walk);
+      more = take(walk, before, next);
 
       // -------------------------------------------------------------- epilogue
       TcItem it;
-      tc_item(p, at, it);
+      if constexpr (SHARED) tc_next(p, n_items, at, it);
+      else tc_item(p, at.i, it);
       const int n_mine = m.n;
       const bool row_valid = r < (sub ? it.rows_valid[1] : it.rows_valid[0]);
       const int64_t token = static_cast<int64_t>(it.q_begin) + (sub ? it.first_tok[1] : it.first_tok[0]) + tq;
@@ -600,10 +709,9 @@ attention_kv4_tc_kernel(Kv4Args p, int n_items) {
         ++outs;
         tc_fence_after();
       }
-      if (slots > 1) {
-        // partial result of this key slice: O as it stands in TMEM, with the maximum and sum it refers to
-        const int slot = p.alternate ? 2 * it.split + sub : it.split;
-        const int64_t idx = (static_cast<int64_t>(slot) * p.tokens + token) * p.hq + head;
+      if (partial) {
+        // partial result of these key tiles: O as it stands in TMEM, with the maximum and sum it refers to
+        const int64_t idx = part_index(it, token);
         if (row_valid) {
           part_ml[2 * idx] = m_run;
           part_ml[2 * idx + 1] = l_run;
@@ -696,7 +804,7 @@ kv4_tc_merge_kernel(Kv4Args p) {
   if (item >= static_cast<int64_t>(q_len) * p.hq) return;
   const int64_t token = q_begin + item / p.hq;
   const int head = static_cast<int>(item % p.hq);
-  const int slots = p.kv_splits * (p.alternate ? 2 : 1);
+  const int slots = p.kv_splits;
   const float* part_ml = p.part + static_cast<int64_t>(slots) * p.tokens * p.hq * D;
   const int64_t stride = static_cast<int64_t>(p.tokens) * p.hq, base = token * p.hq + head;
   float mx = -INFINITY;
@@ -717,17 +825,91 @@ kv4_tc_merge_kernel(Kv4Args p) {
   kv4_write_row<D>(p, acc, sum, token, head, lane);
 }
 
+// Joins the partial results of shared ranges: one CTA per (KV head, request, eight rows), a warp a row.
 template <int D>
+__global__ void __launch_bounds__(256)
+kv4_tc_shared_merge_kernel(Kv4Args p, int ctas) {
+  constexpr int PER = D / 32;
+  __shared__ int64_t scratch[8];
+  const int lane = threadIdx.x & 31, b = blockIdx.y, kvh = blockIdx.x, G = p.hq / p.hkv;
+  const int row = blockIdx.z * 8 + (threadIdx.x >> 5);
+  int64_t before = 0, all = 0;
+  for (int x = threadIdx.x; x < p.batch; x += blockDim.x) {
+    const Kv4Req r = kv4_request(p, x);
+    const Kv4Span span = kv4_span(p, r, 7);
+    const int64_t n = r.len > 0 ? static_cast<int64_t>(span.last - span.first) * p.hkv : 0;
+    all += n;
+    if (x < b) before += n;
+  }
+  before = block_sum_i64<8>(before, scratch);
+  all = block_sum_i64<8>(all, scratch);
+  const Kv4Req r = kv4_request(p, b);
+  pdl_wait();                               // in every block: this grid ends only after the one before it
+  if (row >= r.len * G) return;
+  const Kv4Span span = kv4_span(p, r, 7);
+  const int n_span = span.last - span.first;
+  const int64_t t0 = before + static_cast<int64_t>(kvh) * n_span, t1 = t0 + n_span;   // this item's tiles
+  // tile t belongs to the largest w with floor(all * w / workers) <= t
+  const int64_t workers = min(static_cast<int64_t>(ctas), all);
+  const int w0 = static_cast<int>(((t0 + 1) * workers - 1) / all), w1 = static_cast<int>((t1 * workers - 1) / all);
+  const int max_rows = p.max_q_len * G, n = 2 * (w1 - w0 + 1);
+  const int64_t token = static_cast<int64_t>(r.begin) + row / G;
+  const int head = kvh * G + row % G;
+  const float* part_ml = p.part + kv4_tc_shared_parts(p.tokens, p.hq, ctas, max_rows) * D;
+  // the i-th partial result: sub-tile i % 2 of CTA w0 + i / 2, the first CTA's the beginning
+  const auto index = [&](int i) {
+    return i < 2 ? (static_cast<int64_t>(i) * p.tokens + token) * p.hq + head
+                 : kv4_tc_shared_parts(p.tokens, p.hq, w0 + i / 2, max_rows) + static_cast<int64_t>(i & 1) * max_rows + row;
+  };
+  float mx = -INFINITY;
+  for (int i = lane; i < n; i += 32) mx = fmaxf(mx, part_ml[2 * index(i)]);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+  const float ref = mx == -INFINITY ? 0.f : mx;
+  float acc[PER], sum = 0.f;
+#pragma unroll
+  for (int x = 0; x < PER; ++x) acc[x] = 0.f;
+#pragma unroll 4
+  for (int i = 0; i < n; ++i) {
+    const int64_t at = index(i);
+    const float l = part_ml[2 * at + 1];
+    if (l == 0.f) continue;                                 // a sub-tile without tiles wrote no O
+    const float c = kv_ex2(part_ml[2 * at] - ref);
+    sum += l * c;
+    const float* o = p.part + at * D + lane * PER;
+#pragma unroll
+    for (int x = 0; x < PER; ++x) acc[x] += o[x] * c;
+  }
+  kv4_write_row<D>(p, acc, sum, token, head, lane);
+}
+
+template <int D, bool SHARED>
 static int launch_tc(const Kv4Args& a, cudaStream_t st) {
   const int smem = TcSmem<D>::kTotal + 1024;
   static SmemConfig config;
-  if (int rc = config.ensure(attention_kv4_tc_kernel<D>, smem)) return rc;
+  if (int rc = config.ensure(attention_kv4_tc_kernel<D, SHARED>, smem)) return rc;
+  if constexpr (SHARED) {
+    const int ctas = sm_count();
+    attention_kv4_tc_kernel<D, true><<<ctas, kTcThreads, smem, st>>>(a, 0);
+    if (cudaGetLastError() != cudaSuccess) return MSL_ERR_CUDA;
+    // The merge forms its schedule while the attention runs and waits for it on the device (programmatic launch).
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(a.hkv, a.batch, (a.max_q_len * (a.hq / a.hkv) + 7) / 8);
+    cfg.blockDim = dim3(256);
+    cfg.stream = st;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kv4_tc_shared_merge_kernel<D>, a, ctas) == cudaSuccess ? MSL_OK : MSL_ERR_CUDA;
+  }
   const int tq2 = 2 * (kTM / (a.hq / a.hkv));
   const int64_t items = static_cast<int64_t>((a.max_q_len + tq2 - 1) / tq2) * a.kv_splits * a.hkv * a.batch;
   if (items > 0x7fffffff) return MSL_ERR_UNSUPPORTED;
-  attention_kv4_tc_kernel<D><<<static_cast<int>(std::min<int64_t>(items, sm_count())), kTcThreads, smem, st>>>(
+  attention_kv4_tc_kernel<D, false><<<static_cast<int>(std::min<int64_t>(items, sm_count())), kTcThreads, smem, st>>>(
       a, static_cast<int>(items));
-  if (a.kv_splits > 1 || a.alternate) {
+  if (a.kv_splits > 1) {
     const int64_t rows = static_cast<int64_t>(a.max_q_len) * a.hq;
     kv4_tc_merge_kernel<D><<<dim3(static_cast<unsigned>((rows + 7) / 8), a.batch), 256, 0, st>>>(a);
   }
@@ -735,7 +917,13 @@ static int launch_tc(const Kv4Args& a, cudaStream_t st) {
 }
 
 int launch_kv4_tc(const Kv4Args& a, int head_dim, cudaStream_t st) {
-  return head_dim == 128 ? launch_tc<128>(a, st) : launch_tc<64>(a, st);
+  if (a.alternate) return head_dim == 128 ? launch_tc<128, true>(a, st) : launch_tc<64, true>(a, st);
+  return head_dim == 128 ? launch_tc<128, false>(a, st) : launch_tc<64, false>(a, st);
+}
+
+// Two partial results of two sub-tiles a CTA.
+int64_t kv4_tc_shared_workspace(int rows, int tokens, int hq, int head_dim) {
+  return kv4_tc_shared_parts(tokens, hq, sm_count(), rows) * (head_dim + 2) * 4;
 }
 
 int64_t kv4_tc_workspace(int slots, int tokens, int hq, int head_dim) {

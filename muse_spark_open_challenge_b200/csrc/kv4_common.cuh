@@ -32,7 +32,7 @@ struct Kv4Args {
   int heads;                    //   KV heads a CTA takes at once,
   int tile_shift;               //   log2 of a tile's keys
   int kv_splits;                // many rows: slices of a query block's keys
-  int alternate;                //   one block of up to 128 rows: the two sub-tiles take its key tiles in turn
+  int alternate;                //   up to 128 rows a request: CTAs share the key tiles, their sub-tiles in turn
   int page_shift;               // log2 of the page size, -1: not a power of two
   int* status;
 };
@@ -60,6 +60,44 @@ __device__ __forceinline__ __half2 scales_h2(uint32_t two) {
   asm("{.reg .b16 x;\n\tcvt.u16.u32 x, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, x;}" : "=r"(h) : "r"(two));
   return __hmin2(bits_h2(h), __half2half2(__ushort_as_half(0x5F00)));   // 448
 }
+// A request as the schedule sees it: q rows [begin, begin + len), `seq` cached tokens.
+struct Kv4Req {
+  int begin, len, seq;
+};
+__device__ __forceinline__ Kv4Req kv4_request(const Kv4Args& p, int b) {
+  Kv4Req r;
+  r.begin = max(0, min(p.cu_seqlens_q[b], p.tokens));
+  const int end = max(r.begin, min(p.cu_seqlens_q[b + 1], p.tokens));
+  r.len = min(end - r.begin, p.max_q_len);
+  r.seq = p.seq_lens[b];
+  return r;
+}
+// Key tiles [first, last) that a request's rows can see, 2^tile_shift keys a tile.
+struct Kv4Span {
+  int first, last;
+};
+__device__ __forceinline__ Kv4Span kv4_span(const Kv4Args& p, const Kv4Req& r, int tile_shift) {
+  // keys past the table's row have no page: they are not walked (the kernel reports them)
+  const int hi = static_cast<int>(min(static_cast<int64_t>(r.seq) + r.len,
+                                      static_cast<int64_t>(p.max_pages) * p.page_size));
+  const int lo = p.window ? max(0, r.seq - p.window + 1) : 0;
+  Kv4Span s;
+  s.first = lo >> tile_shift;
+  s.last = max(s.first + 1, (hi + (1 << tile_shift) - 1) >> tile_shift);   // with nothing to see: zeros are written
+  return s;
+}
+template <int W>
+__device__ __forceinline__ int64_t block_sum_i64(int64_t v, int64_t* scratch) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = v;
+  __syncthreads();
+  int64_t s = 0;
+  for (int w = 0; w < W; ++w) s += scratch[w];
+  __syncthreads();
+  return s;
+}
+
 // Programmatic launch: the next kernel's blocks may start; wait until the kernel before has ended and its writes show.
 __device__ __forceinline__ void pdl_launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
@@ -110,5 +148,6 @@ __device__ __forceinline__ void kv4_write_row(const Kv4Args& p, float (&o)[D / 3
 // Many query rows per KV head (prefill, chunks): csrc/attention_kv4_tc.cu.
 int launch_kv4_tc(const Kv4Args& a, int head_dim, cudaStream_t st);
 int64_t kv4_tc_workspace(int slots, int tokens, int hq, int head_dim);
+int64_t kv4_tc_shared_workspace(int rows, int tokens, int hq, int head_dim);
 
 }  // namespace msl

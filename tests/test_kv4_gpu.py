@@ -354,6 +354,21 @@ def test_attention_many_workers_and_ragged_batches(ops, status, batch, ctx_hi):
     assert torch.equal(first, again) and int(status) == 0
 
 
+@pytest.mark.parametrize("batch,hq,hkv,d,new_hi,ctx_hi,window", [
+    (90, 16, 8, 64, 12, 300, 0),      # several whole (request, KV head) pairs in one block's range of key tiles
+    (400, 8, 2, 64, 9, 40, 0),        # one key tile each
+    (3, 16, 2, 128, 16, 9000, 0),     # one pair over many blocks
+    (70, 16, 4, 128, 32, 1500, 200),  # ranges that end inside pairs, a window in front
+])
+def test_attention_blocks_of_rows_share_the_key_tiles(ops, status, batch, hq, hkv, d, new_hi, ctx_hi, window):
+    rng = random.Random(batch)
+    new = [rng.choice([0, 1, rng.randint(1, new_hi)]) for _ in range(batch)]
+    new[1] = new_hi                   # 17 to 128 rows a KV head
+    ctx = [rng.randint(0, ctx_hi) for _ in range(batch)]
+    check_attention(ops, status, new, ctx, hq, hkv, d, 16, window, batch % 20 == 0, seed=batch)
+    assert int(status) == 0
+
+
 @pytest.mark.parametrize("new", [1, 140])
 def test_attention_offsets_beyond_32_bits(ops, status, new):
     """Cache rows whose byte offset passes 2^32 (keys and values share one buffer to save memory)."""
