@@ -18,9 +18,10 @@
 // Codes become f16 by the e2m1 conversion, times their block scale: exact (2 + 4 significant bits).  P^T moves
 // from the accumulator's layout to the operand's by one 8 x 8 transpose in registers.  Queries (bf16) are scaled by
 // a power of two per row so that the largest magnitude lies in [2^14, 2^15) and held in f16: exact for every
-// element within 2^28 of the row's largest.  P is f16 (half a step 2^-11), statistics and O are fp32.
+// element within 2^28 of the row's largest.  P is f16 (half a step 2^-11) times 2^6, which keeps the weights of a long
+// context behind one dominating key out of f16's subnormals down to 2^-20; statistics and O are fp32.
 //
-// What bounds it: issue slots.  64 requests x 8192 keys, 8 heads x 128 (604 MB): 174 us = 3.5 TB/s of the measured 6.55
+// What bounds it: issue slots.  64 requests x 8192 keys, 8 heads x 128 (604 MB): 146 us = 4.1 TB/s of the measured 6.55
 // with DRAM traffic equal to the bytes needed; 720 warp instructions per 32 keys (640 of them converting and scaling
 // 8192 elements), 0.6 issued per cycle and scheduler, ALU half busy.  On the way: codes straight from global memory into
 // registers 330 us (one ragged batch), the ring 263 us, the heads of a cache row fetched together 171 us.
@@ -28,7 +29,8 @@
 
 namespace msl {
 
-constexpr float kKvTau = 8.0f;             // the running maximum may lag by 2^8: P stays within f16
+constexpr float kKvTau = 8.0f;             // the running maximum may lag by 2^8,
+constexpr float kKvShift = 6.0f;           // so P 2^6 stays below 2^15, within f16
 
 // Tiles of a request, all its KV heads, when a CTA takes `heads` of them at once.
 __device__ __forceinline__ int64_t kv4_tiles(const Kv4Args& p, const Kv4Req& r, int heads, int tile_shift) {
@@ -405,7 +407,9 @@ attention_kv4_kernel(Kv4Args p) {
         uint32_t pf[2][NB][2];
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) {
-          const float n0 = m[nb][0] == -INFINITY ? 0.f : m[nb][0], n1 = m[nb][1] == -INFINITY ? 0.f : m[nb][1];
+          // l and O carry P's 2^shift alike, here and in the partial results
+          const float n0 = m[nb][0] == -INFINITY ? 0.f : m[nb][0] - kKvShift;
+          const float n1 = m[nb][1] == -INFINITY ? 0.f : m[nb][1] - kKvShift;
 #pragma unroll
           for (int h = 0; h < 2; ++h)
 #pragma unroll

@@ -2,6 +2,7 @@
 exactly, attention within a bound derived from its roundings; masks that leave little or nothing, pages of any size,
 ragged and empty requests, pitches, garbage in hidden places, capture, other streams, and the layer over such a cache."""
 import dataclasses
+import math
 import random
 
 import pytest
@@ -367,6 +368,30 @@ def test_attention_blocks_of_rows_share_the_key_tiles(ops, status, batch, hq, hk
     ctx = [rng.randint(0, ctx_hi) for _ in range(batch)]
     check_attention(ops, status, new, ctx, hq, hkv, d, 16, window, batch % 20 == 0, seed=batch)
     assert int(status) == 0
+
+
+@pytest.mark.parametrize("batch,new", [(300, 1), (300, 4), (3, 24), (2, 150)])
+def test_attention_small_weights_behind_dominating_keys(ops, status, batch, new):
+    """Eight keys take nearly all the weight and have no value; each of 2000 others weighs 1.37 * 2^-22 of one of them.
+    P carries 2^6, so such a weight is 1.37 * 2^-16 and rounded by at most 2^-25, below 2^-9 of it; fp32 sums and
+    exponentials are good to 2^-13, and bf16 adds 2^-8."""
+    hq, hkv, d, page, ctx = 8, 2, 64, 16, 2000
+    pages = -(-(ctx + new) // page)
+    k = torch.zeros((pages * page, hkv, d // 2), dtype=torch.uint8)
+    v = torch.full_like(k, 0x22)                                    # ones
+    sf = torch.full((pages * page, hkv, d // 16), 0x38, dtype=torch.uint8)
+    k[0:256:32] = 0x22
+    v[0:256:32] = 0
+    q = torch.ones((batch * new, hq, d), dtype=torch.bfloat16, device="cuda")
+    one = torch.tensor(1.0, device="cuda")
+    table = torch.arange(pages, dtype=torch.int32).repeat(batch, 1)
+    scale = math.log(2 ** 22 / 1.37) / d
+    got = run_attention(ops, q, (k, sf, v, sf), table, [ctx] * batch, [new * b for b in range(batch + 1)], new, hq, hkv, d,
+                        page, 0, scale, status=status, scales=(one, one))
+    assert int(status) == 0
+    others = (ctx + 1 - 8 + torch.arange(new).double()) * 1.37 * 2 ** -22
+    want = (others / (8 + others)).repeat(batch)[:, None]
+    assert ((got.cpu().double() - want).abs() <= want * (2 ** -8 + 2 ** -9 + 2 ** -12)).all()
 
 
 @pytest.mark.parametrize("new", [1, 140])
