@@ -398,7 +398,8 @@ qk_rope_store_kv4_kernel(StoreArgs p) {
       }
       // fp32 errors, in half steps of 2^-24: 14 in r (16 products and 3 sums of shuffles, halved by the root; the root
       // 4), 1 in e, 3 in cosine and sine, 2 in the rotation, so 20 (|e| + |o|) <= 40 largest magnitudes of the block:
-      // 2^-18.6 of it, 1.6e-5 of a code's unit; the nudge is 3e-5
+      // 2^-18.6 of it.  That magnitude is at most 6.4 of a code's units, so 1.6e-5 of one; the nudge is 3e-5.  (Where the
+      // scale saturates at 448 the block reaches further: 64 bits.)
       float amax = 0.f;
 #pragma unroll
       for (int i = 0; i < 16; ++i) amax = fmaxf(amax, fabsf(v[i]));
@@ -407,7 +408,7 @@ qk_rope_store_kv4_kernel(StoreArgs p) {
       const float inv = __fdividef(inv_k, e4m3_to_f32(s8));
       uint2 packed = e2m1_of_16<true>(v, inv, 3.0517578125e-5f);
       const uint2 below = e2m1_of_16<false>(v, inv, 3.0517578125e-5f);
-      sure &= packed.x == below.x && packed.y == below.y && ss < 1e38f;
+      sure &= packed.x == below.x && packed.y == below.y && ss < 1e38f && amax * inv < 6.5f;
       if (__any_sync(0xffffffffu, in && !sure))
         packed = key_codes_f64<D, ROPE>(src + now * p.ld + (first + at) * 16, in,
                                         static_cast<double>(p.positions[t0 + now]), p.inv_freq, k_scale, s8);

@@ -140,6 +140,29 @@ def test_store(ops, status, hq, hkv, d, tokens, theta, scale):
     assert int(status) == 0
 
 
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("scale", [1e-6, 1e-3])
+def test_store_blocks_whose_scale_saturates(ops, status, d, scale):
+    """A cache scale far too small for the keys: block scales stop at 448, and what is left inside the grid has rotation
+    partners thousands of units larger, whose fp32 error reaches over a border."""
+    t, hq, hkv = 2000, 8, 8
+    g = torch.Generator(device="cuda").manual_seed(d)
+    qkv = torch.randn((t, (2 * hq + 2 * hkv) * d), generator=g, device="cuda").to(torch.bfloat16)
+    pos = torch.randint(0, 1 << 20, (t,), generator=g, device="cuda")
+    loc = torch.randperm(t, generator=g, device="cuda")
+    inv = (1e4 ** (-torch.arange(0, d, 2, device="cuda") / d)).float()
+    keys = qkv[:, hq * d:(hq + hkv) * d].view(t, hkv, d // 2, 2)      # half of the pairs nearly cancel: e cos - o sin
+    angle = pos[:, None].double() * inv.double()
+    cancel = keys[..., 0].double() * (angle.cos() / angle.sin())[:, None]
+    some = (cancel.abs() < 4) & (torch.rand(cancel.shape, generator=g, device="cuda") < 0.5)
+    keys[..., 1] = torch.where(some, cancel.to(torch.bfloat16), keys[..., 1])
+    scales = [torch.tensor(scale, device="cuda"), torch.tensor(scale, device="cuda")]
+    cache = empty_cache(t, hkv, d)
+    q = run_store(ops, qkv, pos, loc, inv, scales, cache, hq, hkv, d, status)
+    assert int(status) == 0
+    check_store(q, cache, loc, qkv, pos, inv, scales, hq, hkv, d)
+
+
 def test_store_ties_zeros_and_values_without_a_code(ops, status):
     """V is stored without a norm: exact ties, all-zero blocks, values beyond the format, infinities and NaN."""
     hq = hkv = 1
