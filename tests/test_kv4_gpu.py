@@ -383,6 +383,8 @@ def test_attention_many_workers_and_ragged_batches(ops, status, batch, ctx_hi):
     (400, 8, 2, 64, 9, 40, 0),        # one key tile each
     (3, 16, 2, 128, 16, 9000, 0),     # one pair over many blocks
     (70, 16, 4, 128, 32, 1500, 200),  # ranges that end inside pairs, a window in front
+    (4, 128, 1, 64, 1, 600, 0),       # one token fills the block of rows
+    (3, 100, 1, 128, 1, 700, 64),
 ])
 def test_attention_blocks_of_rows_share_the_key_tiles(ops, status, batch, hq, hkv, d, new_hi, ctx_hi, window):
     rng = random.Random(batch)
@@ -415,6 +417,52 @@ def test_attention_small_weights_behind_dominating_keys(ops, status, batch, new)
     others = (ctx + 1 - 8 + torch.arange(new).double()) * 1.37 * 2 ** -22
     want = (others / (8 + others)).repeat(batch)[:, None]
     assert ((got.cpu().double() - want).abs() <= want * (2 ** -8 + 2 ** -9 + 2 ** -12)).all()
+
+
+@pytest.mark.parametrize("longest", [1, 12, 90])
+def test_attention_captured_once_serves_other_lengths_beside_another_stream(ops, longest):
+    """A captured call reads its lengths on the device, and calls on two streams at once do not share a workspace."""
+    hq, hkv, d, page, batch = 8, 2, 64, 16, 6
+    rng = random.Random(longest)
+    steps = [([rng.randint(0, longest) for _ in range(batch)], [rng.randint(0, 1500) for _ in range(batch)]) for _ in range(3)]
+    table, cache = paged(rng, [longest] * batch, [1500] * batch, page, hkv, d, longest)
+    k, ks, v, vs = [c.cuda() for c in cache]
+    half = torch.tensor(0.5, device="cuda")
+    t = longest * batch
+    q = torch.randn((t, hq, d), generator=torch.Generator(device="cuda").manual_seed(1), device="cuda").to(torch.bfloat16)
+    table_gpu, ctx, cu = table.cuda(), i32([0] * batch), i32([0] * (batch + 1))
+
+    def call(ctx, cu, out):
+        ops.attention_kv4(q, k, ks.view(FP8), v, vs.view(FP8), table_gpu, ctx, cu, half, half, 0.3, batch, longest, hq, hkv,
+                          d, page, 0, out=out)
+    outs = [torch.full((t, hq * d), 7.0, dtype=torch.bfloat16, device="cuda") for _ in range(2)]
+    call(ctx, cu, outs[0])                                          # (with nothing to do)
+    torch.cuda.synchronize()
+    assert (outs[0] == 7).all()
+    graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    with torch.cuda.graph(graph):
+        call(ctx, cu, outs[0])
+    rows = [K.dequantise(cache[i], cache[i + 1], 0.5) for i in (0, 2)]
+    lengths = []
+    for new, past in steps:
+        sums = [sum(new[:b]) for b in range(batch + 1)]
+        lengths.append((i32(past), i32(sums), past, sums))
+    torch.cuda.synchronize()
+    for i, (past_gpu, sums_gpu, _, _) in enumerate(lengths):
+        ctx.copy_(past_gpu), cu.copy_(sums_gpu)
+        outs[0].fill_(7.0)
+        other = lengths[i - 1]
+        side.wait_stream(torch.cuda.current_stream())
+        for _ in range(4):
+            graph.replay()
+            with torch.cuda.stream(side):
+                call(other[0], other[1], outs[1])
+        torch.cuda.synchronize()
+        for out, (_, _, past, sums) in ((outs[0], lengths[i]), (outs[1], other)):
+            n = sums[-1]                                            # rows behind it stay as they were
+            want, bound = K.attend(q[:n].cpu(), *rows, table, past, sums, 0.3, page, 0)
+            assert ((out[:n].cpu().double() - want).abs() <= bound).all()
+        assert (outs[0][lengths[i][3][-1]:] == 7).all()
 
 
 @pytest.mark.parametrize("new", [1, 140])
