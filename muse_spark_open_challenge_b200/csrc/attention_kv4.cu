@@ -656,8 +656,11 @@ static int launch_kv4(Kv4Args a, cudaStream_t st) {
 // Query rows a CTA holds: one MMA column block of 8 where the group's rows fit, else two.
 static int kv4_row_blocks(int64_t rows) { return rows <= 8 ? 1 : 2; }
 
-// Up to this many query rows per KV head the mma.sync kernel above streams the keys once per 16 rows; beyond it the
-// tcgen05 kernel takes them 256 at a time.
+// Up to this many query rows per KV head, the two column blocks that fit its registers, the mma.sync kernel above is
+// used; beyond it the tcgen05 kernel, whose 128 rows cost the same however few are used.  8 heads x 128, this kernel
+// against tcgen05: 16 rows, 16 requests of 4096 keys 57 us against 73, 64 of 1024 51 against 123, 1 of 30000 32 against
+// 49.  Beyond 16 rows this kernel would stream the keys again for every 16: 16 requests of 4096 keys, launch included,
+// 32 rows 101 against 94, 64 rows 141 against 94 (2 requests, 32 rows: 54 against 56).
 constexpr int kKvFewRows = 16;
 
 struct Kv4Plan {

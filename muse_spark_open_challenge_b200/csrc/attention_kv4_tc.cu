@@ -1,12 +1,14 @@
 // Causal varlen attention over the paged 4-bit K/V cache, many query rows per KV head (prefill, chunks), on tcgen05.
 //
-// One CTA per (request, KV head, block of 2 * floor(128 / G) query tokens[, key slice]); two 128-row query sub-tiles
-// (rows are (token, head in group) pairs) share every K/V tile.  512 threads:
+// A block of work is (request, KV head, 2 * floor(128 / G) query tokens[, key slice]); two 128-row query sub-tiles
+// (rows are (token, head in group) pairs) share every K/V tile.  One CTA per SM takes blocks one after another; requests
+// of up to 128 rows share out all their key tiles equally instead (TcWalk below).  512 threads:
 //   warps 0-3, 4-7  softmax groups of sub-tile 0 / 1, one thread per row, as in the FP8 kernel (csrc/attention_fp8.cu):
-//                   the row of S in registers, maximum, exponentials taken in turns by the two warps of a scheduler,
-//                   P written back to tensor memory over the first 64 columns of the sub-tile's own S, in two halves.
+//                   the row of S in registers, maximum, exponentials, P written back to tensor memory over the first
+//                   64 columns of the sub-tile's own S, in two halves; arithmetic on pairs of fp32.
 //                   Before that each thread brings its query row into shared memory: scaled by a power of two to f16
-//                   (largest magnitude in [2^14, 2^15)), so that one operand type serves both products
+//                   (largest magnitude in [2^14, 2^15)), so that one operand type serves both products.  The next
+//                   block's queries come before this one's results, whose stores its first Q K^T then covers
 //   warp  8         tensor memory and tcgen05.mma issue: S_s = Q_s K^T, O_s += P_s V (kind::f16, fp32 accumulators)
 //   warps 12-15     producers: thread = key of the tile.  Codes and scales go from global memory to registers a tile
 //                   ahead, become f16 (e2m1 conversion times the block scale: exact) and are stored as K-major (K) and
@@ -16,6 +18,18 @@
 // P is f16 (half a step 2^-11) times 2^6, which with a lag of the running maximum of at most 2^8 stays below 2^15.
 // A key whose page is missing is hidden: producers leave one bit per key, and the mask pass takes it with the causal
 // limits.  Every wait is bounded.
+//
+// What bounds it: neither a pipe nor memory, but the chain S -> maximum -> exponentials -> P -> P V of each sub-tile,
+// which two of them hide only in part, and instruction fetch.  4 x 2048 causal, 32 + 8 heads x 128: tensor pipe 34 %
+// active, exponential unit 35 %, ALU 32 %, issue 38 %.  4 x 4096 (0.55 TFLOP): 646 us = 851 TFLOP/s, 711 us with the
+// norm and gate.  Without the producers' loads it takes 592 us, without their conversion 616 us.
+// Kept on the way, 4 x 4096: 1170 us -> 717 packed fp32 arithmetic, O rescaled before the exponentials, no turns at the
+// exponential unit -> 665 MMAs issued four to a block in a rolled loop (a smaller loop for the fetch) -> 651 masks by
+// bits; with the gate 832 -> 708 its division by a fast reciprocal.  753-token chunks over 80000 keys, page 1: 262 -> 230
+// persistent CTAs, page entries a tile further ahead -> 216.
+// Measured and not kept: turns at the exponential unit; a cubic in place of some exponentials (4 x 4096 767 us and more
+// against 739 then); registers 176/56/104 (722 against 710); four lanes to a row in the epilogue (755 against 655); S read
+// in pieces; separate warps for the queries; L2 prefetch of the keys two or three tiles ahead (no difference).
 #include "kv4_common.cuh"
 
 namespace msl {
