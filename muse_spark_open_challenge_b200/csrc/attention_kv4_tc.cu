@@ -22,14 +22,18 @@
 // What bounds it: neither a pipe nor memory, but the chain S -> maximum -> exponentials -> P -> P V of each sub-tile,
 // which two of them hide only in part, and instruction fetch.  4 x 2048 causal, 32 + 8 heads x 128: tensor pipe 34 %
 // active, exponential unit 35 %, ALU 32 %, issue 38 %.  4 x 4096 (0.55 TFLOP): 646 us = 851 TFLOP/s, 711 us with the
-// norm and gate.  Without the producers' loads it takes 592 us, without their conversion 616 us.
+// norm and gate.  Without the producers' loads it takes 592 us, without their conversion 616 us.  That is for scores of a
+// deviation near 1; where it is 5 the running maxima move often: 720 us, the
+// difference being the rescaling of O.
 // Kept on the way, 4 x 4096: 1170 us -> 717 packed fp32 arithmetic, O rescaled before the exponentials, no turns at the
 // exponential unit -> 665 MMAs issued four to a block in a rolled loop (a smaller loop for the fetch) -> 651 masks by
 // bits; with the gate 832 -> 708 its division by a fast reciprocal.  753-token chunks over 80000 keys, page 1: 262 -> 230
 // persistent CTAs, page entries a tile further ahead -> 216.
 // Measured and not kept: turns at the exponential unit; a cubic in place of some exponentials (4 x 4096 767 us and more
 // against 739 then); registers 176/56/104 (722 against 710); four lanes to a row in the epilogue (755 against 655); S read
-// in pieces; separate warps for the queries; L2 prefetch of the keys two or three tiles ahead (no difference).
+// in pieces; separate warps for the queries; L2 prefetch of the keys two or three tiles ahead (no difference); for wide
+// scores, O rescaled 32 columns at a time (no difference), two pieces in flight (763 against 723, registers), a lag of up
+// to 2^9.75 (3 us).
 #include "kv4_common.cuh"
 
 namespace msl {
