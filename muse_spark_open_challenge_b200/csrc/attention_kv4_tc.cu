@@ -259,7 +259,8 @@ __device__ __forceinline__ bool tc_item(const Kv4Args& p, int i, TcItem& it) {
 //   SHARED = false  block i, i + gridDim.x, ... of the list above
 //   SHARED = true   up to 128 rows a request (verify blocks): the key tiles of all requests and KV heads, laid end to
 //                   end, are cut into equal ranges, one a CTA, as in csrc/attention_kv4.cu; the two sub-tiles hold the same
-//                   rows and take the tiles of an item in turn.  16 requests x 8 tokens after 500 .. 8192: 94 us
+//                   rows and take the tiles of an item in turn.  Producers that load two tiles ahead, in registers taken
+//                   from the softmax warps (168/56/120), need 99 us for 16 x 8 x 4096 against 78.  16 requests x 8 tokens after 500 .. 8192: 94 us
 //                   against 125 with the requests' own slices.
 template <bool SHARED>
 struct TcWalk;
