@@ -79,8 +79,22 @@ def prepare(weights: dict, config: Config) -> dict:
             "status": torch.zeros(1, dtype=torch.int32, device=dev)}
 
 
+def check_caches(data: dict, config: Config) -> None:
+    """`msl_layer_prefill` takes the caches as FP8 rows by their address alone: a cache held in 4 bits, or one with
+    fewer rows than `config.cache_rows`, would be written past its end."""
+    if "k_cache_sf" in data or "v_cache_sf" in data:
+        raise MslError("the C host needs an FP8 cache, not one held in 4 bits (layer.kernel_fn takes either)")
+    need = config.cache_rows * config.hkv * config.head_dim
+    for name in ("k_cache", "v_cache"):
+        t = data[name]
+        if t.dtype != torch.float8_e4m3fn or not t.is_contiguous() or t.numel() < need:
+            raise MslError(f"{name}: expected a contiguous FP8 cache of {config.cache_rows} rows of {config.hkv} heads x "
+                           f"{config.head_dim} channels, got {t.dtype}, {tuple(t.shape)}")
+
+
 def kernel_fn(data: dict, st: dict, config: Config, fork: bool = True):
     """(hidden bf16 [T, H], stream fp32 [T, H], expert ids int32 [T, K]) through `msl_layer_prefill`."""
+    check_caches(data, config)
     lib = _lib.lib()
     dev = st["device"]
     need = lib.msl_layer_workspace_bytes(C.byref(config))

@@ -135,3 +135,29 @@ def test_synthetic_cache_has_the_documented_layout():
     assert c["v_cache_sf"].dtype == torch.float8_e4m3fn and torch.isfinite(c["v_cache_sf"].float()).all()
     v = K.dequantise(c["v_cache"], c["v_cache_sf"], 1.0)
     assert 0.5 < float(v.std()) < 2.0
+
+
+@pytest.mark.parametrize("what", ["codes with scales", "codes alone", "one cache of codes", "half a cache"])
+def test_c_host_binding_refuses_what_is_not_an_fp8_cache(what):
+    """`clayer.kernel_fn` passes addresses on: an FP8 store into 4-bit codes, or into fewer rows than the configuration
+    says, would write past the caches.  The state is empty, so anything but the refusal would be another error."""
+    from muse_spark_open_challenge_b200 import clayer, synth
+    from muse_spark_open_challenge_b200._lib import MslError
+    shape = synth.TINY
+    data = synth.make_input(shape, [3], [5], seed=1, page=16)
+    config = clayer.Config()
+    config.hkv, config.head_dim = shape.hkv, shape.head_dim
+    config.cache_rows = data["k_cache"].numel() // (shape.hkv * shape.head_dim)
+    with pytest.raises(KeyError):                    # this one is taken, as far as the empty state
+        clayer.kernel_fn(data, {}, config)
+    codes = synth.kv4_cache(shape, data["k_cache"].shape[0], 16, seed=1)
+    if what == "codes with scales":
+        data.update(codes)
+    elif what == "codes alone":
+        data["k_cache"], data["v_cache"] = codes["k_cache"], codes["v_cache"]
+    elif what == "one cache of codes":
+        data["v_cache"] = codes["v_cache"]
+    else:
+        data["v_cache"] = data["v_cache"][:data["v_cache"].shape[0] // 2]
+    with pytest.raises(MslError, match="cache"):
+        clayer.kernel_fn(data, {}, config)
