@@ -268,7 +268,7 @@ attention_kv4_kernel(Kv4Args p) {
         // 2^(141 - e) takes the exponent e to 141 = 127 + 14; its inverse goes into the row's score scale
         const int e = min(max(static_cast<int>(mx >> 7), 16), 254);
         const float up = __uint_as_float(static_cast<uint32_t>(127 + 141 - e) << 23);
-        const float down = scale_log2 / up;
+        const float down = kv4_row_scale(scale_log2, up);
 #pragma unroll
         for (int w = 0; w < KS * 2; ++w)
           qf[nb][w / 2][w & 1] = h2_bits(__floats2half2_rn(bf16_bits_to_f32(raw[w] & 0xffffu) * up,

@@ -609,7 +609,7 @@ attention_kv4_tc_kernel(Kv4Args p, int n_items) {
         for (int x = 0; x < D / 2; ++x) mx = max(mx, max(w[x] & 0x7fffu, (w[x] >> 16) & 0x7fffu));
         const int e = min(max(static_cast<int>(mx >> 7), 16), 254);
         const float up = __uint_as_float(static_cast<uint32_t>(127 + 141 - e) << 23);
-        m.scale_log2 = scale0 / up;
+        m.scale_log2 = kv4_row_scale(scale0, up);
 #pragma unroll
         for (int x = 0; x < D / 8; ++x) {
           uint32_t h[4];

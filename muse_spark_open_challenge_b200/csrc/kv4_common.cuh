@@ -60,6 +60,14 @@ __device__ __forceinline__ __half2 scales_h2(uint32_t two) {
   asm("{.reg .b16 x;\n\tcvt.u16.u32 x, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, x;}" : "=r"(h) : "r"(two));
   return __hmin2(bits_h2(h), __half2half2(__ushort_as_half(0x5F00)));   // 448
 }
+// A query row's score scale: the softmax's, in log2 units, without the power of two `up` that the row was multiplied
+// by.  It stays above zero: a hidden score is -inf, and -inf * 0 would make a row NaN.  (Only a row of nothing but tiny
+// values, whose scores weigh all keys alike, has a factor this small.)
+__device__ __forceinline__ float kv4_row_scale(float scale_log2, float up) {
+  float s = scale_log2 / up;
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(s) : "f"(1.17549435e-38f));   // (a NaN stays one)
+  return s;
+}
 // A request as the schedule sees it: q rows [begin, begin + len), `seq` cached tokens.
 struct Kv4Req {
   int begin, len, seq;

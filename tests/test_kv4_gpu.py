@@ -679,3 +679,23 @@ def test_stack_over_4_bit_caches_chains_its_layers(ops):
         layer.check_status(st)
         assert torch.equal(e, ids[i])
     assert torch.equal(h, hidden) and torch.equal(s, stream)
+
+
+# ------------------------------------------------------------------------------------------------ odd numbers
+@pytest.mark.parametrize("new", [[1, 1], [4, 2], [20, 9], [150, 150]])
+def test_attention_zero_query_rows_under_small_scales(ops, status, new):
+    """A row of zeros weighs all visible keys alike, also where softmax_scale * k_scale over the power of two that the
+    row was scaled by is below the smallest fp32 number."""
+    ctx, hq, hkv, d, page = [200, 90], 8, 2, 64, 16
+    table, cache = paged(random.Random(6), new, ctx, page, hkv, d, 6)
+    g = torch.Generator(device="cuda").manual_seed(6)
+    q = torch.randn((sum(new), hq, d), generator=g, device="cuda").to(torch.bfloat16)
+    q[0, 1] = 0
+    q[-1] = 0
+    cu = [0, new[0], sum(new)]
+    k_scale, v_scale = torch.tensor(1e-8, device="cuda"), torch.tensor(0.5, device="cuda")
+    got = run_attention(ops, q, cache, table, ctx, cu, max(new), hq, hkv, d, page, 0, 0.125, status=status,
+                        scales=(k_scale, v_scale))
+    rows = [K.dequantise(cache[i], cache[i + 1], s.cpu()) for i, s in ((0, k_scale), (2, v_scale))]
+    want, bound = K.attend(q.cpu(), *rows, table, ctx, cu, 0.125, page, 0)
+    assert ((got.cpu().double() - want).abs() <= bound).all() and int(status) == 0
