@@ -357,8 +357,9 @@ int msl_qk_rope_store_kv4(const void* qkv, int64_t ld, const int64_t* positions,
                           int64_t cache_rows, int* status, void* stream);
 
 /* Read-back: out[i, :] = the values of cache row rows[i], i < n, for rows of `width` = hkv * head_dim elements
- * (out_mode MSL_OUT_BF16 or MSL_OUT_F32; rounded once from fp32).  A negative row gives zeros; one at or beyond
- * cache_rows gives zeros and MSL_ERR_CAPACITY in *status. */
+ * (out_mode MSL_OUT_BF16 or MSL_OUT_F32; rounded once from fp32).  Scale bytes 0x7f and 0xff (NaN, never stored) read
+ * as 448, as in the attention.  A negative row gives zeros; one at or beyond cache_rows gives zeros and MSL_ERR_CAPACITY
+ * in *status. */
 int msl_kv4_rows(const void* codes, const void* scales, const float* scale, const int64_t* rows, int64_t n, int width,
                  int64_t cache_rows, int out_mode, void* out, int* status, void* stream);
 

@@ -493,7 +493,7 @@ kv4_rows_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ s
     } else if (row >= 0) {
       const int64_t at = row * blocks + x % blocks;
       w = *reinterpret_cast<const uint2*>(codes + at * 8);
-      s = e4m3_to_f32(scales[at]);
+      s = fminf(e4m3_to_f32(scales[at]), 448.f);            // the NaN codes too, as the attention reads them
     }
     // code * s is exact (2 + 4 bits), so the fp32 product with the tensor's scale rounds once
     float v[16];

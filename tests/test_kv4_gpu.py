@@ -699,3 +699,13 @@ def test_attention_zero_query_rows_under_small_scales(ops, status, new):
     rows = [K.dequantise(cache[i], cache[i + 1], s.cpu()) for i, s in ((0, k_scale), (2, v_scale))]
     want, bound = K.attend(q.cpu(), *rows, table, ctx, cu, 0.125, page, 0)
     assert ((got.cpu().double() - want).abs() <= bound).all() and int(status) == 0
+
+
+def test_rows_whose_scale_is_a_nan_code_read_as_448(ops, status):
+    """... as in the attention, which must not spread a NaN."""
+    codes, sf = empty_cache(4, 2, 64, fill=0x5A)[:2]
+    sf.fill_(0x30)
+    sf[1, 0, 2], sf[2, 1, 0], sf[3] = 0x7F, 0xFF, 0x7E
+    half = torch.tensor(0.5, device="cuda")
+    got = ops.kv4_rows(codes, sf, half, torch.arange(4, device="cuda"), dtype=torch.float32, status=status)
+    assert torch.equal(got.cpu().double(), K.dequantise(codes.cpu(), sf.cpu(), 0.5)) and int(status) == 0
