@@ -365,8 +365,8 @@ int msl_kv4_rows(const void* codes, const void* scales, const float* scale, cons
 
 /* msl_attention_fp8 over the 4-bit cache: the same masks, paging and epilogue, queries in bf16 [tokens, hq,
  * head_dim] with row pitch ld_q, any number of query heads per KV head up to 128; softmax_scale and
- * *k_scale must be positive.  max_q_len is the longest
- * request's number of new tokens (rows beyond it, and rows behind the last request, are left as they are).  A page
+ * *k_scale must be positive.  max_q_len is the longest request's number of new tokens: rows beyond it are left as
+ * they are and MSL_ERR_CAPACITY goes to *status; rows behind the last request are left as they are.  A page
  * table entry that is negative, beyond the cache or missing (past max_pages) hides its keys and is reported in
  * *status; a row that sees no key is zero.  Scale bytes 0x7f and 0xff (NaN, never stored) read as 448.  The cache
  * must hold fewer than 2^31 rows.  `workspace`: msl_attention_kv4_workspace bytes (may be 0) of caller-owned device

@@ -181,6 +181,7 @@ attention_kv4_kernel(Kv4Args p) {
   int64_t mine_all = 0, mine = 0;                           // tiles with p.heads heads a CTA, and with one
   for (int b = b0; b < b1; ++b) {
     const Kv4Req r = kv4_request(p, b);
+    if (r.over && blockIdx.x == 0) report_error(p.status, MSL_ERR_CAPACITY);
     mine_all += kv4_tiles(p, r, p.heads, p.tile_shift);
     mine += kv4_tiles(p, r, 1, kWide);
   }

@@ -13,7 +13,7 @@
 //   warps 12-15     producers: thread = key of the tile.  Codes and scales go from global memory to registers a tile
 //                   ahead, become f16 (e2m1 conversion times the block scale: exact) and are stored as K-major (K) and
 //                   N-major (V) swizzled operand tiles of a ring
-//   warps 9-11      idle: they round the warpgroup up whose registers the others use
+//   warps 9-11      round the warpgroup up whose registers the others use; warp 9 looks for requests over max_q_len
 // Registers are split 184 (softmax) / 56 / 88 (producers): 128 x (184 + 184 + 56 + 88) = 65536, the launch's total.
 // P is f16 (half a step 2^-11) times 2^6, which with a lag of the running maximum of at most 2^8 stays below 2^15.
 // A key whose page is missing is hidden: producers leave one bit per key, and the mask pass takes it with the causal
@@ -359,7 +359,10 @@ attention_kv4_tc_kernel(Kv4Args p, int n_items) {
     const int per = (p.batch + kTcThreads - 1) / kTcThreads;
     const int b0 = min(static_cast<int>(threadIdx.x) * per, p.batch), b1 = min(b0 + per, p.batch);
     int64_t mine = 0, total = 0;
-    for (int b = b0; b < b1; ++b) mine += tiles_of(b);
+    for (int b = b0; b < b1; ++b) {
+      if (blockIdx.x == 0 && kv4_request(p, b).over) report_error(p.status, MSL_ERR_CAPACITY);
+      mine += tiles_of(b);
+    }
     int64_t inc = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -541,6 +544,9 @@ attention_kv4_tc_kernel(Kv4Args p, int n_items) {
         done1 += it.n_sub[1];
       }
       if (!ok && lane == 0) { *abort_flag = 1; report_error(p.status, MSL_ERR_DEVICE_TIMEOUT); }
+    } else if (!SHARED && warp == 9 && blockIdx.x == 0) {
+      for (int b = lane; b < p.batch; b += 32)
+        if (kv4_request(p, b).over) report_error(p.status, MSL_ERR_CAPACITY);
     }
   } else {
     // ------------------------------------------------------------------ softmax / correction / epilogue

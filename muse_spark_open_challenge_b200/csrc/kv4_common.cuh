@@ -71,12 +71,14 @@ __device__ __forceinline__ float kv4_row_scale(float scale_log2, float up) {
 // A request as the schedule sees it: q rows [begin, begin + len), `seq` cached tokens.
 struct Kv4Req {
   int begin, len, seq;
+  bool over;                    // has rows past max_q_len, which nothing writes
 };
 __device__ __forceinline__ Kv4Req kv4_request(const Kv4Args& p, int b) {
   Kv4Req r;
   r.begin = max(0, min(p.cu_seqlens_q[b], p.tokens));
   const int end = max(r.begin, min(p.cu_seqlens_q[b + 1], p.tokens));
   r.len = min(end - r.begin, p.max_q_len);
+  r.over = end - r.begin > p.max_q_len;
   r.seq = p.seq_lens[b];
   return r;
 }

@@ -498,8 +498,8 @@ def _attention_kv4_workspace(index, *sizes):
 def attention_kv4(q, k_cache, k_sf, v_cache, v_sf, page_table, seq_lens, cu_seqlens_q, k_scale, v_scale, softmax_scale,
                   batch, max_q_len, hq, hkv, head_dim, page_size, window, gate=None, out=None, status=None):
     """`attention` over the 4-bit cache: q bf16 [T, hq, head_dim] (`qk_rope_store_kv4`'s; the heads of a token must be
-    contiguous), result bf16 [T, hq * head_dim].  Rows behind the last request are left as they are (undefined when
-    `out` is not given); a row that sees no key is zero."""
+    contiguous), result bf16 [T, hq * head_dim].  Rows behind the last request, and a request's rows from `max_q_len` on
+    (reported in `status`), are left as they are (undefined when `out` is not given); a row that sees no key is zero."""
     index = q.get_device()
     if not (0 <= index == k_cache.get_device() == k_sf.get_device() == v_cache.get_device() == v_sf.get_device() ==
             page_table.get_device() == seq_lens.get_device() == cu_seqlens_q.get_device() == k_scale.get_device() ==

@@ -709,3 +709,25 @@ def test_rows_whose_scale_is_a_nan_code_read_as_448(ops, status):
     half = torch.tensor(0.5, device="cuda")
     got = ops.kv4_rows(codes, sf, half, torch.arange(4, device="cuda"), dtype=torch.float32, status=status)
     assert torch.equal(got.cpu().double(), K.dequantise(codes.cpu(), sf.cpu(), 0.5)) and int(status) == 0
+
+
+@pytest.mark.parametrize("new,longest", [([3, 1], 2), ([1, 9], 8), ([2, 150, 20], 140)])
+def test_attention_reports_a_request_longer_than_max_q_len(ops, status, new, longest):
+    """Rows up to max_q_len are right, the ones behind them are left as they are, and the status says so."""
+    ctx, hq, hkv, d, page = [40, 200, 7][:len(new)], 8, 2, 64, 16
+    table, cache = paged(random.Random(8), new, ctx, page, hkv, d, 8)
+    t = sum(new)
+    q = torch.randn((t, hq, d), generator=torch.Generator(device="cuda").manual_seed(8), device="cuda").to(torch.bfloat16)
+    cu = [sum(new[:b]) for b in range(len(new) + 1)]
+    out = torch.full((t, hq * d), 7.0, dtype=torch.bfloat16, device="cuda")
+    run_attention(ops, q, cache, table, ctx, cu, longest, hq, hkv, d, page, 0, 0.3, out=out, status=status)
+    assert int(status) == -6
+    rows = [K.dequantise(cache[i], cache[i + 1], 0.5) for i in (0, 2)]
+    want, bound = K.attend(q.cpu(), *rows, table, ctx, cu, 0.3, page, 0)
+    for b, n in enumerate(new):
+        at = slice(cu[b], cu[b] + min(n, longest))
+        assert ((out[at].cpu().double() - want[at]).abs() <= bound[at]).all()
+        assert (out[at.stop:cu[b + 1]] == 7).all()
+    status.zero_()
+    run_attention(ops, q, cache, table, ctx, cu, max(new), hq, hkv, d, page, 0, 0.3, out=out, status=status)
+    assert int(status) == 0
