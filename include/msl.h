@@ -344,8 +344,12 @@ int msl_page_plan(const int* new_lens, const int* seq_lens, int* page_table, int
                   int n_free, const int* free_head, int* free_head_out, int batch, int page_size, int tokens,
                   int* cu_seqlens_q, int64_t* positions, int64_t* cache_loc, int* status, void* stream);
 
-/* msl_qk_rope_store for the 4-bit cache: the same norm and rotation of q and k; q -> bf16 [tokens, hq, head_dim];
- * k and v -> codes and scales of row cache_loc[t].  For each block of 16
+/* msl_qk_rope_store for the 4-bit cache: the same norm, pairs and direction of rotation of q and k, but not the same
+ * rounding of the angle.  Here positions[t] * inv_freq[i] is a 64-bit product; there, as in the reference
+ * (reference.py:329-336), an fp32 one, off by up to 2^-24 of the angle: 0.0005 rad below position 16384, 0.004 at 100000.
+ * Within a cache queries and keys are turned alike, but q and k of the two stores are that far apart, and a key's code
+ * next to a border may differ.  q -> bf16 [tokens, hq, head_dim]; k and v -> codes and scales of row cache_loc[t].  For
+ * each block of 16
  *   s = e4m3(min(448, max|z| / (6 * scale))),  c = e2m1(z / (s * scale)),
  * to nearest, ties to even, decided on values held in 64 bits; a block whose s is 0 gets zero codes.  Infinities and
  * NaN of k and v have no code: they count as +-2^128 or a little above and saturate.  A negative cache_loc marks a

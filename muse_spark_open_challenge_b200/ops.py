@@ -434,8 +434,9 @@ def page_plan(new_lens, seq_lens, page_table, free_pages, free_head, page_size, 
 def qk_rope_store_kv4(qkv, positions, cache_loc, inv_freq, k_scale, v_scale, k_cache, k_sf, v_cache, v_sf, hq, hkv,
                       head_dim, status=None):
     """`qk_rope_store` for the 4-bit cache: returns q bf16 [T, hq, head_dim] and writes the new K/V rows as codes
-    (u8 [..., hkv, head_dim / 2]) and block scales (e4m3 [..., hkv, head_dim / 16]).  A negative cache_loc marks a padding
-    token, which is not stored."""
+    (u8 [..., hkv, head_dim / 2]) and block scales (e4m3 [..., hkv, head_dim / 16]).  The angle of the rotation is a
+    64-bit product, not `qk_rope_store`'s fp32 one (up to 2^-24 of it apart).  A negative cache_loc marks a padding token,
+    which is not stored."""
     index = qkv.get_device()
     if not (0 <= index == positions.get_device() == cache_loc.get_device() == k_scale.get_device() ==
             v_scale.get_device() == k_cache.get_device() == k_sf.get_device() == v_cache.get_device() ==

@@ -731,3 +731,26 @@ def test_attention_reports_a_request_longer_than_max_q_len(ops, status, new, lon
     status.zero_()
     run_attention(ops, q, cache, table, ctx, cu, max(new), hq, hkv, d, page, 0, 0.3, out=out, status=status)
     assert int(status) == 0
+
+
+@pytest.mark.parametrize("hq,hkv,d", [(8, 2, 64), (4, 4, 128)])
+@pytest.mark.parametrize("far", [0, 900, 1 << 18])
+def test_store_turns_queries_as_the_fp8_store_does(ops, status, hq, hkv, d, far):
+    """The two stores agree on norm, pairs and direction; the angle is an fp32 product in the FP8 one (off by half a step,
+    2^-24 of it) and a 64-bit one here.  Beside that: half an E4M3 step (2^-4, or 2^-10 among the subnormals) and half a
+    bf16 one, and 2^-19 of the pair for the norms, sines and cosines formed in fp32 on both sides."""
+    t = 60
+    g = torch.Generator(device="cuda").manual_seed(far + d)
+    qkv = torch.randn((t, (hq + 2 * hkv) * d), generator=g, device="cuda").to(torch.bfloat16)
+    pos = torch.randint(0, far + 1, (t,), generator=g, device="cuda")
+    loc = torch.arange(t, device="cuda")
+    inv = (1e4 ** (-torch.arange(0, d, 2, device="cuda") / d)).float()
+    one = torch.ones((), device="cuda")
+    k, v = (torch.zeros((t, hkv, d), device="cuda").to(FP8) for _ in range(2))
+    theirs = ops.qk_rope_store(qkv, pos, loc, inv, one, one, k, v, hq, hkv, d, status=status).double()
+    mine = run_store(ops, qkv, pos, loc, inv, [one, one], empty_cache(t, hkv, d), hq, hkv, d, status).double()
+    pair = mine.view(t, hq, d // 2, 2).norm(dim=-1)
+    turn = (pos.double()[:, None] * inv.double() * 2 ** -24).unsqueeze(1)
+    slack = (pair * (turn + 2 ** -19 + 2 ** -8)).repeat_interleave(2, -1)
+    bound = slack + (mine.abs() + slack) * 2 ** -4 + 2 ** -10
+    assert ((mine - theirs).abs() <= bound).all() and int(status) == 0
