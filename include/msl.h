@@ -352,9 +352,11 @@ int msl_page_plan(const int* new_lens, const int* seq_lens, int* page_table, int
  * each block of 16
  *   s = e4m3(min(448, max|z| / (6 * scale))),  c = e2m1(z / (s * scale)),
  * to nearest, ties to even, decided on values held in 64 bits; a block whose s is 0 gets zero codes.  Infinities and
- * NaN of k and v have no code: they count as +-2^128 or a little above and saturate.  A negative cache_loc marks a
- * padding token (nothing is stored, nothing reported); one at or beyond cache_rows is skipped and reported in
- * *status.  No two tokens may share a row.  head_dim 64 or 128. */
+ * NaN of k and v have no code: in k they count as +-2^128 or a little above, in v as the largest finite bf16, and
+ * saturate.  *k_scale and *v_scale lie between 2^-100 and 2^100.  A query's norm is formed in fp32, as in
+ * msl_qk_rope_store: its elements stay below 2^60.  A negative cache_loc marks a padding token (nothing is stored,
+ * nothing reported); one at or beyond cache_rows is skipped and reported in *status.  No two tokens may share a row.
+ * head_dim 64 or 128. */
 int msl_qk_rope_store_kv4(const void* qkv, int64_t ld, const int64_t* positions, const int64_t* cache_loc,
                           const float* inv_freq, const float* k_scale, const float* v_scale, void* q, void* k_cache,
                           void* k_sf, void* v_cache, void* v_sf, int tokens, int hq, int hkv, int head_dim,

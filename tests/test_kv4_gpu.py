@@ -754,3 +754,24 @@ def test_store_turns_queries_as_the_fp8_store_does(ops, status, hq, hkv, d, far)
     slack = (pair * (turn + 2 ** -19 + 2 ** -8)).repeat_interleave(2, -1)
     bound = slack + (mine.abs() + slack) * 2 ** -4 + 2 ** -10
     assert ((mine - theirs).abs() <= bound).all() and int(status) == 0
+
+
+@pytest.mark.parametrize("power", [-100, -8, 100])
+def test_store_values_and_scale_times_a_power_of_two(ops, status, power):
+    """V and its scale times the same power of two have the same codes and block scales, to the ends of the range that
+    the interface gives for scales; with a single one they saturate or vanish."""
+    t, hq, hkv, d = 50, 2, 2, 64
+    g = torch.Generator(device="cuda").manual_seed(3)
+    qkv = torch.randn((t, (2 * hq + 2 * hkv) * d), generator=g, device="cuda").to(torch.bfloat16)
+    qkv[3, (hq + hkv) * d:] = 0
+    loc = torch.arange(t, device="cuda")
+    one, scale = torch.ones((), device="cuda"), torch.tensor(2.0 ** power, device="cuda")
+    far = qkv.clone()
+    far[:, (hq + hkv) * d:] *= 2.0 ** power
+    first, second = empty_cache(t, hkv, d), empty_cache(t, hkv, d)
+    run_store(ops, qkv, loc, loc, None, [one, one], first, hq, hkv, d, status)
+    run_store(ops, far, loc, loc, None, [scale, scale], second, hq, hkv, d, status)
+    assert torch.equal(first[2], second[2]) and torch.equal(first[3], second[3]) and int(status) == 0
+    _, keys, _ = K.store(qkv.cpu(), loc.cpu(), None, hq, hkv, d)
+    want = K.quantise(keys, 2.0 ** power)
+    assert torch.equal(second[0].cpu(), want[0]) and torch.equal(second[1].cpu(), want[1].view(torch.uint8))
