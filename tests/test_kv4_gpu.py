@@ -775,3 +775,57 @@ def test_store_values_and_scale_times_a_power_of_two(ops, status, power):
     _, keys, _ = K.store(qkv.cpu(), loc.cpu(), None, hq, hkv, d)
     want = K.quantise(keys, 2.0 ** power)
     assert torch.equal(second[0].cpu(), want[0]) and torch.equal(second[1].cpu(), want[1].view(torch.uint8))
+
+
+def test_captured_step_that_moves_its_lengths_on(ops, status):
+    """A decode step captured once, with the free list's head and the cached lengths moved on at its end, replayed for one
+    token after another: pages, slots and lengths are those of the steps one by one, and every step's attention is right."""
+    hq, hkv, d, page, batch = 8, 2, 64, 4, 3
+    seq, new = [5, 0, 8], [1, 1, 0]
+    table = [[7, 3, -1, -1, -1], [-1] * 5, [0, 11, -1, -1, -1]]
+    free, head = [9, 2, 10, 1, 8, 4, 6, 5], 0
+    g = torch.Generator(device="cuda").manual_seed(12)
+    steps = torch.randn((7, 3, (hq + 2 * hkv) * d), generator=g, device="cuda").to(torch.bfloat16)
+    half = torch.tensor(0.5, device="cuda")
+    cache = empty_cache(12 * page, hkv, d, fill=0)
+    for c, fill in zip(cache, (0x31, 0x38, 0x52, 0x30)):
+        c.fill_(fill)
+    k, ks, v, vs = cache
+    kv = (k, ks.view(FP8), v, vs.view(FP8))
+    dev = {"new": i32(new), "seq": i32(seq), "table": i32(table), "free": i32(free), "head": i32([head]), "qkv": steps[0].clone()}
+
+    def step():
+        cu, pos, loc, after = ops.page_plan(dev["new"], dev["seq"], dev["table"], dev["free"], dev["head"], page, 3,
+                                            status=status)
+        q = ops.qk_rope_store_kv4(dev["qkv"], pos, loc, None, half, half, *kv, hq, hkv, d, status=status)
+        out = ops.attention_kv4(q, *kv, dev["table"], dev["seq"], cu, half, half, 0.3, batch, 1, hq, hkv, d, page, 0,
+                                status=status)
+        dev["head"].copy_(after)
+        dev["seq"].add_(dev["new"])
+        return q, out
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    start = {n: x.clone() for n, x in dev.items()}
+    before = [c.clone() for c in cache]
+    with torch.cuda.stream(side):                             # a first call outside the capture, taken back
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    for n, x in start.items():
+        dev[n].copy_(x)
+    for c, b in zip(cache, before):
+        c.copy_(b)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        q, out = step()
+    for qkv in steps:
+        dev["qkv"].copy_(qkv)
+        graph.replay()
+        table, cu, _, loc, head, bad = K.plan(new, seq, table, free, head, page, 3)
+        rows = [K.dequantise(cache[i].cpu(), cache[i + 1].cpu(), 0.5) for i in (0, 2)]
+        want, bound = K.attend(q.cpu()[:2], *rows, torch.tensor(table), seq, cu, 0.3, page, 0)
+        assert ((out[:2].cpu().double() - want).abs() <= bound).all()
+        seq = [c + n for c, n in zip(seq, new)]
+        assert not bad and dev["table"].tolist() == table and dev["seq"].tolist() == seq and dev["head"].tolist() == [head]
+        check_store(q[:2], cache, torch.tensor(loc[:2], device="cuda"), qkv[:2], torch.zeros(2), None, (half, half), hq, hkv, d)
+    assert head == 3 and int(status) == 0
