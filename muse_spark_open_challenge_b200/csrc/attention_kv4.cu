@@ -21,10 +21,15 @@
 // element within 2^28 of the row's largest.  P is f16 (half a step 2^-11) times 2^6, which keeps the weights of a long
 // context behind one dominating key out of f16's subnormals down to 2^-20; statistics and O are fp32.
 //
-// What bounds it: issue slots.  64 requests x 8192 keys, 8 heads x 128 (604 MB): 146 us = 4.1 TB/s of the measured 6.55
-// with DRAM traffic equal to the bytes needed; 720 warp instructions per 32 keys (640 of them converting and scaling
-// 8192 elements), 0.6 issued per cycle and scheduler, ALU half busy.  On the way: codes straight from global memory into
+// What bounds it: the chain of a warp's step (copies, conversion, MMA, maximum, exponentials, MMA), which four warps a
+// scheduler cover in part; no unit is at its limit.  64 requests x 4096 keys, 8 heads x 128: 0.59 instructions issued per
+// cycle and scheduler, ALU 50 % and DRAM 44 % busy, 718 warp instructions per 32 keys of a head; for each one issued, 1.1
+// warps wait out a fixed latency, 0.9 for a math pipe and 0.9 for memory.  64 requests x 8192 keys (604 MB): 146 us = 4.1 TB/s
+// of the measured 6.55, with DRAM traffic equal to the bytes needed.  On the way: codes straight from global memory into
 // registers 330 us (one ragged batch), the ring 263 us, the heads of a cache row fetched together 171 us.
+//
+// The ranges follow from the sum of all lengths, so where a request is cut, whether heads are taken together, and with
+// that the order of its sums and its last bits, depend on the rest of its batch.  The same call gives the same bits.
 #include "kv4_common.cuh"
 
 namespace msl {
@@ -41,8 +46,8 @@ __device__ __forceinline__ int64_t kv4_tiles(const Kv4Args& p, const Kv4Req& r, 
 // A CTA takes p.heads KV heads of 32 W / p.heads keys at once where every worker has at least kKvLong tiles (below), and
 // one head of 32 W keys otherwise: the heads of a cache row lie side by side, so taking them together fetches whole rows
 // (a 64-byte piece of one costs as much DRAM time as 128 bytes), but it also leaves p.heads times as many partial
-// results per item to join, which a short step cannot hide.  64 requests x 8192 keys, 8 heads: 291 -> 174 us with all
-// heads at once; 1 x 4096: 18 -> 40 us.
+// results per item to join, which a short step cannot hide.  When the choice was made, 64 requests x 8192 keys, 8 heads:
+// 291 -> 174 us with all heads at once (146 since); 1 x 4096: 18 -> 40 us.
 constexpr int kKvLong = 8;
 
 __device__ __forceinline__ void mma_16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,

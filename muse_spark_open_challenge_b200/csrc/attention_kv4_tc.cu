@@ -21,11 +21,13 @@
 //
 // What bounds it: neither a pipe nor memory, but the chain S -> maximum -> exponentials -> P -> P V of each sub-tile,
 // which two of them hide only in part, and instruction fetch.  4 x 2048 causal, 32 + 8 heads x 128: tensor pipe 34 %
-// active, exponential unit 35 %, ALU 32 %, issue 38 %.  4 x 4096 (0.55 TFLOP): 646 us = 851 TFLOP/s, 711 us with the
-// norm and gate.  Without the producers' loads it takes 592 us, without their conversion 616 us.  That is for scores of a
-// deviation near 1; where it is 5 the running maxima move often: 720 us, the
-// difference being the rescaling of O.
-// Kept on the way, 4 x 4096: 1170 us -> 717 packed fp32 arithmetic, O rescaled before the exponentials, no turns at the
+// active, exponential unit 35 %, ALU 32 %, issue 38 %.  4 x 4096 (0.55 TFLOP) as the layer calls it, scores of a
+// deviation near 5 and the norm and gate: 787 us = 699 TFLOP/s.  Where the scores are that wide the running maxima move
+// often, and O is rescaled: without the gate 730 us, against 650 for scores of a deviation near 1 (715 with the gate; 592
+// without the producers' loads, 616 without their conversion).
+// Registers are short: at 128 a thread at launch the compiler spills 92 bytes of stores and 136 of loads (head_dim 128),
+// 48 and 60 (head_dim 64), and 196 and 300 (196 and 296) where ranges are shared.
+// Kept on the way, 4 x 4096, narrow scores: 1170 us -> 717 packed fp32 arithmetic, O rescaled before the exponentials, no turns at the
 // exponential unit -> 665 MMAs issued four to a block in a rolled loop (a smaller loop for the fetch) -> 651 masks by
 // bits; with the gate 832 -> 708 its division by a fast reciprocal.  753-token chunks over 80000 keys, page 1: 262 -> 230
 // persistent CTAs, page entries a tile further ahead -> 216.

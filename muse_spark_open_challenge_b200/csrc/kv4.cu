@@ -137,7 +137,11 @@ __global__ void __launch_bounds__(kPlanThreads) page_plan_kernel(PlanArgs p) {
 // exact in fp32) by doing its heads again in 64 bits, which one warp in a hundred has to.
 // What it is bound by is issue slots, then HBM: 16384 tokens of 32 + 8 + 8 heads x 128 (354 MB) took 190 us with
 // everything in 64 bits, 116 with the queries in fp32, 100 with the keys' proposal in fp32, 85 with a block of 16
-// channels a lane (4.2 TB/s of the measured 6.55).
+// channels a lane (4.2 TB/s of the measured 6.55).  Counted: 0.75 instructions issued per cycle and scheduler with two
+// more warps ready for each one, DRAM 48 % busy, ALU 46 %.  64 registers for four blocks an SM cost 24 to 32 bytes of spill
+// stores a thread (up to 60 in key_codes_f64).
+// A key channel that is exactly zero, or a block of keys whose scale is below 2^-6 (a row of zeros, so a padding token), takes the 64-bit way
+// too, and the whole warp with it.
 constexpr int kStoreThreads = 256, kStoreWarps = kStoreThreads / 32;
 constexpr int kStoreTok = 4;               // most tokens of a block
 
@@ -181,7 +185,8 @@ __device__ __forceinline__ uint2 e2m1_of_16(const float (&u)[16], float f) {
   for (int i = 0; i < 16; ++i) v[i] = fmaf(u[i], f, 0.0f);
   return make_uint2(e2m1_pack(v), e2m1_pack(v + 8));
 }
-// ... with the magnitude moved up or down by `nudge` (a zero keeps code 0 when it is moved up).
+// ... with the magnitude moved up or down by `nudge`.  A value within it of zero changes its sign when it is moved down,
+// and a zero does in one of the two (-0 when it is moved up): the codes then differ and 64 bits decide.
 template <bool UP>
 __device__ __forceinline__ uint2 e2m1_of_16(const float (&u)[16], float f, float nudge) {
   float v[16];

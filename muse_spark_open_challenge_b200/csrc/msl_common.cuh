@@ -226,6 +226,7 @@ __device__ __forceinline__ void tc_mma_f8_ts_if(uint32_t on, uint32_t d_tmem, ui
       ::"r"(d_tmem), "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(on)
       : "memory");
 }
+
 // 4 x 4 transpose of 32-byte units among the four lanes of a quad (lanes 4k .. 4k + 3).  Lane q gives the
 // four units u[8 j .. 8 j + 7] (j = 0..3) of ITS row and ends with unit q of the quad's four rows in
 // f[8 j .. 8 j + 7] (row j of the quad).  With a lane per row, four lanes can then write 128 contiguous bytes
