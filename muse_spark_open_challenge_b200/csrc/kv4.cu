@@ -140,8 +140,8 @@ __global__ void __launch_bounds__(kPlanThreads) page_plan_kernel(PlanArgs p) {
 // channels a lane (4.2 TB/s of the measured 6.55).  Counted: 0.75 instructions issued per cycle and scheduler with two
 // more warps ready for each one, DRAM 48 % busy, ALU 46 %.  64 registers for four blocks an SM cost 24 to 32 bytes of spill
 // stores a thread (up to 60 in key_codes_f64).
-// A key channel that is exactly zero, or a block of keys whose scale is below 2^-6 (a row of zeros, so a padding token), takes the 64-bit way
-// too, and the whole warp with it.
+// A key channel that is exactly zero, or a block of keys whose scale is below 2^-6 (a row of zeros, so a padding token),
+// takes the 64-bit way too, and the whole warp with it.
 constexpr int kStoreThreads = 256, kStoreWarps = kStoreThreads / 32;
 constexpr int kStoreTok = 4;               // most tokens of a block
 
