@@ -376,7 +376,7 @@ int msl_kv4_rows(const void* codes, const void* scales, const float* scale, cons
  * table entry that is negative, beyond the cache or missing (past max_pages) hides its keys and is reported in
  * *status; a row that sees no key is zero.  Up to 128 query rows per KV head the keys of the whole batch are cut into
  * equal shares, so the order of a request's sums, and with it its last bits, depends on the lengths of the others (the
- * same call gives the same bits); beyond that it depends on the sizes alone.  Scale bytes 0x7f and 0xff (NaN, never stored) read as 448.  The cache
+ * same call gives the same bits); beyond that it depends on its own lengths and the sizes.  Scale bytes 0x7f and 0xff (NaN, never stored) read as 448.  The cache
  * must hold fewer than 2^31 rows.  `workspace`: msl_attention_kv4_workspace bytes (may be 0) of caller-owned device
  * memory, 16-byte aligned, no initialisation; calls that overlap on the GPU need one each. */
 int64_t msl_attention_kv4_workspace(int batch, int max_q_len, int tokens, int hq, int hkv, int head_dim, int max_pages,
